@@ -560,6 +560,155 @@ int ncm_ncm_forward_f32_dev(ncm_ctx_t* ctx, const ncm_ncm_shape_t* shape,
                             const float* target_inputs, const float* cosine, const float* sine,
                             float* output, float* hidden_states);
 
+/* ---- continuing a sequence: rotary positions, paged K/V cache, logits ---- */
+
+/* Pairs that a rotation turns: p and rot_dim / 2 + p of a head, or 2 p and
+ * 2 p + 1. */
+enum { NCM_ROPE_HALF = 0, NCM_ROPE_INTERLEAVED = 1 };
+
+/* Rotation of every head of every row at given positions: with a = positions
+ * [row] * inv_freq[p] (the product in 64 bits, so far positions keep their
+ * angle), c = scale cos a and s = scale sin a, pair p of a head (x, y) becomes
+ * (x c - y s, y c + x s) in fp32, rounded once. No counterpart in the
+ * reference, whose rotate_head (packages/kernels/root.zig:615-634, here
+ * ncm_rope_rotate_dev) takes tables and rounds each bf16 operation. x, y:
+ * [rows, stride], `heads` heads of head_dim values from column 0, float
+ * (dtype NCM_OUT_F32) or bf16 bits (NCM_OUT_BF16); y may be x, and must not
+ * overlap it otherwise. Values of a head behind rot_dim are copied.
+ * positions: int32 [rows], of either sign; inv_freq: float [rot_dim / 2].
+ * rot_dim even, 0 < rot_dim <= head_dim. Any stride and alignment; the
+ * 16-byte path needs 16-byte aligned x, y, rows and heads. Device pointers. */
+int ncm_rope_positions_dev(ncm_ctx_t* ctx, const void* x, void* y, const int32_t* positions,
+                           const float* inv_freq, int64_t rows, int heads, int head_dim,
+                           int rot_dim, int64_t x_stride, int64_t y_stride, int layout,
+                           float scale, int dtype);
+
+/* What a cache holds of a value. FP8: e4m3 codes (no infinities, largest 448)
+ * and per token and head a scale 2^e, the smallest with max |x| <= 448 * 2^e
+ * (e at least -126). INT8: codes rint(x * 127 / max |x|) and the scale
+ * max |x| / 127. A head of a token that holds a NaN or an infinity gets the
+ * scale NaN and codes 0: it reads back as NaN. */
+enum { NCM_KV_BF16 = 0, NCM_KV_FP8 = 1, NCM_KV_INT8 = 2 };
+
+/* A paged K/V cache on the device: pages of page_size tokens (a power of two,
+ * 16 .. 1024), k and v [pages][kv_heads][page_size][head_dim] codes, k_scale
+ * and v_scale [pages][kv_heads][page_size] (both NULL for NCM_KV_BF16). The
+ * strides count elements from a page to the next (at least a page's size; the
+ * cache may be one layer's part of a larger buffer). head_dim 64 or 128; k, v
+ * and their pages 16-byte aligned, the scales 16-byte aligned with strides of
+ * a multiple of 4. */
+typedef struct ncm_kv_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t k_scale_stride;
+    int64_t v_scale_stride;
+    int64_t pages;
+    int32_t kv_heads;
+    int32_t page_size;
+    int32_t head_dim;
+    int32_t codes;      /* NCM_KV_* */
+} ncm_kv_cache_t;
+
+/* The requests of one step. Request r's new rows are offsets[r] ..
+ * offsets[r + 1] - 1 of the `rows` rows of the step's tensors; its row i is
+ * token starts[r] + i of its sequence, which lies in page
+ * page_table[r * table_stride + token / page_size] (table_width entries a
+ * request) at token % page_size. Device int32 arrays, read on the stream, so
+ * a captured step follows what they hold at replay. Offsets are clamped to
+ * [0, rows] and starts to >= 0; a token past the table or in a page outside
+ * [0, pages) is not there: a write leaves it out, a read gives zeros, the
+ * attention does not see it. Rows of no request are left as they were. */
+typedef struct ncm_kv_batch {
+    const int32_t* offsets;     /* [requests + 1] */
+    const int32_t* starts;      /* [requests] */
+    const int32_t* page_table;  /* [requests][table_stride] */
+    int64_t requests;
+    int64_t rows;
+    int64_t table_width;
+    int64_t table_stride;
+} ncm_kv_batch_t;
+
+/* Writes the K and V rows of a step into the cache, quantised. k, v: bf16
+ * bits [rows, stride], kv_heads heads from column 0; strides multiples of 8,
+ * 16-byte aligned. Two rows that name the same place leave either's value
+ * there. Device pointers. */
+int ncm_kv_write_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                     const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride);
+
+/* Reads the tokens of a step back: code * scale, rounded to bf16, into rows
+ * of k and v laid out as ncm_kv_write_dev takes them. */
+int ncm_kv_read_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                    uint16_t* k, uint16_t* v, int64_t k_stride, int64_t v_stride);
+
+/* Attention of a step's rows over the cache, which holds their K and V
+ * already (ncm_kv_write_dev): out = softmax(scale q.k) v over the tokens that
+ * a row sees, in fp32 with one rounding to bf16 (the probabilities enter the
+ * MFMA as bf16). Row i of request r, c = starts[r], sees
+ *   the tokens before c, with window > 0 only those > p - window, where p =
+ *   positions[row], or c + i where positions is NULL (a position below c
+ *   counts as c);
+ *   the request's new token c + j where bit j % 64 of tree_mask[row][j / 64]
+ *   is set, or, where tree_mask is NULL, with j <= i and in the window too.
+ * A row that sees nothing gets zeros, and a value that a row does not see
+ * does not reach it, not even an infinity or a NaN. q: bf16 bits [rows,
+ * q_stride], query head h at column h * head_dim reading K/V head h /
+ * (q_heads / kv_heads); out: bf16 bits [rows, out_stride]. Strides multiples
+ * of 8, 16-byte aligned. tree_mask: uint64 [rows, mask_words]; new tokens past
+ * 64 * mask_words are not seen. workspace: at least the bytes that
+ * ncm_kv_attention_workspace gives for the same cache, batch and q_heads,
+ * 16-byte aligned; the call leaves nothing there that a later one needs, and
+ * no two calls that may run at once can share it. Device pointers. */
+int ncm_kv_attention_workspace(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                               int q_heads, size_t* bytes);
+int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
+                         const ncm_kv_batch_t* batch, const uint16_t* q, uint16_t* out,
+                         int q_heads, int64_t q_stride, int64_t out_stride, float scale,
+                         int64_t window, const int32_t* positions, const uint64_t* tree_mask,
+                         int64_t mask_words, void* workspace, size_t workspace_bytes);
+
+/* Rules on logits; every pointer may be NULL (its rule is off), device memory.
+ * Request r's rows are offsets[r] .. offsets[r + 1] - 1; offsets NULL: row r
+ * is request r's. For token t of a row, count is how often t stands in
+ * history[r][prompt_lens[r] .. history_lens[r]) and on the row's drafted path
+ * (draft_tokens of the request's rows j whose bit is set in the row's
+ * tree_mask; tree_mask NULL: rows up to and including its own), and t is seen
+ * when count > 0 or it stands in history[r][0 .. prompt_lens[r]). In fp32:
+ *   seen:  x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   x = x - frequency[r] * count, then x = x - presence[r] where count > 0
+ *   x = x + (the sum, in list order, of bias_values[r][e] with bias_ids[r][e] == t)
+ *   bit t % 32 of allowed[row][t / 32] clear: x = -infinity
+ * and one rounding. Ids outside [0, vocab) are ignored; lengths are clamped
+ * to [0, history_width]. */
+typedef struct ncm_logit_rules {
+    const int32_t* offsets;       /* [requests + 1] */
+    const int32_t* history;       /* [requests][history_width] */
+    const int32_t* prompt_lens;   /* [requests]; NULL: 0 */
+    const int32_t* history_lens;  /* [requests]; NULL: history_width */
+    const float* repetition;      /* [requests] */
+    const float* frequency;       /* [requests] */
+    const float* presence;        /* [requests] */
+    const int32_t* bias_ids;      /* [requests][bias_count] */
+    const float* bias_values;     /* [requests][bias_count] */
+    const uint32_t* allowed;      /* [rows][(vocab + 31) / 32] */
+    const int32_t* draft_tokens;  /* [rows]; needs offsets */
+    const uint64_t* tree_mask;    /* [rows][mask_words] */
+    int64_t requests;
+    int64_t history_width;
+    int64_t bias_count;
+    int64_t mask_words;
+} ncm_logit_rules_t;
+
+/* out = the rules applied to logits: float (dtype NCM_OUT_F32) or bf16 bits
+ * (NCM_OUT_BF16) [rows, stride]; out may be logits, and must not overlap them
+ * otherwise. Rows of no request are left as they were. */
+int ncm_adjust_logits_dev(ncm_ctx_t* ctx, const ncm_logit_rules_t* rules, const void* logits,
+                          void* out, int64_t rows, int64_t vocab, int64_t in_stride,
+                          int64_t out_stride, int dtype);
+
 /* ---- multiscale residual vector quantization ---- */
 
 /* csq[l * v + k] = squared norm of codebook row (l, k), in the fixed fp32

@@ -68,6 +68,14 @@ SIGNATURES = [
     ("ncm_decoder_forward_f32_dev", i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, vp, vp]),
     ("ncm_ncm_forward_dev", i32, [vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp]),
     ("ncm_ncm_forward_f32_dev", i32, [vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp]),
+    ("ncm_rope_positions_dev", i32, [vp, vp, vp, vp, vp, i64, i32, i32, i32, i64, i64, i32,
+                                     C.c_float, i32]),
+    ("ncm_kv_write_dev", i32, [vp, vp, vp, vp, vp, i64, i64]),
+    ("ncm_kv_read_dev", i32, [vp, vp, vp, vp, vp, i64, i64]),
+    ("ncm_kv_attention_workspace", i32, [vp, vp, i32, C.POINTER(sz)]),
+    ("ncm_kv_attention_dev", i32, [vp, vp, vp, vp, vp, i32, i64, i64, C.c_float, i64, vp, vp, i64,
+                                   vp, sz]),
+    ("ncm_adjust_logits_dev", i32, [vp, vp, vp, vp, i64, i64, i64, i64, i32]),
     ("ncm_rvq_prepare", i32, [vp, vp, i64, i64, i64, vp]),
     ("ncm_rvq_encode", i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp]),
     ("ncm_rvq_encode_counts", i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp, vp,

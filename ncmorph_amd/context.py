@@ -70,3 +70,21 @@ def default_context(device: int = 0) -> Context:
     if device not in ctxs:
         ctxs[device] = Context(device)
     return ctxs[device]
+
+
+def stream_context(device, ctx: Context | None = None) -> Context:
+    """A context on torch's current stream of `device` (a torch.device) for
+    entry points that use no workspace of the context: `ctx`, or one of this
+    thread and device that only they use. It never holds a workspace, so its
+    changes of stream need no event, and a call can be captured into a graph
+    whatever the default context has done before."""
+    if ctx is None:
+        ctxs = getattr(_tls, "stream_ctxs", None)
+        if ctxs is None:
+            ctxs = _tls.stream_ctxs = {}
+        index = device.index or 0
+        ctx = ctxs.get(index)
+        if ctx is None:
+            ctx = ctxs[index] = Context(index)
+    ctx.bind_stream()
+    return ctx

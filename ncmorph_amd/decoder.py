@@ -189,6 +189,63 @@ def rope_inverse_frequencies(spec: DecoderSpec) -> np.ndarray:
     return out
 
 
+def rope_frequencies(rot_dim: int, theta: float, scaling: dict | None = None):
+    """(inv_freq float32 [rot_dim / 2], scale) for kernels.rope_positions:
+    theta^(-2 p / rot_dim), in 64 bits and rounded once, stretched for contexts
+    longer than the trained one as `scaling` says. Its "rope_type" (or "type"):
+      "default"  as they are
+      "linear"   all divided by factor
+      "ntk"      theta times factor^(rot_dim / (rot_dim - 2)): the slowest pair
+                 is stretched by factor, the fastest kept
+      "llama3"   pairs of wavelengths above original_max_position_embeddings /
+                 low_freq_factor divided by factor, those below the same over
+                 high_freq_factor kept, blended between (root.zig:636-682)
+      "yarn"     pairs that turn less than beta_slow (1) times in
+                 original_max_position_embeddings divided by factor, those that
+                 turn more than beta_fast (32) times kept, a linear ramp over
+                 the pairs between; sines and cosines times attention_factor
+                 (0.1 ln factor + 1)."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and positive")
+    if not theta > 1.0:
+        raise ValueError("theta must be above 1")
+    scaling = dict(scaling or {})
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    p = np.arange(rot_dim // 2, dtype=np.float64)
+    inv = theta ** (-2.0 * p / rot_dim)
+    if kind == "default":
+        return inv.astype(np.float32), 1.0
+    if kind not in ("linear", "ntk", "llama3", "yarn"):
+        raise ValueError(f"rope type {kind!r} is not supported")
+    factor = float(scaling["factor"])
+    if not factor > 0.0:
+        raise ValueError("factor must be positive")
+    if kind == "linear":
+        return (inv / factor).astype(np.float32), 1.0
+    if kind == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk needs more than one pair")
+        base = theta * factor ** (rot_dim / (rot_dim - 2.0))
+        return (base ** (-2.0 * p / rot_dim)).astype(np.float32), 1.0
+    length = float(scaling["original_max_position_embeddings"])
+    if kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        turns = length * inv / (2.0 * math.pi)
+        keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
+        return (inv * (keep + (1.0 - keep) / factor)).astype(np.float32), 1.0
+
+    def pair(turns):  # the pair that turns so many times in the trained length
+        return rot_dim * math.log(length / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
+
+    first = max(math.floor(pair(float(scaling.get("beta_fast", 32.0)))), 0)
+    last = min(math.ceil(pair(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+    ramp = np.clip((p - first) / max(last - first, 0.001), 0.0, 1.0)
+    scale = scaling.get("attention_factor")
+    if scale is None:
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return (inv * (1.0 - ramp) + inv / factor * ramp).astype(np.float32), float(scale)
+
+
 def rope_tables(spec: DecoderSpec, positions: int):
     """cosine, sine float32 [positions, head_dim] (root.zig:328-348), system
     cosf / sinf of the f32 angle position * inverse frequency."""

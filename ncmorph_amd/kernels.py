@@ -18,7 +18,7 @@ import numpy as np
 
 from . import _check as _ck
 from ._lib import NCM_OUT_BF16, NCM_OUT_BF16_F32, NCM_OUT_F32, NcmError, check, lib
-from .context import default_context
+from .context import default_context, stream_context
 
 _OUT_MODES = {"f32": NCM_OUT_F32, "bf16_f32": NCM_OUT_BF16_F32, "bf16": NCM_OUT_BF16}
 
@@ -543,4 +543,119 @@ def tied_head_logits_levels(z, codebooks, csq, level_rows, log_inv_t=None, bias=
     check(lib().ncm_tied_head_logits_levels(
         ctx.handle, pz, pe, pc, pb, lit.ctypes.data_as(C.c_void_p),
         rows.ctypes.data_as(C.c_void_p), L, d, v, po), W)
+    return out
+
+
+_ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def rope_positions(x, positions, inv_freq, heads: int, head_dim: int, layout: str = "half",
+                   scale: float = 1.0, out=None, ctx=None):
+    """Rotation of every head of every row of x (torch.bfloat16 or float32
+    [rows, >= heads * head_dim], rows may be strided) at positions (int32
+    [rows]): pair p turns by position * inv_freq[p] (float32 [rot / 2], rot <=
+    head_dim; decoder.rope_frequencies), its sine and cosine times scale. layout
+    "half": pairs (p, p + rot / 2), "interleaved": (2 p, 2 p + 1); values of a
+    head behind rot are copied. The angle is formed in 64 bits, the rotation in
+    float32, rounded once; rope_rotate has the reference's rounding of every
+    operation. out may be x; returns a new [rows, heads * head_dim] without one."""
+    import torch
+
+    W = "rope_positions"
+    a = _ck.Args(W)
+    n_rows, _ = _ck.dims(x, "x", W, 2)
+    (half,) = _ck.dims(inv_freq, "inv_freq", W, 1)
+    if layout not in _ROPE_LAYOUTS:
+        raise NcmError(-7, W, f"layout must be one of {sorted(_ROPE_LAYOUTS)}")
+    width = heads * head_dim
+    px, xs = a.rows(x, "x", ("bfloat16", "float32"), n_rows, width)
+    pp = a.dev(positions, "positions", _ck.I32, (n_rows,))
+    pf = a.dev(inv_freq, "inv_freq", _ck.F32, (half,))
+    if out is None:
+        out = torch.empty((n_rows, width), dtype=x.dtype, device=x.device)
+    po, os_ = a.rows(out, "out", (_ck._dtype(x),), n_rows, width)
+    a.done()
+    ctx = stream_context(x.device, ctx)
+    check(lib().ncm_rope_positions_dev(ctx.handle, px, po, pp, pf, n_rows, heads, head_dim,
+                                       2 * half, max(xs, width), max(os_, width),
+                                       _ROPE_LAYOUTS[layout], scale,
+                                       NCM_OUT_BF16 if x.dtype == torch.bfloat16 else NCM_OUT_F32),
+          W)
+    return out
+
+
+class _LogitRules(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in
+                ("offsets", "history", "prompt_lens", "history_lens", "repetition", "frequency",
+                 "presence", "bias_ids", "bias_values", "allowed", "draft_tokens", "tree_mask")]
+    _fields_ += [(n, C.c_int64) for n in
+                 ("requests", "history_width", "bias_count", "mask_words")]
+
+
+def adjust_logits(logits, history=None, prompt_lens=None, history_lens=None, repetition=None,
+                  frequency=None, presence=None, bias_ids=None, bias_values=None, allowed=None,
+                  offsets=None, draft_tokens=None, tree_mask=None, out=None, ctx=None):
+    """Penalties, biases and grammar masks on logits (torch.float32 or bfloat16
+    [rows, vocab], rows may be strided), before a token is picked; every rule is
+    off where its tensors are not given. Row r is request r, or, with offsets
+    (int32 [requests + 1], as in ncmorph_amd.cache), the rows of request r are
+    offsets[r] .. offsets[r + 1] - 1. Per request: history (int32 [requests,
+    width]) holds its prompt (the first prompt_lens[r]) and the tokens made
+    since (up to history_lens[r]); repetition, frequency, presence (float32
+    [requests]) penalise them; bias_ids and bias_values (int32, float32
+    [requests, n]) add to single tokens. Per row: allowed (int32 [rows,
+    ceil(vocab / 32)]), the bits of the tokens that may follow; draft_tokens
+    (int32 [rows]) with tree_mask (as cache.attention takes it) count the
+    drafted tokens on the row's path as made. The order is
+      seen:  x / repetition where x > 0, else x * repetition
+      x - frequency * count, then x - presence where count > 0
+      x + biases;  -infinity where not allowed
+    in float32, rounded once. out may be logits; new without one."""
+    import torch
+
+    W = "adjust_logits"
+    a = _ck.Args(W)
+    rows, vocab = _ck.dims(logits, "logits", W, 2)
+    requests = rows
+    if offsets is not None:
+        requests = _ck.dims(offsets, "offsets", W, 1)[0] - 1
+        if requests < 0:
+            raise NcmError(-2, W, "offsets must have requests + 1 entries")
+    pl, ls = a.rows(logits, "logits", ("float32", "bfloat16"), rows, vocab)
+    width = nb = words = 0
+    if history is not None:
+        _, width = _ck.dims(history, "history", W, 2)
+    elif prompt_lens is not None or history_lens is not None:
+        raise NcmError(-1, W, "prompt_lens and history_lens need a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise NcmError(-1, W, "bias_ids and bias_values come together")
+    if bias_ids is not None:
+        _, nb = _ck.dims(bias_ids, "bias_ids", W, 2)
+    if draft_tokens is None and tree_mask is not None:
+        raise NcmError(-1, W, "tree_mask needs draft_tokens")
+    if draft_tokens is not None and offsets is None:
+        raise NcmError(-1, W, "draft_tokens need offsets")
+    if tree_mask is not None:
+        _, words = _ck.dims(tree_mask, "tree_mask", W, 2)
+    per, i32, f32 = (requests,), _ck.I32, _ck.F32
+    opt = [(t, n, d, s) for t, n, d, s in (
+        (offsets, "offsets", i32, (requests + 1,)), (history, "history", i32, (requests, width)),
+        (prompt_lens, "prompt_lens", i32, per), (history_lens, "history_lens", i32, per),
+        (repetition, "repetition", f32, per), (frequency, "frequency", f32, per),
+        (presence, "presence", f32, per), (bias_ids, "bias_ids", i32, (requests, nb)),
+        (bias_values, "bias_values", f32, (requests, nb)),
+        (allowed, "allowed", i32 + ("uint32",), (rows, (vocab + 31) // 32)),
+        (draft_tokens, "draft_tokens", i32, (rows,)),
+        (tree_mask, "tree_mask", _ck.U64, (rows, words)))]
+    rules = _LogitRules(*[a.dev(t, n, d, s, optional=True) for t, n, d, s in opt],
+                        requests, width, nb, words)
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    po, os_ = a.rows(out, "out", (_ck._dtype(logits),), rows, vocab)
+    a.done()
+    ctx = stream_context(logits.device, ctx)
+    check(lib().ncm_adjust_logits_dev(ctx.handle, C.byref(rules), pl, po, rows, vocab,
+                                      max(ls, vocab), max(os_, vocab),
+                                      NCM_OUT_BF16 if logits.dtype == torch.bfloat16
+                                      else NCM_OUT_F32), W)
     return out
