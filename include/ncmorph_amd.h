@@ -621,7 +621,8 @@ typedef struct ncm_kv_cache {
  * a captured step follows what they hold at replay. Offsets are clamped to
  * [0, rows] and starts to >= 0; a token past the table or in a page outside
  * [0, pages) is not there: a write leaves it out, a read gives zeros, the
- * attention does not see it. Rows of no request are left as they were. */
+ * attention does not see it. Rows of no request are left as they were. A
+ * table may reach at most 2^30 tokens. */
 typedef struct ncm_kv_batch {
     const int32_t* offsets;     /* [requests + 1] */
     const int32_t* starts;      /* [requests] */

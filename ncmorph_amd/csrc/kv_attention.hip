@@ -1,12 +1,36 @@
 // Attention of a step's rows over the paged cache (ncm_kv_attention_dev).
 //
-// One workgroup per row and query head: its four wavefronts take every fourth
-// token, a lane two (head_dim 128) or one of its values, and keep a running
-// maximum and sum of the softmax; the four are joined through LDS.
+// One pass with the running maximum and sum of a softmax:
+//   s_j = scale q.k_j (times the scale of k_j), m' = max(m, max s_j),
+//   l' = l 2^(m - m') + sum 2^(s_j - m'), o' = o 2^(m - m') + sum 2^(s_j - m') v_j
+// with log2(e) folded into the scale. The query heads of a K/V head and the
+// rows of a request stand together: R times 16 (row, head) pairs are the
+// columns of v_mfma_f32_16x16x32_bf16 products, tokens the rows of S^T = K Q^T
+// and the summed index of O^T = V^T P^T.
+//
+// Bound by the cache's bytes for one token a request, so K and V go from
+// memory to registers, each read once, without LDS between: the lane layout of S^T (a column's
+// four tokens g * 4 .. + 3 in lane group g) is that of the second product's
+// P^T operand if its summed index runs over the tokens in the order the lanes
+// hold them, and a lane then needs of V those same tokens' values of its own
+// dims, which are its own rows' loads, their 16-bit halves regrouped with
+// v_perm_b32. 8-bit codes are widened to bf16 in registers (exact); their
+// scales multiply scores and probabilities, not values.
+//
+// Work: a request's (K/V head, block of 16 R pairs) is a unit of ceil(tokens /
+// 128) tiles; all units' tiles in a row are cut into equal runs, one per
+// workgroup, whatever the requests' lengths, its four wavefronts taking 32
+// tokens of each tile. A unit inside one run is written out, the parts of one
+// that is cut go to the workspace, and kv_attention_join_kernel adds them in
+// order.
 #include "step.h"
 
 namespace ncm {
 namespace {
+
+constexpr int kTile = 128;     // tokens of a tile, 32 per wavefront
+constexpr int kCus = 256;
+constexpr float kNoMax = -1e30f;  // a finite start: 2^(-inf - m) stays 0
 
 struct AttnArgs {
     KvView cache;
@@ -14,76 +38,677 @@ struct AttnArgs {
     const uint16_t* q;
     uint16_t* out;
     const int32_t* positions;
-    const uint64_t* tree_mask;
+    const uint32_t* tree_mask;  // pairs of words
     int64_t q_stride, out_stride, window, mask_words;
     float scale;
-    int q_heads;
+    int q_heads, group;
+    // Workspace: the number of units, a join record per unit, and two parts
+    // per workgroup (the end of a unit that an earlier one began, and the
+    // beginning of one that a later one ends): m and l, then o, per pair.
+    int units;          // records there is room for
+    int* unit_count;
+    int4* joins;        // {first workgroup, parts, request, unit of the request}
+    float2* part_ml;
+    float* part_o;
 };
 
+// What a request asks for, in units and tiles.
+struct Need {
+    Request q;
+    int end;           // tokens that its rows can see lie in [.., end)
+    int before;        // tokens before its rows, at most the table's
+    int tile0, tiles;  // of a unit
+    int blocks;        // of 16 R pairs
+};
+template <int R>
+__device__ __forceinline__ Need need_of(const AttnArgs& a, int r) {
+    Need d;
+    d.q = request_of(a.batch, r);
+    const int64_t cap = a.batch.capacity;
+    d.end = (int)min((int64_t)d.q.before + d.q.n, cap);
+    d.before = (int)min((int64_t)d.q.before, cap);
+    const int64_t low = a.window > 0 ? max((int64_t)d.q.before - a.window + 1, (int64_t)0) : 0;
+    d.tile0 = (int)(min(low, cap) / kTile);
+    d.tiles = max((d.end + kTile - 1) / kTile - d.tile0, 1);
+    d.blocks = (int)(((int64_t)d.q.n * a.group + 16 * R - 1) / (16 * R));
+    return d;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = (uint32_t)uniform((int)v), hi = (uint32_t)uniform((int)(v >> 32));
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// Four codes of a dword as two dwords of bf16 pairs.
 template <int CODES>
-__device__ __forceinline__ float value_of(const char* p, int64_t i) {
-    if constexpr (CODES == NCM_KV_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
-    else if constexpr (CODES == NCM_KV_FP8) return __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)p)[i], 0);
-    else return (float)((const int8_t*)p)[i];
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (CODES == NCM_KV_FP8) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, true));
+    } else {
+        // Integers to 127 are exact in bf16: the high halves of their floats.
+        uint32_t f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __float_as_uint((float)(int8_t)(w >> (8 * i)));
+        lo = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);
+        hi = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
+    }
+}
+
+// 32 tokens of K and V in a wavefront's registers. Lane l: c = l % 16, g = l /
+// 16. k[half]: token 16 half + c, 16 bytes at 64 j + 16 g of its row; v[4 half
+// + i]: token 16 half + 4 g + i, its values at dims HD / 16 * c onwards.
+template <int HD, int CODES>
+struct Tile {
+    static constexpr int ES = CODES == NCM_KV_BF16 ? 2 : 1;
+    static constexpr int KL = HD * ES / 64, VW = HD * ES / 64;
+    typedef uint32_t vec __attribute__((ext_vector_type(VW)));
+    u32x4_t k[2][KL];
+    vec v[8];
+    f32x4_t ks[2], vs[2];
+
+    // page: those of tokens key .. key + 15 and key + 16 .. key + 31, at
+    // least 0; tokens of a page past what the request has are loaded too.
+    __device__ __forceinline__ void load_k(const KvView& cache, int h, int key, int page0,
+                                           int page1, int lane) {
+        const int c = lane & 15, g = lane >> 4, mask = (1 << cache.page_log2) - 1;
+        const uint32_t off = (uint32_t)(c * HD * ES + g * 16);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int64_t page = half ? page1 : page0;
+            const int64_t at = ((int64_t)h << cache.page_log2) + ((key + 16 * half) & mask);
+            const char* base = cache.k + (page * cache.k_stride + at * HD) * ES;
+#pragma unroll
+            for (int j = 0; j < KL; ++j) k[half][j] = *(const u32x4_t*)(base + off + 64 * j);
+            if constexpr (CODES != NCM_KV_BF16)
+                ks[half] = *(const f32x4_t*)(cache.ks + page * cache.ks_stride + at + 4 * g);
+        }
+    }
+    __device__ __forceinline__ void load_v(const KvView& cache, int h, int key, int page0,
+                                           int page1, int lane) {
+        const int c = lane & 15, g = lane >> 4, mask = (1 << cache.page_log2) - 1;
+        const uint32_t off = (uint32_t)(4 * g * HD * ES + c * (HD / 16) * ES);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int64_t page = half ? page1 : page0;
+            const int64_t at = ((int64_t)h << cache.page_log2) + ((key + 16 * half) & mask);
+            const char* base = cache.v + (page * cache.v_stride + at * HD) * ES;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * half + i] = *(const vec*)(base + off + i * HD * ES);
+            if constexpr (CODES != NCM_KV_BF16)
+                vs[half] = *(const f32x4_t*)(cache.vs + page * cache.vs_stride + at + 4 * g);
+        }
+    }
+    // The bf16 operand of k-step s (32 dims) of 16 tokens.
+    __device__ __forceinline__ bf16x8_t k_operand(int half, int s) const {
+        if constexpr (CODES == NCM_KV_BF16) {
+            return __builtin_bit_cast(bf16x8_t, k[half][s]);
+        } else {
+            u32x4_t w;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t lo, hi;
+                widen4<CODES>(k[half][s / 2][2 * (s % 2) + j], lo, hi);
+                w[2 * j] = lo, w[2 * j + 1] = hi;
+            }
+            return __builtin_bit_cast(bf16x8_t, w);
+        }
+    }
+    // The dims of a head that k-step s takes from lane group g.
+    static __device__ __forceinline__ int k_dims(int s, int g) {
+        return CODES == NCM_KV_BF16 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
+    }
+    // V of the eight tokens as bf16 pairs: w[i][u] holds dims 2 u and 2 u + 1
+    // of the lane's HD / 16.
+    __device__ __forceinline__ void v_pairs(uint32_t (&w)[8][HD / 32]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (CODES == NCM_KV_BF16) {
+#pragma unroll
+                for (int u = 0; u < HD / 32; ++u) w[i][u] = v[i][u];
+            } else {
+#pragma unroll
+                for (int u = 0; u < HD / 64; ++u) widen4<CODES>(v[i][u], w[i][2 * u], w[i][2 * u + 1]);
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ float max_over_groups(float v) {
+    u32x2_t p = swap16(__float_as_uint(v));
+    v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    p = swap32(__float_as_uint(v));
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+    u32x2_t p = swap16(__float_as_uint(v));
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    p = swap32(__float_as_uint(v));
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// A wavefront's softmax state for 16 R pairs, and what it needs of them: lane
+// l holds pair l % 16 of each sixteen.
+template <int HD, int R>
+struct State {
+    bf16x8_t q[R][HD / 32];
+    f32x4_t o[R][HD / 16];
+    float m[R], l[R];  // l: of the lane group's own tokens
+    int row[R];        // the pair's row of the request
+    int near[R];       // it sees tokens above this
+};
+
+// Which of a tile's 32 tokens the lane's pair sees: bit 4 half + i for token 16
+// half + 4 g + i. there: bit t, token key + t exists.
+__device__ __forceinline__ uint32_t seen_tokens(const AttnArgs& a, const Need& d, int row, int near,
+                                                int key, uint32_t there, int g) {
+    const int j0 = key - d.before, word = j0 >> 5, words = (int)a.mask_words * 2;
+    uint32_t bits = 0;  // of new tokens
+    if (a.tree_mask) {
+        const uint32_t* m = a.tree_mask + (int64_t)(d.q.o0 + row) * words;
+        const uint32_t lo = word >= 0 && word < words ? m[word] : 0;
+        const uint32_t hi = word >= -1 && word + 1 < words ? m[word + 1] : 0;
+        bits = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j0 & 31));
+    }
+    uint32_t see = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int at = 16 * (i / 4) + 4 * g + i % 4, token = key + at;
+        const bool old = token < d.before;
+        const bool ok = old || !a.tree_mask ? token > near && (old || j0 + at <= row)
+                                            : (bits >> at) & 1u;
+        see |= (ok && ((there >> at) & 1u) ? 1u : 0u) << i;
+    }
+    return see;
+}
+
+// V of the lane's eight tokens where some are not there, or hold a value that
+// is not finite: 0 times either must stay 0 for a pair that does not see them.
+// Tokens that are not there become zero, whatever their places hold. Infinities
+// and NaN become zero too, and per pair and dim those that it sees are counted
+// by a product of their own, 1 for +inf, 64 for -inf, 4096 for NaN (32 tokens
+// at most, so the counts keep apart), and then added to o.
+template <int HD, int R>
+__device__ __forceinline__ void clean_values(uint32_t (&w)[8][HD / 32], const uint32_t (&see)[R],
+                                             uint32_t there, int g, f32x4_t (&o)[R][HD / 16]) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool ok = (there >> (16 * (i / 4) + 4 * g + i % 4)) & 1u;
+#pragma unroll
+        for (int u = 0; u < HD / 32; ++u) {
+            w[i][u] = ok ? w[i][u] : 0u;
+            const uint32_t e = w[i][u] & 0x7F807F80u;
+            bad |= (e & 0xFFFFu) == 0x7F80u || (e >> 16) == 0x7F80u;
+        }
+    }
+    if (!__any(bad)) return;
+    bf16x8_t sees[R];
+#pragma unroll
+    for (int rr = 0; rr < R; ++rr) {
+        u32x4_t b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            b[i] = ((see[rr] >> (2 * i)) & 1u ? 0x3F80u : 0u) |
+                   ((see[rr] >> (2 * i + 1)) & 1u ? 0x3F800000u : 0u);
+        sees[rr] = __builtin_bit_cast(bf16x8_t, b);
+    }
+#pragma unroll
+    for (int u = 0; u < HD / 32; ++u) {
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+            u32x4_t mark = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t v = odd ? w[i][u] >> 16 : w[i][u] & 0xFFFFu;
+                const bool is = (v & 0x7F80u) == 0x7F80u;
+                const uint32_t f = v == 0x7F80u ? 0x3F80u : v == 0xFF80u ? 0x4280u : 0x4580u;
+                mark[i / 2] |= (is ? f : 0u) << (16 * (i % 2));
+                w[i][u] = is ? w[i][u] & (odd ? 0x0000FFFFu : 0xFFFF0000u) : w[i][u];
+            }
+#pragma unroll
+            for (int rr = 0; rr < R; ++rr) {
+                const f32x4_t n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, mark), sees[rr],
+                    f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = (int)n[i];
+                    float add = (k & 63) ? INFINITY : 0.0f;
+                    add = (k >> 6) & 63 ? add - INFINITY : add;
+                    add = k >> 12 ? __builtin_nanf("") : add;
+                    o[rr][2 * u + odd][i] += add;
+                }
+            }
+        }
+    }
+}
+
+// Adds a tile's 32 tokens and loads the next tile's into its registers, K once
+// the scores are formed and V once the outputs are: each load has the other
+// half of a round to arrive in, and a wavefront needs one tile's registers.
+template <int HD, int CODES, int R, typename NextK, typename NextV>
+__device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, Tile<HD, CODES>& t,
+                                           State<HD, R>& st, int key, uint32_t there, bool full,
+                                           float to_log2, int lane, NextK next_k, NextV next_v) {
+    const int g = lane >> 4;
+    float s[R][8];
+    {
+        f32x4_t sc[R][2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int rr = 0; rr < R; ++rr) sc[rr][half] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < HD / 32; ++k) {
+                const bf16x8_t op = t.k_operand(half, k);
+#pragma unroll
+                for (int rr = 0; rr < R; ++rr)
+                    sc[rr][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, st.q[rr][k], sc[rr][half], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int rr = 0; rr < R; ++rr)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s[rr][i] = sc[rr][i / 4][i % 4] * to_log2;
+                if constexpr (CODES != NCM_KV_BF16) s[rr][i] = s[rr][i] * t.ks[i / 4][i % 4];
+            }
+    }
+    next_k();
+    uint32_t see[R];
+    if (!full) {
+#pragma unroll
+        for (int rr = 0; rr < R; ++rr) {
+            see[rr] = seen_tokens(a, d, st.row[rr], st.near[rr], key, there, g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : -INFINITY;
+        }
+    }
+    bf16x8_t p[R];
+#pragma unroll
+    for (int rr = 0; rr < R; ++rr) {
+        float top = st.m[rr];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, s[rr][i]);
+        top = max_over_groups(top);
+        if (__any(top > st.m[rr])) {
+            const float f = __builtin_amdgcn_exp2f(st.m[rr] - top);
+            st.m[rr] = top;
+            st.l[rr] *= f;
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) st.o[rr][n] *= f;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s[rr][i] = __builtin_amdgcn_exp2f(s[rr][i] - st.m[rr]);
+            sum += s[rr][i];
+            if constexpr (CODES != NCM_KV_BF16) s[rr][i] = s[rr][i] * t.vs[i / 4][i % 4];
+        }
+        if (CODES != NCM_KV_BF16 && !full)  // 0 times a scale that is NaN
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : 0.0f;
+        st.l[rr] += sum;
+        // To bf16 for the product: each term of the sum over tokens is off by
+        // up to 2^-9 of itself at random, below the output's own rounding.
+        u32x4_t w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = bf16x2_rne(s[rr][2 * i], s[rr][2 * i + 1]);
+        p[rr] = __builtin_bit_cast(bf16x8_t, w);
+    }
+    uint32_t w[8][HD / 32];
+    t.v_pairs(w);
+    if (!full) clean_values<HD, R>(w, see, there, g, st.o);
+#pragma unroll
+    for (int u = 0; u < HD / 32; ++u) {
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+            u32x4_t b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                b[j] = __builtin_amdgcn_perm(w[2 * j + 1][u], w[2 * j][u], odd ? 0x07060302u : 0x05040100u);
+            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, b);
+#pragma unroll
+            for (int rr = 0; rr < R; ++rr)
+                st.o[rr][2 * u + odd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rr], st.o[rr][2 * u + odd], 0, 0, 0);
+        }
+    }
+    next_v();
+}
+
+template <int HD, int R>
+struct Lds {
+    static constexpr int PITCH = HD + 4;
+    float o[4][16 * R][PITCH];
+    float m[4][16 * R], l[4][16 * R];
+};
+
+// Tiles [first, first + count) of a unit, by the whole workgroup: into `out`
+// where slot < 0, else as a part.
+template <int HD, int CODES, int R>
+__device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r, int h, int block,
+                                         int first, int count, int slot, Lds<HD, R>& lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int pairs = d.q.n * a.group - block * 16 * R;  // of the unit, in all
+    typedef Tile<HD, CODES> T;
+    State<HD, R> st;
+    int far = -1;  // the largest `near`
+#pragma unroll
+    for (int rr = 0; rr < R; ++rr) {
+        const int pair = block * 16 * R + min(16 * rr + c, pairs - 1);
+        const int row = pair / a.group, head = h * a.group + pair - row * a.group;
+        const uint16_t* q = a.q + (d.q.o0 + row) * a.q_stride + (int64_t)head * HD;
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s)
+            st.q[rr][s] = __builtin_bit_cast(bf16x8_t, *(const u32x4_t*)(q + T::k_dims(s, g)));
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) st.o[rr][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        st.m[rr] = kNoMax;
+        st.l[rr] = 0.0f;
+        st.row[rr] = row;
+        st.near[rr] = -1;
+        if (a.window > 0) {
+            int64_t pos = (int64_t)d.q.before + row;
+            if (a.positions) pos = max(a.positions[d.q.o0 + row], d.q.before);
+            st.near[rr] = (int)min(max(pos - a.window, (int64_t)-1), kMaxTokens);
+            far = max(far, st.near[rr]);
+        }
+    }
+    if (a.window > 0)
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) far = max(far, __shfl_xor(far, x));
+    far = uniform(far);
+
+    // Pages of 16 tokens each, 32 tiles' worth at a time: lane 2 s + half.
+    const float to_log2 = a.scale * 1.4426950408889634f;
+    const int key0 = (d.tile0 + first) * kTile + 32 * wave;
+    int pages = -1;
+    auto look_up = [&](int s) {
+        const int t = key0 + (s + (lane >> 1)) * kTile + 16 * (lane & 1);
+        pages = (s + (lane >> 1)) < count && t < d.end ? page_of(a.batch, a.cache, r, t) : -1;
+    };
+    auto page = [&](int s, int half) { return __builtin_amdgcn_readlane(pages, 2 * (s & 31) + half); };
+    auto tokens_there = [&](int key, int p0, int p1) {
+        const int n = min(max(d.end - key, 0), 32);
+        uint32_t m = n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+        if (p0 < 0) m &= 0xFFFF0000u;
+        if (p1 < 0) m &= 0x0000FFFFu;
+        return m;
+    };
+    T t;
+    look_up(0);
+    int p0 = page(0, 0), p1 = page(0, 1);
+    t.load_k(a.cache, h, key0, max(p0, 0), max(p1, 0), lane);
+    t.load_v(a.cache, h, key0, max(p0, 0), max(p1, 0), lane);
+    for (int s = 0; s < count; ++s) {
+        const int key = key0 + s * kTile;
+        const uint32_t there = tokens_there(key, p0, p1);
+        // The last round loads its own tokens again: no branch around the loads.
+        const int s2 = min(s + 1, count - 1);
+        if (s2 != s && (s2 & 31) == 0) look_up(s2);
+        p0 = page(s2, 0), p1 = page(s2, 1);
+        const int key2 = key0 + s2 * kTile;
+        const bool full = there == 0xFFFFFFFFu && key + 32 <= d.before && key > far;
+        add_tokens<HD, CODES, R>(
+            a, d, t, st, key, there, full, to_log2, lane,
+            [&] { t.load_k(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); },
+            [&] { t.load_v(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); });
+    }
+
+    // The four wavefronts' states, joined.
+#pragma unroll
+    for (int rr = 0; rr < R; ++rr) {
+        st.l[rr] = sum_over_groups(st.l[rr]);
+        if (g == 0) lds.m[wave][16 * rr + c] = st.m[rr];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rr = 0; rr < R; ++rr) {
+        const int pr = 16 * rr + c;
+        const float top = fmaxf(fmaxf(lds.m[0][pr], lds.m[1][pr]), fmaxf(lds.m[2][pr], lds.m[3][pr]));
+        const float f = __builtin_amdgcn_exp2f(st.m[rr] - top);
+        if (g == 0) lds.l[wave][pr] = st.l[rr] * f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float* to = &lds.o[wave][pr][(HD / 16) * (4 * g + i)];
+#pragma unroll
+            for (int n = 0; n < HD / 16; n += 4) {
+                f32x4_t v;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[x] = st.o[rr][n + x][i] * f;
+                *(f32x4_t*)(to + n) = v;
+            }
+        }
+    }
+    __syncthreads();
+    constexpr int CH = HD / 8;
+    const int dim = 8 * (tid % CH);
+    for (int pr = tid / CH; pr < min(16 * R, pairs); pr += 256 / CH) {
+        float l = 0.0f;
+        f32x4_t v0 = {0.0f, 0.0f, 0.0f, 0.0f}, v1 = v0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            l += lds.l[w][pr];
+            v0 += *(const f32x4_t*)&lds.o[w][pr][dim];
+            v1 += *(const f32x4_t*)&lds.o[w][pr][dim + 4];
+        }
+        if (slot < 0) {
+            const int pair = block * 16 * R + pr;
+            const int row = pair / a.group, head = h * a.group + pair - row * a.group;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            u32x4_t b;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                b[i] = bf16x2_bits_rne(v0[2 * i] * inv, v0[2 * i + 1] * inv);
+                b[2 + i] = bf16x2_bits_rne(v1[2 * i] * inv, v1[2 * i + 1] * inv);
+            }
+            *(u32x4_t*)(a.out + (d.q.o0 + row) * a.out_stride + (int64_t)head * HD + dim) = b;
+        } else {
+            const int64_t at = (int64_t)slot * 16 * R + pr;
+            if (dim == 0) {
+                const float top = fmaxf(fmaxf(lds.m[0][pr], lds.m[1][pr]),
+                                        fmaxf(lds.m[2][pr], lds.m[3][pr]));
+                a.part_ml[at] = float2{top, l};
+            }
+            *(f32x4_t*)(a.part_o + at * HD + dim) = v0;
+            *(f32x4_t*)(a.part_o + at * HD + dim + 4) = v1;
+        }
+    }
+    __syncthreads();
+}
+
+template <int HD, int CODES, int R>
+__global__ __launch_bounds__(256, R == 4 ? 1 : R == 2 ? 2 : 3) void kv_attention_kernel(AttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char dyn[];
+    Lds<HD, R>& lds = *(Lds<HD, R>*)dyn;
+    __shared__ int64_t wave_tiles[4], found_at;
+    __shared__ int wave_units[4], found, found_units;
+    const int tid = threadIdx.x, lane = tid & 63, heads = a.cache.kv_heads;
+
+    // Tiles and units ahead of each thread's share of the requests.
+    const int per = (a.batch.requests + 255) / 256, r0 = tid * per;
+    const int r1 = min(r0 + per, a.batch.requests);
+    int64_t tiles = 0;
+    int units = 0;
+    for (int r = r0; r < r1; ++r) {
+        const Need d = need_of<R>(a, r);
+        units += d.blocks * heads;
+        tiles += (int64_t)d.blocks * heads * d.tiles;
+    }
+    int64_t t_sum = tiles;
+    int u_sum = units;
+    for (int x = 1; x < 64; x <<= 1) {
+        const int64_t t = __shfl_up(t_sum, x);
+        const int u = __shfl_up(u_sum, x);
+        if (lane >= x) t_sum += t, u_sum += u;
+    }
+    if (lane == 63) wave_tiles[tid >> 6] = t_sum, wave_units[tid >> 6] = u_sum;
+    __syncthreads();
+    int64_t all = 0, t_at = t_sum - tiles;
+    int all_units = 0, u_at = u_sum - units;
+    for (int w = 0; w < 4; ++w) {
+        if (w < (tid >> 6)) t_at += wave_tiles[w], u_at += wave_units[w];
+        all += wave_tiles[w], all_units += wave_units[w];
+    }
+    all = uniform(all);
+    // Runs of tiles: a workgroup each, at most one per tile; neighbours, which
+    // may read the same K and V, on one XCD where every workgroup has a run.
+    const int64_t groups = min((int64_t)gridDim.x, all);
+    const int me = all >= gridDim.x ? xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
+    if (blockIdx.x == 0 && tid == 0) *a.unit_count = min(all_units, a.units);
+    if (me >= groups) return;
+    int64_t at = all * me / groups;
+    const int64_t end = all * (me + 1) / groups;
+    if (at >= t_at && at < t_at + tiles) {
+        int r = r0;
+        for (; r < r1 - 1; ++r) {
+            const Need d = need_of<R>(a, r);
+            const int64_t n = (int64_t)d.blocks * heads * d.tiles;
+            if (at < t_at + n) break;
+            t_at += n, u_at += d.blocks * heads;
+        }
+        found = r, found_at = t_at, found_units = u_at;
+    }
+    __syncthreads();
+    int r = uniform(found), u0 = uniform(found_units);
+    int64_t start = uniform(found_at);  // of the request's tiles
+    while (at < end) {
+        const Need d = need_of<R>(a, r);
+        const int64_t n = (int64_t)d.blocks * heads * d.tiles;
+        if (at >= start + n) {
+            start += n, u0 += d.blocks * heads, ++r;
+            continue;
+        }
+        const int u = (int)((at - start) / d.tiles);
+        const int first = (int)((at - start) - (int64_t)u * d.tiles);
+        const int count = (int)min((int64_t)(d.tiles - first), end - at);
+        int slot = -1;
+        if (first > 0) slot = 2 * me;
+        else if (count < d.tiles) slot = 2 * me + 1;
+        if (first == 0 && tid == 0 && u0 + u < a.units) {
+            // The workgroup that has the unit's last tile ends it.
+            const int64_t last = ((at + d.tiles) * groups - 1) / all;
+            a.joins[u0 + u] = int4{me, (int)(last - me) + 1, r, u};
+        }
+        const int h = u / d.blocks;
+        run_unit<HD, CODES, R>(a, d, r, h, u - h * d.blocks, first, count, slot, lds);
+        at += count;
+    }
+}
+
+// One workgroup per unit that was cut: per pair, its parts' sums brought to
+// their common maximum and added, by a wavefront where they are few, else by
+// all four.
+template <int HD, int R>
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(AttnArgs a) {
+    if ((int)blockIdx.x >= *a.unit_count) return;
+    const int4 j = a.joins[blockIdx.x];
+    const int parts = j.y;
+    if (parts < 2) return;
+    const Need d = need_of<R>(a, j.z);
+    const int h = j.w / d.blocks, block = j.w - h * d.blocks;
+    const int pairs = min(16 * R, d.q.n * a.group - block * 16 * R);
+    constexpr int L = HD / 4;  // lanes of a part
+    const bool few = parts <= 16;
+    const int span = few ? 64 : 256, mine = threadIdx.x % span;
+    const int lanes = mine % L, k0 = mine / L, step = span / L;
+    __shared__ f32x4_t so[256];
+    __shared__ float sm[256], sl[256];
+    const int rows = 256 / span;
+    for (int base = blockIdx.y * rows; base < pairs; base += gridDim.y * rows) {
+        const int pr = base + threadIdx.x / span;
+        float m = kNoMax, l = 0.0f;
+        f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (pr < pairs) {
+#pragma unroll 4
+            for (int k = k0; k < parts; k += step) {
+                const int64_t at = (int64_t)(k == 0 ? 2 * j.x + 1 : 2 * (j.x + k)) * 16 * R + pr;
+                const float2 ml = a.part_ml[at];
+                const f32x4_t v = *(const f32x4_t*)(a.part_o + at * HD + 4 * lanes);
+                const float top = fmaxf(m, ml.x);
+                const float f = __builtin_amdgcn_exp2f(m - top), e = __builtin_amdgcn_exp2f(ml.x - top);
+                l = l * f + ml.y * e;
+                o = o * f + v * e;
+                m = top;
+            }
+        }
+        so[threadIdx.x] = o, sm[threadIdx.x] = m, sl[threadIdx.x] = l;
+        __syncthreads();
+        if (k0 == 0 && pr < pairs) {
+            for (int k = 1; k < step; ++k) {
+                const int x = threadIdx.x + k * L;
+                const float top = fmaxf(m, sm[x]);
+                const float f = __builtin_amdgcn_exp2f(m - top), e = __builtin_amdgcn_exp2f(sm[x] - top);
+                l = l * f + sl[x] * e;
+                o = o * f + so[x] * e;
+                m = top;
+            }
+            const int pair = block * 16 * R + pr;
+            const int row = pair / a.group, head = h * a.group + pair - row * a.group;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const u32x2_t b = {bf16x2_bits_rne(o[0] * inv, o[1] * inv),
+                               bf16x2_bits_rne(o[2] * inv, o[3] * inv)};
+            *(u32x2_t*)(a.out + (d.q.o0 + row) * a.out_stride + (int64_t)head * HD + 4 * lanes) = b;
+        }
+        __syncthreads();
+    }
+}
+
+// How a step is laid out: by its sizes alone, so that the workspace's size and
+// the launch agree.
+struct Layout {
+    int r16;            // R
+    int64_t units;      // at most
+    int64_t groups;     // workgroups
+    bool cut;           // whether a unit can be
+    size_t joins, ml, o, bytes;  // offsets in the workspace
+};
+
+Layout layout_of(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int q_heads) {
+    Layout s;
+    const int64_t group = q_heads / c.kv_heads, pairs = b.rows * group;
+    const int64_t some = std::max<int64_t>(1, std::min(b.requests, b.rows));
+    // 16 R pairs a unit: as many as a request has on average, up to 64.
+    s.r16 = pairs <= 16 * some ? 1 : pairs <= 32 * some ? 2 : 4;
+    s.units = (pairs / (16 * s.r16) + some) * c.kv_heads;
+    const int64_t tiles = std::max<int64_t>(1, ((b.table_width * c.page_size) + kTile - 1) / kTile);
+    s.cut = tiles > 1;
+    s.groups = std::min<int64_t>(s.units * tiles, s.r16 == 4 ? kCus : s.r16 == 2 ? 2 * kCus : 3 * kCus);
+    const size_t slots = 2 * (size_t)s.groups * 16 * s.r16;
+    s.joins = 16;
+    s.ml = s.joins + 16 * (size_t)s.units;
+    s.o = s.ml + (slots * 8 + 15) / 16 * 16;
+    s.bytes = s.o + slots * c.head_dim * 4;
+    return s;
+}
+
+template <int HD, int CODES, int R>
+hipError_t launch(const AttnArgs& a, const Layout& s, hipStream_t st) {
+    constexpr int lds = sizeof(Lds<HD, R>);
+    if constexpr (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kv_attention_kernel<HD, CODES, R>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    kv_attention_kernel<HD, CODES, R><<<(uint32_t)s.groups, 256, lds, st>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !s.cut) return e;
+    // Few units that are cut into many parts: a workgroup per pair.
+    const uint32_t y = s.units * 8 <= s.groups ? 16 * R : 4 * R;
+    kv_attention_join_kernel<HD, R><<<dim3((uint32_t)s.units, y), 256, 0, st>>>(a);
+    return hipGetLastError();
 }
 
 template <int HD, int CODES>
-__global__ __launch_bounds__(256) void kv_attention_kernel(AttnArgs a) {
-    constexpr int PER = HD / 64;
-    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int h = head / (a.q_heads / a.cache.kv_heads);
-    int r = 0;
-    for (int j = 0; j < a.batch.requests; ++j) r += a.batch.offsets[j + 1] <= row;
-    if (r >= a.batch.requests) return;
-    const Request rq = request_of(a.batch, r);
-    if (row < rq.o0 || row >= rq.o0 + rq.n) return;
-    const int i = row - rq.o0;
-    const int64_t pos = a.positions ? max(a.positions[row], rq.before) : (int64_t)rq.before + i;
-    float q[PER], o[PER];
-    for (int d = 0; d < PER; ++d) {
-        q[d] = __uint_as_float((uint32_t)a.q[row * a.q_stride + head * HD + lane + 64 * d] << 16);
-        o[d] = 0.0f;
+hipError_t launch_r(const AttnArgs& a, const Layout& s, hipStream_t st) {
+    switch (s.r16) {
+        case 1: return launch<HD, CODES, 1>(a, s, st);
+        case 2: return launch<HD, CODES, 2>(a, s, st);
+        default: return launch<HD, CODES, 4>(a, s, st);
     }
-    float m = -1e30f, l = 0.0f;
-    for (int64_t t = wave; t < (int64_t)rq.before + rq.n; t += 4) {
-        const int64_t j = t - rq.before;
-        bool see;
-        if (j < 0 || !a.tree_mask) see = j <= i && (a.window <= 0 || t > pos - a.window);
-        else see = (j >> 6) < a.mask_words &&
-                   ((a.tree_mask[row * a.mask_words + (j >> 6)] >> (j & 63)) & 1u);
-        if (!see) continue;
-        const int page = page_of(a.batch, a.cache, r, t);
-        if (page < 0) continue;
-        const int64_t in_page = ((int64_t)h << a.cache.page_log2) + (t & ((1 << a.cache.page_log2) - 1));
-        const int64_t kb = page * a.cache.k_stride + in_page * HD, vb = page * a.cache.v_stride + in_page * HD;
-        float s = 0.0f;
-        for (int d = 0; d < PER; ++d) s = fmaf(q[d], value_of<CODES>(a.cache.k, kb + lane + 64 * d), s);
-        s = wave_sum_xor(s) * a.scale;
-        float vs = 1.0f;
-        if constexpr (CODES != NCM_KV_BF16) {
-            s *= a.cache.ks[page * a.cache.ks_stride + in_page];
-            vs = a.cache.vs[page * a.cache.vs_stride + in_page];
-        }
-        const float mn = fmaxf(m, s), al = expf(m - mn), p = expf(s - mn);
-        l = l * al + p;
-        for (int d = 0; d < PER; ++d)
-            o[d] = fmaf(p * vs, value_of<CODES>(a.cache.v, vb + lane + 64 * d), o[d] * al);
-        m = mn;
-    }
-    __shared__ float sm[4], sl[4], so[4][HD];
-    if (lane == 0) sm[wave] = m, sl[wave] = l;
-    for (int d = 0; d < PER; ++d) so[wave][lane + 64 * d] = o[d];
-    __syncthreads();
-    if (threadIdx.x >= HD) return;
-    const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    float total = 0.0f, acc = 0.0f;
-    for (int w = 0; w < 4; ++w) {
-        const float f = expf(sm[w] - top);
-        total = fmaf(sl[w], f, total);
-        acc = fmaf(so[w][threadIdx.x], f, acc);
-    }
-    a.out[row * a.out_stride + head * HD + threadIdx.x] =
-        (uint16_t)bf16_bits_rne(total == 0.0f ? 0.0f : acc / total);
 }
 
 int check_attention(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch, int q_heads,
@@ -92,8 +717,11 @@ int check_attention(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch, in
     if (rc) return rc;
     rc = check_batch(batch, a->cache.page_log2, &a->batch);
     if (rc) return rc;
-    if (q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads) return NCM_E_SHAPE;
+    if (q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads ||
+        batch->rows * q_heads > 0x7FFFFFFF)
+        return NCM_E_SHAPE;
     a->q_heads = q_heads;
+    a->group = q_heads / cache->kv_heads;
     return NCM_OK;
 }
 
@@ -107,7 +735,10 @@ extern "C" int ncm_kv_attention_workspace(const ncm_kv_cache_t* cache,
     if (!bytes) return NCM_E_NULL;
     *bytes = 0;
     AttnArgs a = {};
-    return check_attention(cache, batch, q_heads, &a);
+    const int rc = check_attention(cache, batch, q_heads, &a);
+    if (rc) return rc;
+    if (batch->rows > 0 && batch->requests > 0) *bytes = layout_of(*cache, *batch, q_heads).bytes;
+    return NCM_OK;
 }
 
 extern "C" int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
@@ -121,33 +752,40 @@ extern "C" int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
     AttnArgs a = {};
     int rc = check_attention(cache, batch, q_heads, &a);
     if (rc) return rc;
-    if (window < 0 || mask_words < 0 || mask_words > kMaxRows) return NCM_E_SHAPE;
+    if (window < 0 || mask_words < 0 || mask_words > kMaxRows / 2) return NCM_E_SHAPE;
     if (batch->rows == 0 || batch->requests == 0) return NCM_OK;
     const int64_t width = (int64_t)q_heads * cache->head_dim;
     rc = check_rows(q, q_stride, width);
     if (!rc) rc = check_rows(out, out_stride, width);
     if (rc) return rc;
-    a.q = q, a.out = out, a.positions = positions, a.tree_mask = tree_mask;
+    const Layout s = layout_of(*cache, *batch, q_heads);
+    if (!workspace) return NCM_E_NULL;
+    if (workspace_bytes < s.bytes) return NCM_E_LENGTH;
+    if ((uintptr_t)workspace % 16) return NCM_E_ARG;
+    char* ws = (char*)workspace;
+    a.q = q, a.out = out, a.positions = positions, a.tree_mask = (const uint32_t*)tree_mask;
     a.q_stride = q_stride, a.out_stride = out_stride, a.window = window;
     a.mask_words = mask_words, a.scale = scale;
+    a.units = (int)s.units;
+    a.unit_count = (int*)ws;
+    a.joins = (int4*)(ws + s.joins);
+    a.part_ml = (float2*)(ws + s.ml);
+    a.part_o = (float*)(ws + s.o);
     const DeviceScope scope(ncm_ctx_device(ctx));
     rc = step_hip(scope.error(), "kv_attention device");
     if (rc) return rc;
     const hipStream_t st = ncm_ctx_stream(ctx);
-    const dim3 grid((uint32_t)batch->rows, (uint32_t)q_heads);
     const bool wide = cache->head_dim == 128;
+    hipError_t e;
     switch (cache->codes) {
         case NCM_KV_BF16:
-            wide ? kv_attention_kernel<128, NCM_KV_BF16><<<grid, 256, 0, st>>>(a)
-                 : kv_attention_kernel<64, NCM_KV_BF16><<<grid, 256, 0, st>>>(a);
+            e = wide ? launch_r<128, NCM_KV_BF16>(a, s, st) : launch_r<64, NCM_KV_BF16>(a, s, st);
             break;
         case NCM_KV_FP8:
-            wide ? kv_attention_kernel<128, NCM_KV_FP8><<<grid, 256, 0, st>>>(a)
-                 : kv_attention_kernel<64, NCM_KV_FP8><<<grid, 256, 0, st>>>(a);
+            e = wide ? launch_r<128, NCM_KV_FP8>(a, s, st) : launch_r<64, NCM_KV_FP8>(a, s, st);
             break;
         default:
-            wide ? kv_attention_kernel<128, NCM_KV_INT8><<<grid, 256, 0, st>>>(a)
-                 : kv_attention_kernel<64, NCM_KV_INT8><<<grid, 256, 0, st>>>(a);
+            e = wide ? launch_r<128, NCM_KV_INT8>(a, s, st) : launch_r<64, NCM_KV_INT8>(a, s, st);
     }
-    return step_hip(hipGetLastError(), "kv_attention launch");
+    return step_hip(e, "kv_attention launch");
 }

@@ -89,6 +89,7 @@ __device__ __forceinline__ int page_of(const BatchView& b, const KvView& c, int6
 
 constexpr int64_t kMaxRequests = 65535;
 constexpr int64_t kMaxRows = int64_t(1) << 30;
+constexpr int64_t kMaxTokens = int64_t(1) << 30;  // of a sequence
 
 inline int check_cache(const ncm_kv_cache_t* c, KvView* view) {
     if (!c) return NCM_E_NULL;
@@ -126,7 +127,7 @@ inline int check_batch(const ncm_kv_batch_t* b, int page_log2, BatchView* view) 
     if (!b) return NCM_E_NULL;
     if (b->requests < 0 || b->requests > kMaxRequests || b->rows < 0 || b->rows > kMaxRows ||
         b->table_width < 0 || b->table_width > 0x7FFFFFFF || b->table_stride < b->table_width ||
-        b->table_stride > (int64_t(1) << 40))
+        b->table_stride > (int64_t(1) << 40) || b->table_width << page_log2 > kMaxTokens)
         return NCM_E_SHAPE;
     if (b->requests > 0 && b->rows > 0 &&
         (!b->offsets || !b->starts || (!b->page_table && b->table_width > 0)))

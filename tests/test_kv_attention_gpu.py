@@ -317,3 +317,6 @@ def test_refusals(ncm, cuda):
         cache.attention(q, kv, 4, table, offs, starts, window=-1)
     with pytest.raises(NcmError):
         cache.attention(q[:, 1:129], kv, 2, table, offs, starts)         # alignment
+    with pytest.raises(NcmError):
+        cache.attention(q, kv, 4, table, offs, starts,                   # too small
+                        workspace=torch.zeros(8, dtype=torch.uint8, device=cuda))
