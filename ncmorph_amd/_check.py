@@ -29,6 +29,20 @@ def _dtype(t) -> str:
     return name
 
 
+class _Accepted(dict):
+    """The torch dtypes that a tuple of names stands for."""
+
+    def __missing__(self, names):
+        import torch
+
+        got = frozenset(getattr(torch, n) for n in names if hasattr(torch, n))
+        self[names] = got
+        return got
+
+
+_ACCEPTED = _Accepted()
+
+
 def _common(t, name, where, dtypes):
     if not hasattr(t, "data_ptr") or not hasattr(t, "is_cuda"):
         raise NcmError(NCM_E_ARG, where, f"{name} must be a torch tensor")
@@ -61,6 +75,10 @@ class Args:
             if optional:
                 return None
             raise NcmError(NCM_E_NULL, W, f"{name} is required")
+        if (getattr(t, "dtype", None) in _ACCEPTED[dtypes] and t.is_contiguous()
+                and (shape is None or t.shape == shape)):
+            self.seen.append((t, name))  # nothing of what follows applies
+            return t.data_ptr()
         _common(t, name, W, dtypes)
         if shape is not None and tuple(t.shape) != tuple(shape):
             raise NcmError(NCM_E_SHAPE, W,
@@ -77,19 +95,22 @@ class Args:
         W = self.where
         if t is None:
             raise NcmError(NCM_E_NULL, W, f"{name} is required")
-        _common(t, name, W, dtypes)
+        if getattr(t, "dtype", None) not in _ACCEPTED[dtypes]:
+            _common(t, name, W, dtypes)
         if t.dim() != 2 or t.shape[0] != n_rows or t.shape[1] < min_cols:
             raise NcmError(NCM_E_SHAPE, W,
                            f"{name} has shape {tuple(t.shape)}, expected ({n_rows}, >= {min_cols})")
-        if t.stride(1) != 1 or (n_rows > 1 and t.stride(0) < min_cols):
+        stride, inner = t.stride()
+        if inner != 1 or (n_rows > 1 and stride < min_cols):
             raise NcmError(NCM_E_ARG, W, f"{name} must have contiguous, non-overlapping rows")
         self.seen.append((t, name))
-        return t.data_ptr(), t.stride(0)
+        return t.data_ptr(), stride
 
     def done(self):
         device = self.seen[0][0].device if self.seen else None
         for t, name in self.seen:
-            _placed(t, name, self.where, device)
+            if not t.is_cuda or t.device != device:
+                _placed(t, name, self.where, device)
 
 
 def dims(t, name, where, ndim):
@@ -98,4 +119,4 @@ def dims(t, name, where, ndim):
         raise NcmError(NCM_E_NULL, where, f"{name} is required")
     if not hasattr(t, "shape") or len(t.shape) != ndim:
         raise NcmError(NCM_E_SHAPE, where, f"{name} must have {ndim} dimensions")
-    return tuple(map(int, t.shape))
+    return tuple(t.shape)

@@ -17,14 +17,14 @@ ncm_kv_cache_t and ncm_kv_batch_t say the rest. The reference has no cache
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 from . import _check as _ck
 from ._lib import NCM_E_ARG, NCM_E_SHAPE, NcmError, check, lib
 from .context import stream_context
 
 NCM_KV_BF16, NCM_KV_FP8, NCM_KV_INT8 = 0, 1, 2
-_CODES = {"bfloat16": NCM_KV_BF16, "int16": NCM_KV_BF16, "uint16": NCM_KV_BF16,
-          "float8_e4m3fn": NCM_KV_FP8, "int8": NCM_KV_INT8}
+_CODES = {"bfloat16": NCM_KV_BF16, "float8_e4m3fn": NCM_KV_FP8, "int8": NCM_KV_INT8}
 
 
 class _Cache(C.Structure):
@@ -43,8 +43,10 @@ class _Batch(C.Structure):
 
 def _page_stride(t, name, shape, where):
     """Elements from a page to the next of a tensor of contiguous pages."""
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise NcmError(NCM_E_SHAPE, where, f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.is_contiguous():
+        return math.prod(shape[1:])
     inner, strides = 1, t.stride()
     for d in range(len(shape) - 1, 0, -1):
         if shape[d] != 1 and strides[d] != inner:
@@ -62,43 +64,39 @@ class KvCache:
     apart, as those of one layer of a buffer [pages, layers, ...] do.
     page_size: a power of two, 16 to 1024; head_dim 64 or 128."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "struct")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "named")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         W = "KvCache"
         pages, heads, page, hd = shape = _ck.dims(k, "k", W, 4)
-        codes = _CODES.get(_ck._dtype(k))
+        name = _ck._dtype(k)
+        codes = _CODES.get(name)
         if codes is None:
-            raise NcmError(NCM_E_ARG, W, f"k has dtype {_ck._dtype(k)}, expected bfloat16, "
+            raise NcmError(NCM_E_ARG, W, f"k has dtype {name}, expected bfloat16, "
                                          "float8_e4m3fn or int8")
-        _ck._common(v, "v", W, (_ck._dtype(k),))
-        strides = [_page_stride(k, "k", shape, W), _page_stride(v, "v", shape, W), 0, 0]
+        if getattr(v, "dtype", None) != k.dtype:
+            _ck._common(v, "v", W, (name,))
+        ks, vs = _page_stride(k, "k", shape, W), _page_stride(v, "v", shape, W)
         if hd not in (64, 128):
             raise NcmError(NCM_E_SHAPE, W, "head_dim must be 64 or 128")
         if not 16 <= page <= 1024 or page & (page - 1):
             raise NcmError(NCM_E_SHAPE, W, "page_size must be a power of two, 16 to 1024")
-        scales = [(k_scale, "k_scale"), (v_scale, "v_scale")]
-        for i, (t, name) in enumerate(scales):
-            if codes == NCM_KV_BF16:
-                if t is not None:
-                    raise NcmError(NCM_E_ARG, W, f"{name} is for a quantised cache")
-                continue
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        if codes == NCM_KV_BF16:
+            if k_scale is not None or v_scale is not None:
+                raise NcmError(NCM_E_ARG, W, "k_scale and v_scale are for a quantised cache")
+            self.named = (k, "k pages"), (v, "v pages")
+            self.struct = _Cache(k.data_ptr(), v.data_ptr(), None, None, ks, vs, 0, 0, pages,
+                                 heads, page, hd, codes)
+            return
+        self.named = (k, "k pages"), (v, "v pages"), (k_scale, "k_scale"), (v_scale, "v_scale")
+        for t, name in self.named[2:]:
             if t is None:
                 raise NcmError(-1, W, f"{name} is required")
             _ck._common(t, name, W, _ck.F32)
-            strides[2 + i] = _page_stride(t, name, shape[:3], W)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.struct = _Cache(k.data_ptr(), v.data_ptr(),
-                             None if k_scale is None else k_scale.data_ptr(),
-                             None if v_scale is None else v_scale.data_ptr(),
-                             *strides, pages, heads, page, hd, codes)
-
-    def named(self):
-        yield self.k, "k pages"
-        yield self.v, "v pages"
-        if self.k_scale is not None:
-            yield self.k_scale, "k_scale"
-            yield self.v_scale, "v_scale"
+        kss, vss = (_page_stride(t, name, shape[:3], W) for t, name in self.named[2:])
+        self.struct = _Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                             ks, vs, kss, vss, pages, heads, page, hd, codes)
 
 
 def allocate(pages: int, kv_heads: int, page_size: int, head_dim: int, dtype, device) -> KvCache:
@@ -122,7 +120,7 @@ def _batch(a, kv, page_table, offsets, starts, rows):
     ps = a.dev(starts, "starts", _ck.I32, (requests,))
     po = a.dev(offsets, "offsets", _ck.I32, (requests + 1,))
     pt, stride = a.rows(page_table, "page_table", _ck.I32, requests, width)
-    a.seen.extend(kv.named())
+    a.seen += kv.named
     return _Batch(po, ps, pt, requests, rows, width, max(stride, width))
 
 
@@ -160,8 +158,7 @@ def read(kv: KvCache, page_table, offsets, starts, rows: int, out=None, ctx=None
     b = _batch(a, kv, page_table, offsets, starts, rows)
     width = kv.struct.kv_heads * kv.struct.head_dim
     if out is None:
-        out = tuple(torch.empty((rows, width), dtype=torch.bfloat16, device=kv.k.device)
-                    for _ in range(2))
+        out = torch.empty((2, rows, width), dtype=torch.bfloat16, device=kv.k.device).unbind()
     pk, ks = _rows(a, out[0], "out[0]", rows, width)
     pv, vs = _rows(a, out[1], "out[1]", rows, width)
     a.done()

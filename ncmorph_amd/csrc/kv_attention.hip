@@ -159,21 +159,29 @@ struct Tile {
     static __device__ __forceinline__ int k_dims(int s, int g) {
         return CODES == NCM_KV_BF16 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
     }
-    // V of the eight tokens as bf16 pairs: w[i][u] holds dims 2 u and 2 u + 1
-    // of the lane's HD / 16.
-    __device__ __forceinline__ void v_pairs(uint32_t (&w)[8][HD / 32]) const {
+    // Dims 2 x and 2 x + 1 of the lane's HD / 16, x = 2 f .. 2 f + 1, of the
+    // eight tokens, as bf16 pairs.
+    __device__ __forceinline__ void v_pairs(int f, uint32_t (&w)[8][2]) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if constexpr (CODES == NCM_KV_BF16) {
-#pragma unroll
-                for (int u = 0; u < HD / 32; ++u) w[i][u] = v[i][u];
-            } else {
-#pragma unroll
-                for (int u = 0; u < HD / 64; ++u) widen4<CODES>(v[i][u], w[i][2 * u], w[i][2 * u + 1]);
-            }
+            if constexpr (CODES == NCM_KV_BF16) w[i][0] = v[i][2 * f], w[i][1] = v[i][2 * f + 1];
+            else widen4<CODES>(v[i][f], w[i][0], w[i][1]);
         }
     }
 };
+
+// Which values of a dword of V are not finite: all ones in their places.
+template <int CODES>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+    if constexpr (CODES == NCM_KV_BF16) {
+        const uint32_t e = x & 0x7F807F80u;
+        return ((e & 0xFFFFu) == 0x7F80u ? 0xFFFFu : 0u) | ((e >> 16) == 0x7F80u ? 0xFFFF0000u : 0u);
+    } else if constexpr (CODES == NCM_KV_FP8) {
+        return ((((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xFFu;
+    } else {
+        return 0u;
+    }
+}
 
 __device__ __forceinline__ float max_over_groups(float v) {
     u32x2_t p = swap16(__float_as_uint(v));
@@ -223,62 +231,57 @@ __device__ __forceinline__ uint32_t seen_tokens(const AttnArgs& a, const Need& d
     return see;
 }
 
-// V of the lane's eight tokens where some are not there, or hold a value that
-// is not finite: 0 times either must stay 0 for a pair that does not see them.
-// Tokens that are not there become zero, whatever their places hold. Infinities
-// and NaN become zero too, and per pair and dim those that it sees are counted
-// by a product of their own, 1 for +inf, 64 for -inf, 4096 for NaN (32 tokens
-// at most, so the counts keep apart), and then added to o.
-template <int HD, int R>
-__device__ __forceinline__ void clean_values(uint32_t (&w)[8][HD / 32], const uint32_t (&see)[R],
-                                             uint32_t there, int g, f32x4_t (&o)[R][HD / 16]) {
-    bool bad = false;
+// V where some tokens are not there, or hold a value that is not finite: 0
+// times either must stay 0 for a pair that does not see them. Tokens that are
+// not there become zero, whatever their places hold. Infinities and NaN become
+// zero too, and are added to the outputs of the pairs that see them from their
+// token's row in the cache, one such token after another.
+template <int HD, int CODES, int R>
+__device__ __forceinline__ void clean_values(const AttnArgs& a, int h, int key, int page0, int page1,
+                                             Tile<HD, CODES>& t, const uint32_t (&see)[R],
+                                             uint32_t there, int lane, State<HD, R>& st) {
+    typedef Tile<HD, CODES> T;
+    const int c = lane & 15, g = lane >> 4;
+    uint32_t bad = 0;  // bit i: the lane's token i holds one
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const bool ok = (there >> (16 * (i / 4) + 4 * g + i % 4)) & 1u;
 #pragma unroll
-        for (int u = 0; u < HD / 32; ++u) {
-            w[i][u] = ok ? w[i][u] : 0u;
-            const uint32_t e = w[i][u] & 0x7F807F80u;
-            bad |= (e & 0xFFFFu) == 0x7F80u || (e >> 16) == 0x7F80u;
+        for (int u = 0; u < T::VW; ++u) {
+            t.v[i][u] = ok ? t.v[i][u] : 0u;
+            const uint32_t m = not_finite<CODES>(t.v[i][u]);
+            t.v[i][u] &= ~m;
+            bad |= m ? 1u << i : 0u;
         }
     }
-    if (!__any(bad)) return;
-    bf16x8_t sees[R];
+    if constexpr (CODES == NCM_KV_INT8) return;
+    if (!__any(bad != 0)) return;
+    for (int at = 0; at < 32; ++at) {
+        const int i = 4 * (at / 16) + at % 4, tg = (at % 16) / 4;
+        const uint64_t in_lanes = __ballot(g == tg && ((bad >> i) & 1u));
+        if (!in_lanes) continue;
+        const int64_t page = at < 16 ? page0 : page1;
+        const int64_t row = ((int64_t)h << a.cache.page_log2) +
+                            ((key + at) & ((1 << a.cache.page_log2) - 1));
+        const char* p = a.cache.v + (page * a.cache.v_stride + row * HD) * T::ES;
+        bool sees[R];
 #pragma unroll
-    for (int rr = 0; rr < R; ++rr) {
-        u32x4_t b;
+        for (int rr = 0; rr < R; ++rr) sees[rr] = (__shfl((int)see[rr], 16 * tg + c) >> i) & 1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            b[i] = ((see[rr] >> (2 * i)) & 1u ? 0x3F80u : 0u) |
-                   ((see[rr] >> (2 * i + 1)) & 1u ? 0x3F800000u : 0u);
-        sees[rr] = __builtin_bit_cast(bf16x8_t, b);
-    }
+        for (int x = 0; x < 4; ++x) {
+            const typename T::vec v = *(const typename T::vec*)(p + (4 * g + x) * (HD / 16) * T::ES);
 #pragma unroll
-    for (int u = 0; u < HD / 32; ++u) {
+            for (int u = 0; u < T::VW; ++u) {
+                const uint32_t odd = v[u] & not_finite<CODES>(v[u]);
 #pragma unroll
-        for (int odd = 0; odd < 2; ++odd) {
-            u32x4_t mark = {0, 0, 0, 0};
+                for (int k = 0; k < 4 / T::ES; ++k) {
+                    // Where it is not finite, the value; else 0.
+                    const uint32_t bits = odd >> (8 * T::ES * k);
+                    const float add = T::ES == 2 ? __uint_as_float(bits << 16)
+                                                 : (bits & 0x7Fu) ? __builtin_nanf("") : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t v = odd ? w[i][u] >> 16 : w[i][u] & 0xFFFFu;
-                const bool is = (v & 0x7F80u) == 0x7F80u;
-                const uint32_t f = v == 0x7F80u ? 0x3F80u : v == 0xFF80u ? 0x4280u : 0x4580u;
-                mark[i / 2] |= (is ? f : 0u) << (16 * (i % 2));
-                w[i][u] = is ? w[i][u] & (odd ? 0x0000FFFFu : 0xFFFF0000u) : w[i][u];
-            }
-#pragma unroll
-            for (int rr = 0; rr < R; ++rr) {
-                const f32x4_t n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    __builtin_bit_cast(bf16x8_t, mark), sees[rr],
-                    f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = (int)n[i];
-                    float add = (k & 63) ? INFINITY : 0.0f;
-                    add = (k >> 6) & 63 ? add - INFINITY : add;
-                    add = k >> 12 ? __builtin_nanf("") : add;
-                    o[rr][2 * u + odd][i] += add;
+                    for (int rr = 0; rr < R; ++rr)
+                        st.o[rr][4 / T::ES * u + k][x] += sees[rr] ? add : 0.0f;
                 }
             }
         }
@@ -288,10 +291,12 @@ __device__ __forceinline__ void clean_values(uint32_t (&w)[8][HD / 32], const ui
 // Adds a tile's 32 tokens and loads the next tile's into its registers, K once
 // the scores are formed and V once the outputs are: each load has the other
 // half of a round to arrive in, and a wavefront needs one tile's registers.
-template <int HD, int CODES, int R, typename NextK, typename NextV>
-__device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, Tile<HD, CODES>& t,
-                                           State<HD, R>& st, int key, uint32_t there, bool full,
-                                           float to_log2, int lane, NextK next_k, NextV next_v) {
+// FULL: every pair sees every token.
+template <bool FULL, int HD, int CODES, int R, typename NextK, typename NextV>
+__device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int h,
+                                           Tile<HD, CODES>& t, State<HD, R>& st, int key, int page0,
+                                           int page1, uint32_t there, float to_log2, int lane,
+                                           NextK next_k, NextV next_v) {
     const int g = lane >> 4;
     float s[R][8];
     {
@@ -318,7 +323,7 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, Til
     }
     next_k();
     uint32_t see[R];
-    if (!full) {
+    if constexpr (!FULL) {
 #pragma unroll
         for (int rr = 0; rr < R; ++rr) {
             see[rr] = seen_tokens(a, d, st.row[rr], st.near[rr], key, there, g);
@@ -346,10 +351,9 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, Til
             s[rr][i] = __builtin_amdgcn_exp2f(s[rr][i] - st.m[rr]);
             sum += s[rr][i];
             if constexpr (CODES != NCM_KV_BF16) s[rr][i] = s[rr][i] * t.vs[i / 4][i % 4];
+            if constexpr (CODES != NCM_KV_BF16 && !FULL)  // 0 times a scale that is NaN
+                s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : 0.0f;
         }
-        if (CODES != NCM_KV_BF16 && !full)  // 0 times a scale that is NaN
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : 0.0f;
         st.l[rr] += sum;
         // To bf16 for the product: each term of the sum over tokens is off by
         // up to 2^-9 of itself at random, below the output's own rounding.
@@ -358,21 +362,22 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, Til
         for (int i = 0; i < 4; ++i) w[i] = bf16x2_rne(s[rr][2 * i], s[rr][2 * i + 1]);
         p[rr] = __builtin_bit_cast(bf16x8_t, w);
     }
-    uint32_t w[8][HD / 32];
-    t.v_pairs(w);
-    if (!full) clean_values<HD, R>(w, see, there, g, st.o);
+    if constexpr (!FULL) clean_values<HD, CODES, R>(a, h, key, page0, page1, t, see, there, lane, st);
 #pragma unroll
-    for (int u = 0; u < HD / 32; ++u) {
+    for (int f = 0; f < HD / 64; ++f) {
+        uint32_t w[8][2];
+        t.v_pairs(f, w);
 #pragma unroll
-        for (int odd = 0; odd < 2; ++odd) {
+        for (int n = 0; n < 4; ++n) {
             u32x4_t b;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                b[j] = __builtin_amdgcn_perm(w[2 * j + 1][u], w[2 * j][u], odd ? 0x07060302u : 0x05040100u);
+                b[j] = __builtin_amdgcn_perm(w[2 * j + 1][n / 2], w[2 * j][n / 2],
+                                             n % 2 ? 0x07060302u : 0x05040100u);
             const bf16x8_t v = __builtin_bit_cast(bf16x8_t, b);
 #pragma unroll
             for (int rr = 0; rr < R; ++rr)
-                st.o[rr][2 * u + odd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rr], st.o[rr][2 * u + odd], 0, 0, 0);
+                st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rr], st.o[rr][4 * f + n], 0, 0, 0);
         }
     }
     next_v();
@@ -443,19 +448,26 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     int p0 = page(0, 0), p1 = page(0, 1);
     t.load_k(a.cache, h, key0, max(p0, 0), max(p1, 0), lane);
     t.load_v(a.cache, h, key0, max(p0, 0), max(p1, 0), lane);
-    for (int s = 0; s < count; ++s) {
-        const int key = key0 + s * kTile;
-        const uint32_t there = tokens_there(key, p0, p1);
+    // A round: 32 tokens, their K and V in t, their pages in p0 and p1.
+    int s = 0;
+    auto round = [&](auto full) {
+        const int key = key0 + s * kTile, q0 = p0, q1 = p1;
+        const uint32_t there = decltype(full)::value ? 0u : tokens_there(key, p0, p1);
         // The last round loads its own tokens again: no branch around the loads.
-        const int s2 = min(s + 1, count - 1);
+        const int s2 = min(s + 1, count - 1), key2 = key0 + s2 * kTile;
         if (s2 != s && (s2 & 31) == 0) look_up(s2);
         p0 = page(s2, 0), p1 = page(s2, 1);
-        const int key2 = key0 + s2 * kTile;
-        const bool full = there == 0xFFFFFFFFu && key + 32 <= d.before && key > far;
-        add_tokens<HD, CODES, R>(
-            a, d, t, st, key, there, full, to_log2, lane,
+        add_tokens<decltype(full)::value, HD, CODES, R>(
+            a, d, h, t, st, key, max(q0, 0), max(q1, 0), there, to_log2, lane,
             [&] { t.load_k(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); },
             [&] { t.load_v(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); });
+        ++s;
+    };
+    while (s < count) {
+        while (s < count && (p0 | p1) >= 0 && key0 + s * kTile + 32 <= d.before &&
+               key0 + s * kTile > far)
+            round(std::true_type());
+        if (s < count) round(std::false_type());
     }
 
     // The four wavefronts' states, joined.
