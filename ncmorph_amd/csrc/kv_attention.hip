@@ -196,11 +196,23 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// The unit's queries, in the order of the products' operands (element [rr][s]
+// [lane] is lane's operand of k-step s), which the four wavefronts share; and
+// at a unit's end their states.
+template <int HD, int R>
+struct Lds {
+    static constexpr int PITCH = HD + 4;
+    union {
+        u32x4_t q[R][HD / 32][64];
+        float o[2][16 * R][PITCH];
+    };
+    float m[4][16 * R], l[4][16 * R];
+};
+
 // A wavefront's softmax state for 16 R pairs, and what it needs of them: lane
 // l holds pair l % 16 of each sixteen.
 template <int HD, int R>
 struct State {
-    bf16x8_t q[R][HD / 32];
     f32x4_t o[R][HD / 16];
     float m[R], l[R];  // l: of the lane group's own tokens
     int row[R];        // the pair's row of the request
@@ -296,9 +308,12 @@ template <bool FULL, int HD, int CODES, int R, typename NextK, typename NextV>
 __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int h,
                                            Tile<HD, CODES>& t, State<HD, R>& st, int key, int page0,
                                            int page1, uint32_t there, float to_log2, int lane,
-                                           NextK next_k, NextV next_v) {
+                                           const Lds<HD, R>& lds, NextK next_k, NextV next_v) {
     const int g = lane >> 4;
     float s[R][8];
+    // The queries are read from LDS each round: hoisted out of the loop they
+    // would take the registers that a second or third wavefront runs on.
+    asm volatile("" ::: "memory");
     {
         f32x4_t sc[R][2];
 #pragma unroll
@@ -310,7 +325,8 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
                 const bf16x8_t op = t.k_operand(half, k);
 #pragma unroll
                 for (int rr = 0; rr < R; ++rr)
-                    sc[rr][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, st.q[rr][k], sc[rr][half], 0, 0, 0);
+                    sc[rr][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        op, __builtin_bit_cast(bf16x8_t, lds.q[rr][k][lane]), sc[rr][half], 0, 0, 0);
             }
         }
 #pragma unroll
@@ -383,12 +399,6 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
     next_v();
 }
 
-template <int HD, int R>
-struct Lds {
-    static constexpr int PITCH = HD + 4;
-    float o[4][16 * R][PITCH];
-    float m[4][16 * R], l[4][16 * R];
-};
 
 // Tiles [first, first + count) of a unit, by the whole workgroup: into `out`
 // where slot < 0, else as a part.
@@ -407,8 +417,9 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
         const int row = pair / a.group, head = h * a.group + pair - row * a.group;
         const uint16_t* q = a.q + (d.q.o0 + row) * a.q_stride + (int64_t)head * HD;
 #pragma unroll
-        for (int s = 0; s < HD / 32; ++s)
-            st.q[rr][s] = __builtin_bit_cast(bf16x8_t, *(const u32x4_t*)(q + T::k_dims(s, g)));
+        for (int s = 0; s < HD / 32; ++s)  // a quarter of them by each wavefront
+            if ((rr * (HD / 32) + s) % 4 == wave)
+                lds.q[rr][s][lane] = *(const u32x4_t*)(q + T::k_dims(s, g));
 #pragma unroll
         for (int n = 0; n < HD / 16; ++n) st.o[rr][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         st.m[rr] = kNoMax;
@@ -443,6 +454,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
         if (p1 < 0) m &= 0x0000FFFFu;
         return m;
     };
+    __syncthreads();  // the queries
     T t;
     look_up(0);
     int p0 = page(0, 0), p1 = page(0, 1);
@@ -459,7 +471,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
         p0 = page(s2, 0), p1 = page(s2, 1);
         add_tokens<decltype(full)::value, HD, CODES, R>(
             a, d, h, t, st, key, max(q0, 0), max(q1, 0), there, to_log2, lane,
-            [&] { t.load_k(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); },
+            lds, [&] { t.load_k(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); },
             [&] { t.load_v(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); });
         ++s;
     };
@@ -470,13 +482,27 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
         if (s < count) round(std::false_type());
     }
 
-    // The four wavefronts' states, joined.
+    // The four wavefronts' states, joined; the queries are done with.
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
         st.l[rr] = sum_over_groups(st.l[rr]);
         if (g == 0) lds.m[wave][16 * rr + c] = st.m[rr];
     }
     __syncthreads();
+    // The upper two wavefronts' outputs to the lower two, then those to all.
+    auto put = [&] {
+#pragma unroll
+        for (int rr = 0; rr < R; ++rr)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int n = 0; n < HD / 16; n += 4) {
+                    f32x4_t v;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = st.o[rr][n + x][i];
+                    *(f32x4_t*)&lds.o[wave & 1][16 * rr + c][(HD / 16) * (4 * g + i) + n] = v;
+                }
+    };
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
         const int pr = 16 * rr + c;
@@ -484,29 +510,34 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
         const float f = __builtin_amdgcn_exp2f(st.m[rr] - top);
         if (g == 0) lds.l[wave][pr] = st.l[rr] * f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float* to = &lds.o[wave][pr][(HD / 16) * (4 * g + i)];
+        for (int n = 0; n < HD / 16; ++n) st.o[rr][n] *= f;
+    }
+    if (wave >= 2) put();
+    __syncthreads();
+    if (wave < 2) {
 #pragma unroll
-            for (int n = 0; n < HD / 16; n += 4) {
-                f32x4_t v;
+        for (int rr = 0; rr < R; ++rr)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[x] = st.o[rr][n + x][i] * f;
-                *(f32x4_t*)(to + n) = v;
-            }
-        }
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int n = 0; n < HD / 16; n += 4) {
+                    const f32x4_t v =
+                        *(const f32x4_t*)&lds.o[wave][16 * rr + c][(HD / 16) * (4 * g + i) + n];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) st.o[rr][n + x][i] += v[x];
+                }
+        put();  // where it has just read
     }
     __syncthreads();
     constexpr int CH = HD / 8;
     const int dim = 8 * (tid % CH);
     for (int pr = tid / CH; pr < min(16 * R, pairs); pr += 256 / CH) {
         float l = 0.0f;
-        f32x4_t v0 = {0.0f, 0.0f, 0.0f, 0.0f}, v1 = v0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            l += lds.l[w][pr];
-            v0 += *(const f32x4_t*)&lds.o[w][pr][dim];
-            v1 += *(const f32x4_t*)&lds.o[w][pr][dim + 4];
-        }
+        for (int w = 0; w < 4; ++w) l += lds.l[w][pr];
+        const f32x4_t v0 = *(const f32x4_t*)&lds.o[0][pr][dim] + *(const f32x4_t*)&lds.o[1][pr][dim];
+        const f32x4_t v1 =
+            *(const f32x4_t*)&lds.o[0][pr][dim + 4] + *(const f32x4_t*)&lds.o[1][pr][dim + 4];
         if (slot < 0) {
             const int pair = block * 16 * R + pr;
             const int row = pair / a.group, head = h * a.group + pair - row * a.group;
@@ -533,9 +564,8 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
 }
 
 template <int HD, int CODES, int R>
-__global__ __launch_bounds__(256, R == 4 ? 1 : R == 2 ? 2 : 3) void kv_attention_kernel(AttnArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char dyn[];
-    Lds<HD, R>& lds = *(Lds<HD, R>*)dyn;
+__global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttnArgs a) {
+    __shared__ Lds<HD, R> lds;
     __shared__ int64_t wave_tiles[4], found_at;
     __shared__ int wave_units[4], found, found_units;
     const int tid = threadIdx.x, lane = tid & 63, heads = a.cache.kv_heads;
@@ -683,12 +713,15 @@ Layout layout_of(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int q_heads) 
     Layout s;
     const int64_t group = q_heads / c.kv_heads, pairs = b.rows * group;
     const int64_t some = std::max<int64_t>(1, std::min(b.requests, b.rows));
-    // 16 R pairs a unit: as many as a request has on average, up to 64.
-    s.r16 = pairs <= 16 * some ? 1 : pairs <= 32 * some ? 2 : 4;
+    // 16 R pairs a unit. R = 2 where requests have more than 16 on average: each
+    // token's codes are widened and loaded once for twice the pairs. (R = 4, one
+    // wavefront a SIMD: 53 us against 36 for 8 trees of 25 rows and 4 heads over
+    // 4000 tokens, int8, and 148 against 142 for 256-row chunks over 8000, bf16.)
+    s.r16 = pairs <= 16 * some ? 1 : 2;
     s.units = (pairs / (16 * s.r16) + some) * c.kv_heads;
     const int64_t tiles = std::max<int64_t>(1, ((b.table_width * c.page_size) + kTile - 1) / kTile);
     s.cut = tiles > 1;
-    s.groups = std::min<int64_t>(s.units * tiles, s.r16 == 4 ? kCus : s.r16 == 2 ? 2 * kCus : 3 * kCus);
+    s.groups = std::min<int64_t>(s.units * tiles, 2 * kCus);
     const size_t slots = 2 * (size_t)s.groups * 16 * s.r16;
     s.joins = 16;
     s.ml = s.joins + 16 * (size_t)s.units;
@@ -699,14 +732,8 @@ Layout layout_of(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int q_heads) 
 
 template <int HD, int CODES, int R>
 hipError_t launch(const AttnArgs& a, const Layout& s, hipStream_t st) {
-    constexpr int lds = sizeof(Lds<HD, R>);
-    if constexpr (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void*)kv_attention_kernel<HD, CODES, R>,
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) return e;
-    }
-    kv_attention_kernel<HD, CODES, R><<<(uint32_t)s.groups, 256, lds, st>>>(a);
-    hipError_t e = hipGetLastError();
+    kv_attention_kernel<HD, CODES, R><<<(uint32_t)s.groups, 256, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.cut) return e;
     // Few units that are cut into many parts: a workgroup per pair.
     const uint32_t y = s.units * 8 <= s.groups ? 16 * R : 4 * R;
@@ -716,11 +743,7 @@ hipError_t launch(const AttnArgs& a, const Layout& s, hipStream_t st) {
 
 template <int HD, int CODES>
 hipError_t launch_r(const AttnArgs& a, const Layout& s, hipStream_t st) {
-    switch (s.r16) {
-        case 1: return launch<HD, CODES, 1>(a, s, st);
-        case 2: return launch<HD, CODES, 2>(a, s, st);
-        default: return launch<HD, CODES, 4>(a, s, st);
-    }
+    return s.r16 == 1 ? launch<HD, CODES, 1>(a, s, st) : launch<HD, CODES, 2>(a, s, st);
 }
 
 int check_attention(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch, int q_heads,

@@ -104,7 +104,7 @@ def to(r, cuda):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab,width,nb", [
     (1, 1, 1, 1), (1, 5, 3, 2), (3, 33, 40, 7), (2, 2048, 600, 0), (2, 8195, 2000, 300),
-    (5, 50257, 300, 20), (70, 1000, 64, 9), (1, 151936, 5000, 300)])
+    (5, 50257, 300, 20), (70, 1000, 64, 9), (1, 151936, 5000, 300), (128, 66003, 300, 9)])
 def test_rules(ncm, cuda, rows, vocab, width, nb, dtype):
     x = (torch.randn(rows, vocab, generator=torch.Generator().manual_seed(1)) * 4).to(dtype)
     r = rules(2, rows, rows, vocab, width, nb)
