@@ -13,33 +13,51 @@
 namespace ncm {
 namespace {
 
-// The request of a row: the number of requests that end at or before it, each
-// lane of the head counting its share of them.
-template <int LANES>
-__device__ __forceinline__ int request_of_row(const BatchView& b, int row, int lane) {
-    int n = 0;
-    for (int r = lane; r < b.requests; r += LANES) n += b.offsets[r + 1] <= row;
-#pragma unroll
-    for (int d = 1; d < LANES; d <<= 1) n += __shfl_xor(n, d);
-    return n;
-}
-
-// Where a head of a row's token lies: page and token in the page; false where
-// the row is nobody's.
+// Where a row's token lies: its page, -1 where the token is not there, and its
+// place in the page; page kNobody where the row is no request's.
+constexpr int kNobody = -2;
 struct Place {
     int page, at;
 };
-template <int LANES>
-__device__ __forceinline__ bool place_of(const BatchView& b, const KvView& c, int row, int lane,
-                                         Place& p) {
-    const int r = request_of_row<LANES>(b, row, lane);
-    if (r >= b.requests) return false;
+
+// By a whole wavefront: the request of a row is the number of requests that end
+// at or before it, 64 of them a step.
+__device__ __forceinline__ Place place_of(const BatchView& b, const KvView& c, int row, int lane) {
+    int r = 0;
+    for (int j = 0; j < b.requests; j += 64)
+        r += __popcll(__ballot(j + lane < b.requests && b.offsets[min(j + lane, b.requests - 1) + 1] <= row));
+    if (r >= b.requests) return {kNobody, 0};
     const Request q = request_of(b, r);
-    if (row < q.o0 || row >= q.o0 + q.n) return false;
+    if (row < q.o0 || row >= q.o0 + q.n) return {kNobody, 0};
     const int64_t t = (int64_t)q.before + (row - q.o0);
-    p.page = page_of(b, c, r, t);
-    p.at = (int)(t & ((1 << c.page_log2) - 1));
-    return true;
+    return {page_of(b, c, r, t), (int)(t & ((1 << c.page_log2) - 1))};
+}
+
+// A workgroup moves ROWS rows: their places first, a wavefront each, then their
+// heads, HD / 8 lanes each, K's and V's of a row after one another. f(row,
+// place, is_v, head, lane of the head).
+template <int HD, int ROWS, typename F>
+__device__ __forceinline__ void for_heads(const BatchView& b, const KvView& c, F f) {
+    __shared__ Place places[ROWS];
+    constexpr int LANES = HD / 8;
+    const int tid = threadIdx.x, first = (int)blockIdx.x * ROWS, heads = c.kv_heads;
+    for (int i = tid >> 6; i < ROWS; i += 4)
+        if (first + i < b.rows) {
+            const Place p = place_of(b, c, first + i, tid & 63);
+            if ((tid & 63) == 0) places[i] = p;
+        }
+    __syncthreads();
+    const int lane = tid % LANES, items = min(ROWS, b.rows - first) * 2 * heads;
+    int i = 0, which = tid / LANES;
+    while (which >= 2 * heads) which -= 2 * heads, ++i;
+#pragma unroll 4
+    for (int item = tid / LANES; item < items; item += 256 / LANES) {
+        const Place p = places[i];
+        const bool is_v = which >= heads;
+        if (p.page != kNobody) f(first + i, p, is_v, is_v ? which - heads : which, lane);
+        which += 256 / LANES;
+        while (which >= 2 * heads) which -= 2 * heads, ++i;
+    }
 }
 
 // Eight codes of eight values from two dwords of four.
@@ -56,21 +74,15 @@ struct WriteArgs {
     int64_t k_stride, v_stride;
 };
 
+// One head of one row.
 template <int HD, int CODES>
-__global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
-    constexpr int LANES = HD / 8, PER = 256 / LANES;
-    const int lane = threadIdx.x % LANES;
-    const int heads = a.cache.kv_heads;
-    const int64_t item = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
-    const int64_t row64 = item / (2 * heads);
-    if (row64 >= a.batch.rows) return;
-    const int row = (int)row64, which = (int)(item % (2 * heads));
-    const bool is_v = which >= heads;
-    const int h = is_v ? which - heads : which;
-    const uint16_t* src = (is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride) + h * HD + 8 * lane;
+__device__ __forceinline__ void write_head(const WriteArgs& a, int row, Place p, bool is_v, int h,
+                                           int lane) {
+    constexpr int LANES = HD / 8;
+    const uint16_t* src =
+        (is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride) + h * HD + 8 * lane;
     const u32x4_t w = *(const u32x4_t*)src;
-    Place p;
-    if (!place_of<LANES>(a.batch, a.cache, row, lane, p) || p.page < 0) return;
+    if (p.page < 0) return;
     const int64_t in_page = ((int64_t)h << a.cache.page_log2) + p.at;
     char* base = is_v ? a.cache.v : a.cache.k;
     const int64_t at = p.page * (is_v ? a.cache.v_stride : a.cache.k_stride) + in_page * HD + 8 * lane;
@@ -130,18 +142,8 @@ struct ReadArgs {
 };
 
 template <int HD, int CODES>
-__global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
-    constexpr int LANES = HD / 8, PER = 256 / LANES;
-    const int lane = threadIdx.x % LANES;
-    const int heads = a.cache.kv_heads;
-    const int64_t item = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
-    const int64_t row64 = item / (2 * heads);
-    if (row64 >= a.batch.rows) return;
-    const int row = (int)row64, which = (int)(item % (2 * heads));
-    const bool is_v = which >= heads;
-    const int h = is_v ? which - heads : which;
-    Place p;
-    if (!place_of<LANES>(a.batch, a.cache, row, lane, p)) return;
+__device__ __forceinline__ void read_head(const ReadArgs& a, int row, Place p, bool is_v, int h,
+                                          int lane) {
     u32x4_t w = {0, 0, 0, 0};
     if (p.page >= 0) {
         const int64_t in_page = ((int64_t)h << a.cache.page_log2) + p.at;
@@ -174,20 +176,50 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
     *(u32x4_t*)dst = w;
 }
 
-template <typename F>
-void by_codes(int codes, F f) {
+template <int HD, int CODES, int ROWS>
+__global__ __launch_bounds__(256) void kv_write_kernel(WriteArgs a) {
+    for_heads<HD, ROWS>(a.batch, a.cache, [&](int row, Place p, bool is_v, int h, int lane) {
+        write_head<HD, CODES>(a, row, p, is_v, h, lane);
+    });
+}
+template <int HD, int CODES, int ROWS>
+__global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
+    for_heads<HD, ROWS>(a.batch, a.cache, [&](int row, Place p, bool is_v, int h, int lane) {
+        read_head<HD, CODES>(a, row, p, is_v, h, lane);
+    });
+}
+
+template <int HD, int CODES, int ROWS>
+void start(const WriteArgs& a, uint32_t blocks, hipStream_t st) {
+    kv_write_kernel<HD, CODES, ROWS><<<blocks, 256, 0, st>>>(a);
+}
+template <int HD, int CODES, int ROWS>
+void start(const ReadArgs& a, uint32_t blocks, hipStream_t st) {
+    kv_read_kernel<HD, CODES, ROWS><<<blocks, 256, 0, st>>>(a);
+}
+
+// Rows a workgroup: four where that leaves four workgroups a CU. 49500 rows of
+// 8 heads of 128, int8, read back: 143 us (2.3 TB/s) with a search for the
+// request by every head, 77 with eight rows a workgroup, 74 (4.5 TB/s) with four.
+template <int HD, int CODES, typename Args>
+void start_rows(const Args& a, hipStream_t st) {
+    const int64_t rows = a.batch.rows;
+    if (rows >= 4 * 1024) start<HD, CODES, 4>(a, (uint32_t)((rows + 3) / 4), st);
+    else start<HD, CODES, 1>(a, (uint32_t)rows, st);
+}
+template <int HD, typename Args>
+void start_codes(const Args& a, int codes, hipStream_t st) {
     switch (codes) {
-        case NCM_KV_BF16: f(std::integral_constant<int, NCM_KV_BF16>()); break;
-        case NCM_KV_FP8: f(std::integral_constant<int, NCM_KV_FP8>()); break;
-        default: f(std::integral_constant<int, NCM_KV_INT8>()); break;
+        case NCM_KV_BF16: start_rows<HD, NCM_KV_BF16>(a, st); break;
+        case NCM_KV_FP8: start_rows<HD, NCM_KV_FP8>(a, st); break;
+        default: start_rows<HD, NCM_KV_INT8>(a, st);
     }
 }
 
-// Checks that the write and the read share, then the launch for the cache's
-// head_dim and codes.
-template <typename Args, typename Ptr, typename Launch>
+// The checks and the launch of a write or a read.
+template <typename Args, typename Ptr>
 int move_rows(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch, Ptr k,
-              Ptr v, int64_t k_stride, int64_t v_stride, const char* what, Launch go) {
+              Ptr v, int64_t k_stride, int64_t v_stride, const char* what) {
     if (!ctx) return NCM_E_NULL;
     Args a;
     int rc = check_cache(cache, &a.cache);
@@ -200,13 +232,11 @@ int move_rows(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t*
     if (!rc) rc = check_rows(v, v_stride, width);
     if (rc) return rc;
     a.k = k, a.v = v, a.k_stride = k_stride, a.v_stride = v_stride;
-    const int per = 256 / (cache->head_dim / 8);
-    const int64_t blocks = (batch->rows * 2 * cache->kv_heads + per - 1) / per;
-    if (blocks > 0x7FFFFFFF) return NCM_E_SHAPE;
     const DeviceScope scope(ncm_ctx_device(ctx));
     rc = step_hip(scope.error(), what);
     if (rc) return rc;
-    go(a, (uint32_t)blocks, ncm_ctx_stream(ctx));
+    if (cache->head_dim == 128) start_codes<128>(a, cache->codes, ncm_ctx_stream(ctx));
+    else start_codes<64>(a, cache->codes, ncm_ctx_stream(ctx));
     return step_hip(hipGetLastError(), what);
 }
 
@@ -216,31 +246,11 @@ int move_rows(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t*
 extern "C" int ncm_kv_write_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
                                 const ncm_kv_batch_t* batch, const uint16_t* k,
                                 const uint16_t* v, int64_t k_stride, int64_t v_stride) {
-    using namespace ncm;
-    return move_rows<WriteArgs>(
-        ctx, cache, batch, k, v, k_stride, v_stride, "kv_write",
-        [&](const WriteArgs& a, uint32_t blocks, hipStream_t st) {
-            by_codes(cache->codes, [&](auto c) {
-                if (cache->head_dim == 128)
-                    kv_write_kernel<128, decltype(c)::value><<<blocks, 256, 0, st>>>(a);
-                else
-                    kv_write_kernel<64, decltype(c)::value><<<blocks, 256, 0, st>>>(a);
-            });
-        });
+    return ncm::move_rows<ncm::WriteArgs>(ctx, cache, batch, k, v, k_stride, v_stride, "kv_write");
 }
 
 extern "C" int ncm_kv_read_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
                                const ncm_kv_batch_t* batch, uint16_t* k, uint16_t* v,
                                int64_t k_stride, int64_t v_stride) {
-    using namespace ncm;
-    return move_rows<ReadArgs>(
-        ctx, cache, batch, k, v, k_stride, v_stride, "kv_read",
-        [&](const ReadArgs& a, uint32_t blocks, hipStream_t st) {
-            by_codes(cache->codes, [&](auto c) {
-                if (cache->head_dim == 128)
-                    kv_read_kernel<128, decltype(c)::value><<<blocks, 256, 0, st>>>(a);
-                else
-                    kv_read_kernel<64, decltype(c)::value><<<blocks, 256, 0, st>>>(a);
-            });
-        });
+    return ncm::move_rows<ncm::ReadArgs>(ctx, cache, batch, k, v, k_stride, v_stride, "kv_read");
 }

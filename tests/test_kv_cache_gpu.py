@@ -34,7 +34,7 @@ def empty_like_step(step, cuda):
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("new,before,heads,page", [
     ([1], [0], 1, 16), ([1, 1, 1], [0, 15, 16], 2, 16), ([5, 0, 40, 1], [30, 7, 0, 63], 3, 32),
-    ([130], [1], 8, 1024), ([3] * 70, list(range(70)), 1, 16)])
+    ([130], [1], 8, 1024), ([3] * 70, list(range(70)), 1, 16), ([4099, 3], [5, 0], 1, 64)])
 def test_write_and_read(ncm, cuda, dtype, hd, new, before, heads, page):
     step = f64.Step(7, new, before, heads, hd, page, dtype, extra_rows=2)
     kv, table, offs, starts = step.to(cuda)
