@@ -563,6 +563,10 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     __syncthreads();
 }
 
+// Two workgroups a CU. (Three, in 168 registers: 122 us against 105 for 64
+// requests of up to 8192 tokens, fp8: the runs are shorter, and a run begins
+// with a chain of loads. Both of a tile's loads a round ahead, in a second
+// tile's registers: 105, and 163 against 142 us for chunks of 256 rows.)
 template <int HD, int CODES, int R>
 __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttnArgs a) {
     __shared__ Lds<HD, R> lds;
