@@ -117,6 +117,7 @@ def dims(t, name, where, ndim):
     """The shape of a tensor that must have `ndim` dimensions."""
     if t is None:
         raise NcmError(NCM_E_NULL, where, f"{name} is required")
-    if not hasattr(t, "shape") or len(t.shape) != ndim:
+    shape = getattr(t, "shape", None)
+    if shape is None or len(shape) != ndim:
         raise NcmError(NCM_E_SHAPE, where, f"{name} must have {ndim} dimensions")
-    return tuple(t.shape)
+    return tuple(shape)

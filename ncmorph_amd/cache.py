@@ -17,7 +17,6 @@ ncm_kv_cache_t and ncm_kv_batch_t say the rest. The reference has no cache
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 from . import _check as _ck
 from ._lib import NCM_E_ARG, NCM_E_SHAPE, NcmError, check, lib
@@ -41,12 +40,13 @@ class _Batch(C.Structure):
                 ("table_stride", C.c_int64)]
 
 
-def _page_stride(t, name, shape, where):
-    """Elements from a page to the next of a tensor of contiguous pages."""
+def _page_stride(t, name, shape, size, where):
+    """Elements from a page (of `size`) to the next of a tensor of contiguous
+    pages."""
     if t.shape != shape:
         raise NcmError(NCM_E_SHAPE, where, f"{name} has shape {tuple(t.shape)}, expected {shape}")
     if t.is_contiguous():
-        return math.prod(shape[1:])
+        return size
     inner, strides = 1, t.stride()
     for d in range(len(shape) - 1, 0, -1):
         if shape[d] != 1 and strides[d] != inner:
@@ -76,7 +76,8 @@ class KvCache:
                                          "float8_e4m3fn or int8")
         if getattr(v, "dtype", None) != k.dtype:
             _ck._common(v, "v", W, (name,))
-        ks, vs = _page_stride(k, "k", shape, W), _page_stride(v, "v", shape, W)
+        ks = _page_stride(k, "k", shape, heads * page * hd, W)
+        vs = _page_stride(v, "v", shape, heads * page * hd, W)
         if hd not in (64, 128):
             raise NcmError(NCM_E_SHAPE, W, "head_dim must be 64 or 128")
         if not 16 <= page <= 1024 or page & (page - 1):
@@ -90,11 +91,12 @@ class KvCache:
                                  heads, page, hd, codes)
             return
         self.named = (k, "k pages"), (v, "v pages"), (k_scale, "k_scale"), (v_scale, "v_scale")
-        for t, name in self.named[2:]:
-            if t is None:
-                raise NcmError(-1, W, f"{name} is required")
-            _ck._common(t, name, W, _ck.F32)
-        kss, vss = (_page_stride(t, name, shape[:3], W) for t, name in self.named[2:])
+        if k_scale is None or v_scale is None:
+            raise NcmError(-1, W, "k_scale and v_scale are required")
+        _ck._common(k_scale, "k_scale", W, _ck.F32)
+        _ck._common(v_scale, "v_scale", W, _ck.F32)
+        kss = _page_stride(k_scale, "k_scale", shape[:3], heads * page, W)
+        vss = _page_stride(v_scale, "v_scale", shape[:3], heads * page, W)
         self.struct = _Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                              ks, vs, kss, vss, pages, heads, page, hd, codes)
 
@@ -158,9 +160,13 @@ def read(kv: KvCache, page_table, offsets, starts, rows: int, out=None, ctx=None
     b = _batch(a, kv, page_table, offsets, starts, rows)
     width = kv.struct.kv_heads * kv.struct.head_dim
     if out is None:
-        out = torch.empty((2, rows, width), dtype=torch.bfloat16, device=kv.k.device).unbind()
-    pk, ks = _rows(a, out[0], "out[0]", rows, width)
-    pv, vs = _rows(a, out[1], "out[1]", rows, width)
+        out = torch.empty((2, rows, width), dtype=torch.bfloat16, device=kv.k.device)
+        pk, ks, vs = out.data_ptr(), width, width
+        pv = pk + 2 * rows * width
+        out = out.unbind()
+    else:
+        pk, ks = _rows(a, out[0], "out[0]", rows, width)
+        pv, vs = _rows(a, out[1], "out[1]", rows, width)
     a.done()
     ctx = stream_context(kv.k.device, ctx)
     check(lib().ncm_kv_read_dev(ctx.handle, C.byref(kv.struct), C.byref(b), pk, pv, ks, vs), W)
@@ -196,17 +202,21 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
     pp = a.dev(positions, "positions", _ck.I32, (rows,), optional=True)
     if out is None:
         out = torch.empty((rows, q_heads * hd), dtype=torch.bfloat16, device=q.device)
-    po, os_ = _rows(a, out, "out", rows, q_heads * hd)
+        po, os_ = out.data_ptr(), q_heads * hd
+    else:
+        po, os_ = _rows(a, out, "out", rows, q_heads * hd)
     need = C.c_size_t()
     check(lib().ncm_kv_attention_workspace(C.byref(kv.struct), C.byref(b), q_heads,
                                            C.byref(need)), W)
-    if workspace is None and need.value:
+    if workspace is None:
         workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    pw = a.dev(workspace, "workspace", ("uint8",), optional=True)
+        pw = workspace.data_ptr()
+    else:
+        pw = a.dev(workspace, "workspace", ("uint8",))
     a.done()
     ctx = stream_context(q.device, ctx)
     check(lib().ncm_kv_attention_dev(ctx.handle, C.byref(kv.struct), C.byref(b), pq, po, q_heads,
                                      qs, os_, hd ** -0.5 if scale is None else scale, window, pp,
                                      pm, words, pw,
-                                     0 if workspace is None else workspace.numel()), W)
+                                     workspace.numel()), W)
     return out

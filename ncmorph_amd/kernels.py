@@ -573,7 +573,9 @@ def rope_positions(x, positions, inv_freq, heads: int, head_dim: int, layout: st
     pf = a.dev(inv_freq, "inv_freq", _ck.F32, (half,))
     if out is None:
         out = torch.empty((n_rows, width), dtype=x.dtype, device=x.device)
-    po, os_ = a.rows(out, "out", (_ck._dtype(x),), n_rows, width)
+        po, os_ = out.data_ptr(), width
+    else:
+        po, os_ = a.rows(out, "out", (_ck._dtype(x),), n_rows, width)
     a.done()
     ctx = stream_context(x.device, ctx)
     check(lib().ncm_rope_positions_dev(ctx.handle, px, po, pp, pf, n_rows, heads, head_dim,
@@ -582,6 +584,9 @@ def rope_positions(x, positions, inv_freq, heads: int, head_dim: int, layout: st
                                        NCM_OUT_BF16 if x.dtype == torch.bfloat16 else NCM_OUT_F32),
           W)
     return out
+
+
+_U32 = ("int32", "uint32")
 
 
 class _LogitRules(C.Structure):
@@ -638,20 +643,26 @@ def adjust_logits(logits, history=None, prompt_lens=None, history_lens=None, rep
     if tree_mask is not None:
         _, words = _ck.dims(tree_mask, "tree_mask", W, 2)
     per, i32, f32 = (requests,), _ck.I32, _ck.F32
-    opt = [(t, n, d, s) for t, n, d, s in (
-        (offsets, "offsets", i32, (requests + 1,)), (history, "history", i32, (requests, width)),
-        (prompt_lens, "prompt_lens", i32, per), (history_lens, "history_lens", i32, per),
-        (repetition, "repetition", f32, per), (frequency, "frequency", f32, per),
-        (presence, "presence", f32, per), (bias_ids, "bias_ids", i32, (requests, nb)),
-        (bias_values, "bias_values", f32, (requests, nb)),
-        (allowed, "allowed", i32 + ("uint32",), (rows, (vocab + 31) // 32)),
-        (draft_tokens, "draft_tokens", i32, (rows,)),
-        (tree_mask, "tree_mask", _ck.U64, (rows, words)))]
-    rules = _LogitRules(*[a.dev(t, n, d, s, optional=True) for t, n, d, s in opt],
-                        requests, width, nb, words)
+    opt = a.dev
+    rules = _LogitRules(
+        opt(offsets, "offsets", i32, (requests + 1,), True),
+        opt(history, "history", i32, (requests, width), True),
+        opt(prompt_lens, "prompt_lens", i32, per, True),
+        opt(history_lens, "history_lens", i32, per, True),
+        opt(repetition, "repetition", f32, per, True),
+        opt(frequency, "frequency", f32, per, True),
+        opt(presence, "presence", f32, per, True),
+        opt(bias_ids, "bias_ids", i32, (requests, nb), True),
+        opt(bias_values, "bias_values", f32, (requests, nb), True),
+        opt(allowed, "allowed", _U32, (rows, (vocab + 31) // 32), True),
+        opt(draft_tokens, "draft_tokens", i32, (rows,), True),
+        opt(tree_mask, "tree_mask", _ck.U64, (rows, words), True),
+        requests, width, nb, words)
     if out is None:
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-    po, os_ = a.rows(out, "out", (_ck._dtype(logits),), rows, vocab)
+        po, os_ = out.data_ptr(), vocab
+    else:
+        po, os_ = a.rows(out, "out", (_ck._dtype(logits),), rows, vocab)
     a.done()
     ctx = stream_context(logits.device, ctx)
     check(lib().ncm_adjust_logits_dev(ctx.handle, C.byref(rules), pl, po, rows, vocab,
