@@ -333,8 +333,8 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
         for (int rr = 0; rr < R; ++rr)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                s[rr][i] = sc[rr][i / 4][i % 4] * to_log2;
-                if constexpr (CODES != NCM_KV_BF16) s[rr][i] = s[rr][i] * t.ks[i / 4][i % 4];
+                s[rr][i] = sc[rr][i / 4][i % 4];
+                if constexpr (CODES != NCM_KV_BF16) s[rr][i] = s[rr][i] * (t.ks[i / 4][i % 4] * to_log2);
             }
     }
     next_k();
@@ -350,11 +350,18 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
     bf16x8_t p[R];
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
-        float top = st.m[rr];
+        float top = s[rr][0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, s[rr][i]);
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[rr][i]);
         top = max_over_groups(top);
-        if (__any(top > st.m[rr])) {
+        // bf16 caches: s is the plain product, the scale is in the exponent's fma.
+        if constexpr (CODES == NCM_KV_BF16) top = top * to_log2;
+        // m follows the maximum once that has grown by 2^8: sums in fp32 and
+        // the rounding of p, a relative one, are as good to 2^8 as to 1, and o
+        // is seldom touched after the first tiles. The comparison fails for a
+        // pair that has seen nothing yet.
+        if (__any(top > st.m[rr] + 8.0f)) {
+            top = fmaxf(top, st.m[rr]);
             const float f = __builtin_amdgcn_exp2f(st.m[rr] - top);
             st.m[rr] = top;
             st.l[rr] *= f;
@@ -364,10 +371,13 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            s[rr][i] = __builtin_amdgcn_exp2f(s[rr][i] - st.m[rr]);
+            s[rr][i] = __builtin_amdgcn_exp2f(CODES == NCM_KV_BF16 ? fmaf(s[rr][i], to_log2, -st.m[rr])
+                                                                   : s[rr][i] - st.m[rr]);
+            // A scale of 0 times -inf, and 0 times a V scale that is NaN.
+            if constexpr (!FULL) s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : 0.0f;
             sum += s[rr][i];
             if constexpr (CODES != NCM_KV_BF16) s[rr][i] = s[rr][i] * t.vs[i / 4][i % 4];
-            if constexpr (CODES != NCM_KV_BF16 && !FULL)  // 0 times a scale that is NaN
+            if constexpr (CODES != NCM_KV_BF16 && !FULL)
                 s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : 0.0f;
         }
         st.l[rr] += sum;
@@ -411,6 +421,10 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     typedef Tile<HD, CODES> T;
     State<HD, R> st;
     int far = -1;  // the largest `near`
+    // A negative scale turns the queries' signs, so that the maximum of the
+    // products is that of the scores.
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+    const float to_log2 = fabsf(a.scale) * 1.4426950408889634f;
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
         const int pair = block * 16 * R + min(16 * rr + c, pairs - 1);
@@ -419,7 +433,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s)  // a quarter of them by each wavefront
             if ((rr * (HD / 32) + s) % 4 == wave)
-                lds.q[rr][s][lane] = *(const u32x4_t*)(q + T::k_dims(s, g));
+                lds.q[rr][s][lane] = *(const u32x4_t*)(q + T::k_dims(s, g)) ^ sign;
 #pragma unroll
         for (int n = 0; n < HD / 16; ++n) st.o[rr][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         st.m[rr] = kNoMax;
@@ -439,7 +453,6 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     far = uniform(far);
 
     // Pages of 16 tokens each, 32 tiles' worth at a time: lane 2 s + half.
-    const float to_log2 = a.scale * 1.4426950408889634f;
     const int key0 = (d.tile0 + first) * kTile + 32 * wave;
     int pages = -1;
     auto look_up = [&](int s) {
@@ -710,6 +723,7 @@ struct Layout {
     int64_t units;      // at most
     int64_t groups;     // workgroups
     bool cut;           // whether a unit can be
+    int64_t some;       // requests that may have rows
     size_t joins, ml, o, bytes;  // offsets in the workspace
 };
 
@@ -722,6 +736,7 @@ Layout layout_of(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int q_heads) 
     // wavefront a SIMD: 53 us against 36 for 8 trees of 25 rows and 4 heads over
     // 4000 tokens, int8, and 148 against 142 for 256-row chunks over 8000, bf16.)
     s.r16 = pairs <= 16 * some ? 1 : 2;
+    s.some = some;
     s.units = (pairs / (16 * s.r16) + some) * c.kv_heads;
     const int64_t tiles = std::max<int64_t>(1, ((b.table_width * c.page_size) + kTile - 1) / kTile);
     s.cut = tiles > 1;
@@ -739,8 +754,10 @@ hipError_t launch(const AttnArgs& a, const Layout& s, hipStream_t st) {
     kv_attention_kernel<HD, CODES, R><<<(uint32_t)s.groups, 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.cut) return e;
-    // Few units that are cut into many parts: a workgroup per pair.
-    const uint32_t y = s.units * 8 <= s.groups ? 16 * R : 4 * R;
+    // A workgroup per pair where few units are cut into many parts, else per
+    // four; of the pairs that a request has on average (the others' wait).
+    const int64_t pairs = std::min<int64_t>(16 * R, (a.batch.rows * a.group + s.some - 1) / s.some);
+    const uint32_t y = (uint32_t)(s.units * 8 <= s.groups ? pairs : (pairs + 3) / 4);
     kv_attention_join_kernel<HD, R><<<dim3((uint32_t)s.units, y), 256, 0, st>>>(a);
     return hipGetLastError();
 }

@@ -183,7 +183,7 @@ def test_infinities_of_both_signs(ncm, cuda):
     assert bool(torch.isfinite(o[:, rest]).all())
 
 
-@pytest.mark.parametrize("scale", [0.0, 0.5, 3.0])
+@pytest.mark.parametrize("scale", [0.0, 0.5, 3.0, -0.5])
 def test_scales_and_large_scores(ncm, cuda, scale):
     """Scores of hundreds: one token carries the softmax. Their fp32 rounding,
     2^-24 of the score per product and sum, moves a probability by as much:
@@ -194,7 +194,7 @@ def test_scales_and_large_scores(ncm, cuda, scale):
     out = cache.attention(q, kv, 4, table, offs, starts, scale=scale)
     ref, mag = f64.attention(step, q.cpu(), 4, f64.chain(step.new), scale=scale)
     out = out.cpu().double().reshape(ref.shape)
-    tol = f64.attention_bound(ref, mag) + 130 * 2.0 ** -24 * scale * 3200 * mag
+    tol = f64.attention_bound(ref, mag) + 130 * 2.0 ** -24 * abs(scale) * 3200 * mag
     assert bool(((out - ref).abs() <= tol).all())
 
 
