@@ -647,8 +647,8 @@ int ncm_kv_read_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_ba
 
 /* Attention of a step's rows over the cache, which holds their K and V
  * already (ncm_kv_write_dev): out = softmax(scale q.k) v over the tokens that
- * a row sees, in fp32 with one rounding to bf16 (the probabilities enter the
- * MFMA as bf16). Row i of request r, c = starts[r], sees
+ * a row sees, in fp32 with one rounding to bf16 (a probability enters the MFMA
+ * as two bf16 terms, good to 2^-16). Row i of request r, c = starts[r], sees
  *   the tokens before c, with window > 0 only those > p - window, where p =
  *   positions[row], or c + i where positions is NULL (a position below c
  *   counts as c);

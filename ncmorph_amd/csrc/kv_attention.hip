@@ -347,7 +347,7 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
             for (int i = 0; i < 8; ++i) s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : -INFINITY;
         }
     }
-    bf16x8_t p[R];
+    bf16x8_t p[R], rest[R];
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
         float top = s[rr][0];
@@ -381,12 +381,18 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
                 s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : 0.0f;
         }
         st.l[rr] += sum;
-        // To bf16 for the product: each term of the sum over tokens is off by
-        // up to 2^-9 of itself at random, below the output's own rounding.
-        u32x4_t w;
+        // As two bf16 terms for the product, the upper 8 bits and the rest: one
+        // bf16 alone would add an error as large as the output's own rounding.
+        u32x4_t hi, lo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = bf16x2_rne(s[rr][2 * i], s[rr][2 * i + 1]);
-        p[rr] = __builtin_bit_cast(bf16x8_t, w);
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = __float_as_uint(s[rr][2 * i]), y = __float_as_uint(s[rr][2 * i + 1]);
+            hi[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+            lo[i] = bf16x2_rne(s[rr][2 * i] - __uint_as_float(x & 0xFFFF0000u),
+                               s[rr][2 * i + 1] - __uint_as_float(y & 0xFFFF0000u));
+        }
+        p[rr] = __builtin_bit_cast(bf16x8_t, hi);
+        rest[rr] = __builtin_bit_cast(bf16x8_t, lo);
     }
     if constexpr (!FULL) clean_values<HD, CODES, R>(a, h, key, page0, page1, t, see, there, lane, st);
 #pragma unroll
@@ -404,6 +410,9 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
 #pragma unroll
             for (int rr = 0; rr < R; ++rr)
                 st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rr], st.o[rr][4 * f + n], 0, 0, 0);
+#pragma unroll
+            for (int rr = 0; rr < R; ++rr)
+                st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest[rr], st.o[rr][4 * f + n], 0, 0, 0);
         }
     }
     next_v();

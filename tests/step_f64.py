@@ -160,6 +160,7 @@ def attention(step, q, q_heads, allowed, window=0, positions=None, scale=None, m
 
 
 def attention_bound(ref, mag):
-    """bf16 probabilities (half a step, 2^-8, of every term), the output's own
-    rounding (2^-8), a quarter step for fp32 scores, exponentials and sums."""
-    return (2.0 ** -8 + 2.0 ** -10) * mag + 2.0 ** -8 * ref.abs() + 1e-30
+    """The output's own rounding (2^-8), and 2^-10 of sum p |v| for the fp32
+    scores (130 roundings of 2^-24 of sum |q k|), exponentials, sums and
+    probabilities of two bf16 terms (2^-16)."""
+    return 2.0 ** -10 * mag + 2.0 ** -8 * ref.abs() + 1e-30
