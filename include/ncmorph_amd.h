@@ -635,8 +635,8 @@ typedef struct ncm_kv_batch {
 
 /* Writes the K and V rows of a step into the cache, quantised. k, v: bf16
  * bits [rows, stride], kv_heads heads from column 0; strides multiples of 8,
- * 16-byte aligned. Two rows that name the same place leave either's value
- * there. Device pointers. */
+ * 16-byte aligned. What a place holds that two rows name is not defined.
+ * Device pointers. */
 int ncm_kv_write_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                      const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride);
 

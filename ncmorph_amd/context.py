@@ -77,7 +77,8 @@ def stream_context(device, ctx: Context | None = None) -> Context:
     entry points that use no workspace of the context: `ctx`, or one of this
     thread and device that only they use. It never holds a workspace, so its
     changes of stream need no event, and a call can be captured into a graph
-    whatever the default context has done before."""
+    whatever the default context has done before (but for a thread's very first
+    call on a device, which creates the context)."""
     if ctx is None:
         ctxs = getattr(_tls, "stream_ctxs", None)
         if ctxs is None:
@@ -85,6 +86,9 @@ def stream_context(device, ctx: Context | None = None) -> Context:
         index = device.index or 0
         ctx = ctxs.get(index)
         if ctx is None:
-            ctx = ctxs[index] = Context(index)
+            import torch
+
+            with torch.cuda.device(index):  # the caller's own device stays current
+                ctx = ctxs[index] = Context(index)
     ctx.bind_stream()
     return ctx

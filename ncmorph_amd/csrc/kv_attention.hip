@@ -1,7 +1,7 @@
 // Attention of a step's rows over the paged cache (ncm_kv_attention_dev).
 //
-// One pass with the running maximum and sum of a softmax:
-//   s_j = scale q.k_j (times the scale of k_j), m' = max(m, max s_j),
+// One pass with a running maximum and sum of the softmax:
+//   s_j = scale q.k_j (times the scale of k_j), m' >= max(m, max s_j) - 8,
 //   l' = l 2^(m - m') + sum 2^(s_j - m'), o' = o 2^(m - m') + sum 2^(s_j - m') v_j
 // with log2(e) folded into the scale. The query heads of a K/V head and the
 // rows of a request stand together: R times 16 (row, head) pairs are the
@@ -9,13 +9,14 @@
 // and the summed index of O^T = V^T P^T.
 //
 // Bound by the cache's bytes for one token a request, so K and V go from
-// memory to registers, each read once, without LDS between: the lane layout of S^T (a column's
-// four tokens g * 4 .. + 3 in lane group g) is that of the second product's
-// P^T operand if its summed index runs over the tokens in the order the lanes
-// hold them, and a lane then needs of V those same tokens' values of its own
-// dims, which are its own rows' loads, their 16-bit halves regrouped with
-// v_perm_b32. 8-bit codes are widened to bf16 in registers (exact); their
-// scales multiply scores and probabilities, not values.
+// memory to registers, each read once, without LDS between: the lane layout of
+// S^T (a column's four tokens 4 g .. 4 g + 3 in lane group g) is that of the
+// second product's P^T operand if its summed index runs over the tokens in the
+// order the lanes hold them, and a lane then needs of V those same tokens'
+// values of its own dims, which are its own rows' loads, their 16-bit halves
+// regrouped with v_perm_b32. 8-bit codes are widened to bf16 in registers
+// (exact); their scales multiply scores and probabilities, not values. The
+// queries, which all four wavefronts read, are in LDS.
 //
 // Work: a request's (K/V head, block of 16 R pairs) is a unit of ceil(tokens /
 // 128) tiles; all units' tiles in a row are cut into equal runs, one per
@@ -23,6 +24,14 @@
 // tokens of each tile. A unit inside one run is written out, the parts of one
 // that is cut go to the workspace, and kv_attention_join_kernel adds them in
 // order.
+//
+// 64 requests of 1024 to 8192 tokens, one row each, 32 heads over 8 of 128, fp8:
+// 105 us (4.7 TB/s; a copy runs at 5.1). Trees of 25 rows over 2000 to 4000
+// tokens, int8, 8 requests: 36 us; chunks of 256 rows over 8000, bf16, 2
+// requests: 143 us (290 TFLOP/s of unmasked products). Those two are bound by the
+// instructions around the products: per 32 tokens and 32 pairs some 300 vector
+// instructions (exponentials, maxima, regrouping, widening) beside 48 MFMAs, two
+// wavefronts a SIMD.
 #include "step.h"
 
 namespace ncm {
@@ -388,8 +397,12 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
         for (int i = 0; i < 4; ++i) {
             const uint32_t x = __float_as_uint(s[rr][2 * i]), y = __float_as_uint(s[rr][2 * i + 1]);
             hi[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
-            lo[i] = bf16x2_rne(s[rr][2 * i] - __uint_as_float(x & 0xFFFF0000u),
-                               s[rr][2 * i + 1] - __uint_as_float(y & 0xFFFF0000u));
+            // (1 + 2^-20) p less the upper term: above 0 wherever p is, so that
+            // an infinite value times it is no NaN.
+            lo[i] = bf16x2_rne(fmaf(s[rr][2 * i], 1.00000095367431640625f,
+                                    -__uint_as_float(x & 0xFFFF0000u)),
+                               fmaf(s[rr][2 * i + 1], 1.00000095367431640625f,
+                                    -__uint_as_float(y & 0xFFFF0000u)));
         }
         p[rr] = __builtin_bit_cast(bf16x8_t, hi);
         rest[rr] = __builtin_bit_cast(bf16x8_t, lo);
@@ -593,30 +606,27 @@ template <int HD, int CODES, int R>
 __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttnArgs a) {
     __shared__ Lds<HD, R> lds;
     __shared__ int64_t wave_tiles[4], found_at;
-    __shared__ int wave_units[4], found, found_units;
+    __shared__ int64_t wave_units[4], found_units;
+    __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 63, heads = a.cache.kv_heads;
 
     // Tiles and units ahead of each thread's share of the requests.
     const int per = (a.batch.requests + 255) / 256, r0 = tid * per;
     const int r1 = min(r0 + per, a.batch.requests);
-    int64_t tiles = 0;
-    int units = 0;
+    int64_t tiles = 0, units = 0;
     for (int r = r0; r < r1; ++r) {
         const Need d = need_of<R>(a, r);
-        units += d.blocks * heads;
+        units += (int64_t)d.blocks * heads;
         tiles += (int64_t)d.blocks * heads * d.tiles;
     }
-    int64_t t_sum = tiles;
-    int u_sum = units;
+    int64_t t_sum = tiles, u_sum = units;
     for (int x = 1; x < 64; x <<= 1) {
-        const int64_t t = __shfl_up(t_sum, x);
-        const int u = __shfl_up(u_sum, x);
+        const int64_t t = __shfl_up(t_sum, x), u = __shfl_up(u_sum, x);
         if (lane >= x) t_sum += t, u_sum += u;
     }
     if (lane == 63) wave_tiles[tid >> 6] = t_sum, wave_units[tid >> 6] = u_sum;
     __syncthreads();
-    int64_t all = 0, t_at = t_sum - tiles;
-    int all_units = 0, u_at = u_sum - units;
+    int64_t all = 0, t_at = t_sum - tiles, all_units = 0, u_at = u_sum - units;
     for (int w = 0; w < 4; ++w) {
         if (w < (tid >> 6)) t_at += wave_tiles[w], u_at += wave_units[w];
         all += wave_tiles[w], all_units += wave_units[w];
@@ -626,7 +636,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttnArgs a) {
     // may read the same K and V, on one XCD where every workgroup has a run.
     const int64_t groups = min((int64_t)gridDim.x, all);
     const int me = all >= gridDim.x ? xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
-    if (blockIdx.x == 0 && tid == 0) *a.unit_count = min(all_units, a.units);
+    if (blockIdx.x == 0 && tid == 0) *a.unit_count = (int)min(all_units, (int64_t)a.units);
     if (me >= groups) return;
     int64_t at = all * me / groups;
     const int64_t end = all * (me + 1) / groups;
@@ -636,18 +646,18 @@ __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttnArgs a) {
             const Need d = need_of<R>(a, r);
             const int64_t n = (int64_t)d.blocks * heads * d.tiles;
             if (at < t_at + n) break;
-            t_at += n, u_at += d.blocks * heads;
+            t_at += n, u_at += (int64_t)d.blocks * heads;
         }
         found = r, found_at = t_at, found_units = u_at;
     }
     __syncthreads();
-    int r = uniform(found), u0 = uniform(found_units);
-    int64_t start = uniform(found_at);  // of the request's tiles
+    int r = uniform(found);
+    int64_t start = uniform(found_at), u0 = uniform(found_units);  // of the request
     while (at < end) {
         const Need d = need_of<R>(a, r);
         const int64_t n = (int64_t)d.blocks * heads * d.tiles;
         if (at >= start + n) {
-            start += n, u0 += d.blocks * heads, ++r;
+            start += n, u0 += (int64_t)d.blocks * heads, ++r;
             continue;
         }
         const int u = (int)((at - start) / d.tiles);
@@ -824,6 +834,11 @@ extern "C" int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
     if (!rc) rc = check_rows(out, out_stride, width);
     if (rc) return rc;
     const Layout s = layout_of(*cache, *batch, q_heads);
+    // Offsets may give every request all rows: the tiles must still be counted
+    // in 64 bits, times the workgroups.
+    const double most = ((double)batch->rows * q_heads / 16 + cache->kv_heads) * batch->requests *
+                        ((double)a.batch.capacity / kTile + 1);
+    if (most > 0x1p50 || s.units > 0x7FFFFFFF) return NCM_E_SHAPE;
     if (!workspace) return NCM_E_NULL;
     if (workspace_bytes < s.bytes) return NCM_E_LENGTH;
     if ((uintptr_t)workspace % 16) return NCM_E_ARG;

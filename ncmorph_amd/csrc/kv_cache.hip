@@ -7,7 +7,9 @@
 // of a correctly rounded quotient of exact operands (a bf16 value times 127 has
 // 15 bits), so x = m / 2, a tie, rounds as it does in real numbers.
 //
-// Memory bound: a bf16 value in and its code out, or the other way.
+// Memory bound: a bf16 value in and its code out, or the other way. 14700 rows of
+// 8 heads of 128, e4m3: written in 24 us (3.8 TB/s of values, codes and scales),
+// read in 19 (4.8).
 #include "step.h"
 
 namespace ncm {
@@ -50,7 +52,6 @@ __device__ __forceinline__ void for_heads(const BatchView& b, const KvView& c, F
     const int lane = tid % LANES, items = min(ROWS, b.rows - first) * 2 * heads;
     int i = 0, which = tid / LANES;
     while (which >= 2 * heads) which -= 2 * heads, ++i;
-#pragma unroll 4
     for (int item = tid / LANES; item < items; item += 256 / LANES) {
         const Place p = places[i];
         const bool is_v = which >= heads;

@@ -183,6 +183,24 @@ def test_infinities_of_both_signs(ncm, cuda):
     assert bool(torch.isfinite(o[:, rest]).all())
 
 
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("before", [0, 200])
+def test_values_that_are_not_finite_where_all_see_them(ncm, cuda, value, before):
+    """The column of the value holds it, the others what they would without."""
+    step = f64.Step(22, [1, 3], [before, 70], 1, 64, 16, BF16)
+    q = queries(step, 2, cuda)
+    ref, mag = f64.attention(step, q.cpu(), 2, f64.chain(step.new))
+    for r in range(2):
+        step.pages[1][int(step.table[r, 0]), 0, 0, 5] = value
+    kv, table, offs, starts = step.to(cuda)
+    o = cache.attention(q, kv, 2, table, offs, starts).cpu().double().reshape(4, 2, 64)
+    col = o[..., 5]
+    assert bool(torch.isnan(col).all()) if math.isnan(value) else bool((col == value).all())
+    rest = torch.arange(64) != 5
+    err, tol = (o - ref).abs()[..., rest], f64.attention_bound(ref, mag)[..., rest]
+    assert bool((err <= tol).all())
+
+
 @pytest.mark.parametrize("scale", [0.0, 0.5, 3.0, -0.5])
 def test_scales_and_large_scores(ncm, cuda, scale):
     """Scores of hundreds: one token carries the softmax. Their fp32 rounding,
