@@ -168,13 +168,29 @@ struct Tile {
     static __device__ __forceinline__ int k_dims(int s, int g) {
         return CODES == NCM_KV_BF16 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
     }
-    // Dims 2 x and 2 x + 1 of the lane's HD / 16, x = 2 f .. 2 f + 1, of the
-    // eight tokens, as bf16 pairs.
-    __device__ __forceinline__ void v_pairs(int f, uint32_t (&w)[8][2]) const {
+    // The operands of V^T for dims 4 f + n of the lane's HD / 16: w[n][j] holds
+    // the bf16 of tokens 2 j and 2 j + 1 of the lane's eight.
+    __device__ __forceinline__ void v_operands(int f, uint32_t (&w)[4][4]) const {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (CODES == NCM_KV_BF16) w[i][0] = v[i][2 * f], w[i][1] = v[i][2 * f + 1];
-            else widen4<CODES>(v[i][f], w[i][0], w[i][1]);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (CODES == NCM_KV_BF16) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    w[n][j] = __builtin_amdgcn_perm(v[2 * j + 1][2 * f + n / 2], v[2 * j][2 * f + n / 2],
+                                                    n % 2 ? 0x07060302u : 0x05040100u);
+            } else if constexpr (CODES == NCM_KV_FP8) {
+                // The two tokens' bytes side by side, then widened in pairs.
+                const uint32_t lo = __builtin_amdgcn_perm(v[2 * j + 1][f], v[2 * j][f], 0x05010400u);
+                const uint32_t hi = __builtin_amdgcn_perm(v[2 * j + 1][f], v[2 * j][f], 0x07030602u);
+                widen4<CODES>(lo, w[0][j], w[1][j]);
+                widen4<CODES>(hi, w[2][j], w[3][j]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    w[n][j] = __builtin_amdgcn_perm(
+                        __float_as_uint((float)(int8_t)(v[2 * j + 1][f] >> (8 * n))),
+                        __float_as_uint((float)(int8_t)(v[2 * j][f] >> (8 * n))), 0x07060302u);
+            }
         }
     }
 };
@@ -410,16 +426,11 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
     if constexpr (!FULL) clean_values<HD, CODES, R>(a, h, key, page0, page1, t, see, there, lane, st);
 #pragma unroll
     for (int f = 0; f < HD / 64; ++f) {
-        uint32_t w[8][2];
-        t.v_pairs(f, w);
+        uint32_t w[4][4];
+        t.v_operands(f, w);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            u32x4_t b;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                b[j] = __builtin_amdgcn_perm(w[2 * j + 1][n / 2], w[2 * j][n / 2],
-                                             n % 2 ? 0x07060302u : 0x05040100u);
-            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, b);
+            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, u32x4_t{w[n][0], w[n][1], w[n][2], w[n][3]});
 #pragma unroll
             for (int rr = 0; rr < R; ++rr)
                 st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rr], st.o[rr][4 * f + n], 0, 0, 0);
