@@ -107,10 +107,13 @@ class Args:
         return t.data_ptr(), stride
 
     def done(self):
-        device = self.seen[0][0].device if self.seen else None
+        if not self.seen:
+            return
+        first = self.seen[0][0]
+        index = first.get_device() if first.is_cuda else -2
         for t, name in self.seen:
-            if not t.is_cuda or t.device != device:
-                _placed(t, name, self.where, device)
+            if t.get_device() != index or not t.is_cuda:
+                _placed(t, name, self.where, first.device)
 
 
 def dims(t, name, where, ndim):

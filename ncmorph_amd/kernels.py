@@ -9,6 +9,10 @@ ABI; nothing here computes on the CPU.
 `linear_bf16` / `linear_f32` are the device-resident paths: torch tensors
 already in HBM, bf16 (or fp32) operands, fp32 (or bf16) output,
 stream-ordered on torch's current stream.
+
+`rope_positions` and `adjust_logits` belong to a step that continues sequences
+over ncmorph_amd.cache: they take torch tensors, use no workspace and can be
+captured into a graph.
 """
 from __future__ import annotations
 
