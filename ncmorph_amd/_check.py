@@ -97,9 +97,10 @@ class Args:
             raise NcmError(NCM_E_NULL, W, f"{name} is required")
         if getattr(t, "dtype", None) not in _ACCEPTED[dtypes]:
             _common(t, name, W, dtypes)
-        if t.dim() != 2 or t.shape[0] != n_rows or t.shape[1] < min_cols:
+        shape = t.shape
+        if len(shape) != 2 or shape[0] != n_rows or shape[1] < min_cols:
             raise NcmError(NCM_E_SHAPE, W,
-                           f"{name} has shape {tuple(t.shape)}, expected ({n_rows}, >= {min_cols})")
+                           f"{name} has shape {tuple(shape)}, expected ({n_rows}, >= {min_cols})")
         stride, inner = t.stride()
         if inner != 1 or (n_rows > 1 and stride < min_cols):
             raise NcmError(NCM_E_ARG, W, f"{name} must have contiguous, non-overlapping rows")

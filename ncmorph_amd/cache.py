@@ -160,10 +160,9 @@ def read(kv: KvCache, page_table, offsets, starts, rows: int, out=None, ctx=None
     b = _batch(a, kv, page_table, offsets, starts, rows)
     width = kv.struct.kv_heads * kv.struct.head_dim
     if out is None:
-        out = torch.empty((2, rows, width), dtype=torch.bfloat16, device=kv.k.device)
-        pk, ks, vs = out.data_ptr(), width, width
-        pv = pk + 2 * rows * width
-        out = out.unbind()
+        out = (torch.empty(rows, width, dtype=torch.bfloat16, device=kv.k.device),
+               torch.empty(rows, width, dtype=torch.bfloat16, device=kv.k.device))
+        pk, pv, ks, vs = out[0].data_ptr(), out[1].data_ptr(), width, width
     else:
         pk, ks = _rows(a, out[0], "out[0]", rows, width)
         pv, vs = _rows(a, out[1], "out[1]", rows, width)
@@ -200,14 +199,14 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
         _, words = _ck.dims(tree_mask, "tree_mask", W, 2)
     pm = a.dev(tree_mask, "tree_mask", _ck.U64, (rows, words), optional=True)
     pp = a.dev(positions, "positions", _ck.I32, (rows,), optional=True)
-    if out is None:
-        out = torch.empty((rows, q_heads * hd), dtype=torch.bfloat16, device=q.device)
-        po, os_ = out.data_ptr(), q_heads * hd
-    else:
-        po, os_ = _rows(a, out, "out", rows, q_heads * hd)
     need = C.c_size_t()
     check(lib().ncm_kv_attention_workspace(C.byref(kv.struct), C.byref(b), q_heads,
                                            C.byref(need)), W)
+    if out is None:
+        out = torch.empty(rows, q_heads * hd, dtype=torch.bfloat16, device=q.device)
+        po, os_ = out.data_ptr(), q_heads * hd
+    else:
+        po, os_ = _rows(a, out, "out", rows, q_heads * hd)
     if workspace is None:
         workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
         pw = workspace.data_ptr()

@@ -576,7 +576,7 @@ def rope_positions(x, positions, inv_freq, heads: int, head_dim: int, layout: st
     pp = a.dev(positions, "positions", _ck.I32, (n_rows,))
     pf = a.dev(inv_freq, "inv_freq", _ck.F32, (half,))
     if out is None:
-        out = torch.empty((n_rows, width), dtype=x.dtype, device=x.device)
+        out = torch.empty(n_rows, width, dtype=x.dtype, device=x.device)
         po, os_ = out.data_ptr(), width
     else:
         po, os_ = a.rows(out, "out", (_ck._dtype(x),), n_rows, width)
@@ -663,7 +663,7 @@ def adjust_logits(logits, history=None, prompt_lens=None, history_lens=None, rep
         opt(tree_mask, "tree_mask", _ck.U64, (rows, words), True),
         requests, width, nb, words)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
         po, os_ = out.data_ptr(), vocab
     else:
         po, os_ = a.rows(out, "out", (_ck._dtype(logits),), rows, vocab)
