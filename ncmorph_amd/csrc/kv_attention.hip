@@ -762,9 +762,11 @@ Layout layout_of(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int q_heads) 
     const int64_t group = q_heads / c.kv_heads, pairs = b.rows * group;
     const int64_t some = std::max<int64_t>(1, std::min(b.requests, b.rows));
     // 16 R pairs a unit. R = 2 where requests have more than 16 on average: each
-    // token's codes are widened and loaded once for twice the pairs. (R = 4, one
-    // wavefront a SIMD: 53 us against 36 for 8 trees of 25 rows and 4 heads over
-    // 4000 tokens, int8, and 148 against 142 for 256-row chunks over 8000, bf16.)
+    // token's codes are loaded and widened once for twice the pairs. R = 1 and 2:
+    // 41 and 36 us for 8 trees of 25 rows and 4 heads over 4000 tokens, int8, 235
+    // and 143 for 256-row chunks over 8000, bf16; with one row a request, 105 and
+    // 116 for 64 of them, fp8, 8.0 and 10.1 for one over 777 tokens. (R = 4, one
+    // wavefront a SIMD: 53 for the trees, 148 for the chunks.)
     s.r16 = pairs <= 16 * some ? 1 : 2;
     s.some = some;
     s.units = (pairs / (16 * s.r16) + some) * c.kv_heads;

@@ -199,9 +199,11 @@ void start(const ReadArgs& a, uint32_t blocks, hipStream_t st) {
     kv_read_kernel<HD, CODES, ROWS><<<blocks, 256, 0, st>>>(a);
 }
 
-// Rows a workgroup: four where that leaves four workgroups a CU. 49500 rows of
-// 8 heads of 128, int8, read back: 143 us (2.3 TB/s) with a search for the
-// request by every head, 77 with eight rows a workgroup, 74 (4.5 TB/s) with four.
+// Rows a workgroup: four where that leaves four workgroups a CU, for one search
+// and its chain of loads for four times the bytes. One, four and eight: 90, 74
+// and 77 us for 49500 rows of 8 heads of 128, int8, read back (143 with a search
+// by every head), 27, 24 and 25 for 14700 rows, e4m3, written; one and four: 4.2
+// and 7.7 us for 48 rows written.
 template <int HD, int CODES, typename Args>
 void start_rows(const Args& a, hipStream_t st) {
     const int64_t rows = a.batch.rows;

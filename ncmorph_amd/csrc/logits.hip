@@ -233,7 +233,9 @@ __global__ __launch_bounds__(threads_of(BF16, SLICE)) void adjust_logits_kernel(
     }
 }
 
-// Slices small enough for four workgroups a CU.
+// Slices of 8192 tokens where that leaves four workgroups a CU: the history is
+// read once a slice. 8192 and 2048: 51 and 71 us for 200 rows of 151936 float32,
+// 8.1 and 6.4 for 4 rows of 128256.
 int slice_of(int64_t rows, int64_t vocab) {
     return rows * (vocab / 8192 + 1) >= 1024 ? 8192 : 2048;
 }

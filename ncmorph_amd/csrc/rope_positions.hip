@@ -202,7 +202,9 @@ extern "C" int ncm_rope_positions_dev(ncm_ctx_t* ctx, const void* x, void* y,
     const int step = wide ? n : 1;
     a.turn_units = half / step;
     a.units = a.turn_units + (x == y ? 0 : (head_dim - rot_dim) / step);
-    // Heads a thread turns: as many as leave 512 threads a CU.
+    // Heads a thread turns: as many as leave 512 threads a CU, up to eight. One
+    // and eight: 6.6 us with eight against 3.6 for 4 rows of 40 heads of 64; 35.8
+    // with one against 35.7 for 8192 rows of 128 (the memory bounds both).
     const int64_t all = rows * a.units * heads;
     const int64_t each = std::min<int64_t>(8, std::max<int64_t>(1, all / (256 * 512)));
     a.head_groups = (int)((heads + each - 1) / each);
