@@ -576,7 +576,8 @@ enum { NCM_ROPE_HALF = 0, NCM_ROPE_INTERLEAVED = 1 };
  * (dtype NCM_OUT_F32) or bf16 bits (NCM_OUT_BF16); y may be x, and must not
  * overlap it otherwise. Values of a head behind rot_dim are copied.
  * positions: int32 [rows], of either sign; inv_freq: float [rot_dim / 2].
- * rot_dim even, 0 < rot_dim <= head_dim. Any stride and alignment; the
+ * rot_dim even, 0 < rot_dim <= head_dim; rows * heads * head_dim at most 2^32.
+ * Any stride and alignment; the
  * 16-byte path needs 16-byte aligned x, y, rows and heads. Device pointers. */
 int ncm_rope_positions_dev(ncm_ctx_t* ctx, const void* x, void* y, const int32_t* positions,
                            const float* inv_freq, int64_t rows, int heads, int head_dim,

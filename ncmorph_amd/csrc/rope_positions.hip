@@ -7,10 +7,10 @@
 // of sine and cosine to x^9 and x^10 are exact to 2^-25. Pairs are turned in
 // fp32 with one rounding at the end.
 //
-// Memory bound: rows * heads * head_dim values in and out. A thread owns a few
-// pairs of a row, computes their sines once and turns them in several heads
-// of that row, where there are rows enough to fill the GPU that way. 8192 rows of
-// 40 heads of 128, bf16, interleaved: 35.7 us (4.7 TB/s; a copy runs at 5.1).
+// Memory bound: rows * heads * head_dim values in and out. A thread turns 32
+// bytes of one head, sines and all: sharing them among eight heads of a row gave
+// nothing for 8192 rows of 40 heads of 128, bf16, interleaved (33.5 us, 5.0 TB/s; a
+// copy runs at 5.1), and took 6.6 us against 3.5 for 4 rows.
 #include "step.h"
 
 namespace ncm {
@@ -48,7 +48,6 @@ struct RopeArgs {
     int heads, head_dim, half;
     int units;        // threads that cover a head: turned ones, then copied ones
     int turn_units;
-    int head_groups;  // threads that share a row's heads
     float scale;
 };
 
@@ -99,21 +98,18 @@ __global__ __launch_bounds__(256) void rope_positions_kernel(RopeArgs a) {
     typedef Vec<BF16> V;
     typedef typename V::elem T;
     constexpr int N = WIDE ? V::N : 1;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int u = (int)(id % a.units);
-    const int64_t rest = id / a.units;
-    const int hg = (int)(rest % a.head_groups);
-    const int64_t row = rest / a.head_groups;
+    // In 32 bits, whose division is far shorter: 33.5 us against 35.8.
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, rest = id / (uint32_t)a.units;
+    const int u = (int)(id % (uint32_t)a.units);
+    const int64_t row = rest / (uint32_t)a.heads;
     if (row >= a.rows) return;
-    const T* x = (const T*)a.x + row * a.x_stride;
-    T* y = (T*)a.y + row * a.y_stride;
+    const int64_t head = (int64_t)(rest % (uint32_t)a.heads) * a.head_dim;
+    const T* x = (const T*)a.x + row * a.x_stride + head;
+    T* y = (T*)a.y + row * a.y_stride + head;
     if (u >= a.turn_units) {  // behind the rotated part: copied
         const int at = 2 * a.half + (u - a.turn_units) * N;
-        for (int h = hg; h < a.heads; h += a.head_groups) {
-            const int64_t o = (int64_t)h * a.head_dim + at;
-            if constexpr (WIDE) *(u32x4_t*)(y + o) = *(const u32x4_t*)(x + o);
-            else y[o] = x[o];
-        }
+        if constexpr (WIDE) *(u32x4_t*)(y + at) = *(const u32x4_t*)(x + at);
+        else y[at] = x[at];
         return;
     }
     const int p0 = u * N;
@@ -124,39 +120,35 @@ __global__ __launch_bounds__(256) void rope_positions_kernel(RopeArgs a) {
         sincos_turns(pos * (double)a.inv_freq[p0 + i] * 0.15915494309189535, a.scale, c[i], s[i]);
     const int first = INTERLEAVED ? 2 * p0 : p0;
     const int second = INTERLEAVED ? (WIDE ? 2 * p0 + N : 2 * p0 + 1) : a.half + p0;
-#pragma unroll 2
-    for (int h = hg; h < a.heads; h += a.head_groups) {
-        const int64_t o = (int64_t)h * a.head_dim;
-        if constexpr (WIDE) {
-            float f[N], g[N];
-            V::load(x + o + first, f);
-            V::load(x + o + second, g);
-            if constexpr (INTERLEAVED) {
+    if constexpr (WIDE) {
+        float f[N], g[N];
+        V::load(x + first, f);
+        V::load(x + second, g);
+        if constexpr (INTERLEAVED) {
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i) {
-                    const float e = f[2 * i], d = f[2 * i + 1];
-                    f[2 * i] = fmaf(e, c[i], -(d * s[i]));
-                    f[2 * i + 1] = fmaf(d, c[i], e * s[i]);
-                    const int j = N / 2 + i;
-                    const float e2 = g[2 * i], d2 = g[2 * i + 1];
-                    g[2 * i] = fmaf(e2, c[j], -(d2 * s[j]));
-                    g[2 * i + 1] = fmaf(d2, c[j], e2 * s[j]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float e = f[i], d = g[i];
-                    f[i] = fmaf(e, c[i], -(d * s[i]));
-                    g[i] = fmaf(d, c[i], e * s[i]);
-                }
+            for (int i = 0; i < N / 2; ++i) {
+                const float e = f[2 * i], d = f[2 * i + 1];
+                f[2 * i] = fmaf(e, c[i], -(d * s[i]));
+                f[2 * i + 1] = fmaf(d, c[i], e * s[i]);
+                const int j = N / 2 + i;
+                const float e2 = g[2 * i], d2 = g[2 * i + 1];
+                g[2 * i] = fmaf(e2, c[j], -(d2 * s[j]));
+                g[2 * i + 1] = fmaf(d2, c[j], e2 * s[j]);
             }
-            V::store(y + o + first, f);
-            V::store(y + o + second, g);
         } else {
-            const float e = V::get(x + o + first), d = V::get(x + o + second);
-            V::put(y + o + first, fmaf(e, c[0], -(d * s[0])));
-            V::put(y + o + second, fmaf(d, c[0], e * s[0]));
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float e = f[i], d = g[i];
+                f[i] = fmaf(e, c[i], -(d * s[i]));
+                g[i] = fmaf(d, c[i], e * s[i]);
+            }
         }
+        V::store(y + first, f);
+        V::store(y + second, g);
+    } else {
+        const float e = V::get(x + first), d = V::get(x + second);
+        V::put(y + first, fmaf(e, c[0], -(d * s[0])));
+        V::put(y + second, fmaf(d, c[0], e * s[0]));
     }
 }
 
@@ -185,6 +177,7 @@ extern "C" int ncm_rope_positions_dev(ncm_ctx_t* ctx, const void* x, void* y,
         head_dim > 65536 || rot_dim <= 0 || rot_dim % 2 || rot_dim > head_dim)
         return NCM_E_SHAPE;
     const int64_t width = (int64_t)heads * head_dim;
+    if (width > 0 && rows > (int64_t(1) << 32) / width) return NCM_E_SHAPE;
     if (x_stride < width || y_stride < width || x_stride > (int64_t(1) << 40) ||
         y_stride > (int64_t(1) << 40))
         return NCM_E_SHAPE;
@@ -198,18 +191,11 @@ extern "C" int ncm_rope_positions_dev(ncm_ctx_t* ctx, const void* x, void* y,
     const bool wide = !(((uintptr_t)x | (uintptr_t)y) % 16) && x_stride % n == 0 &&
                       y_stride % n == 0 && head_dim % n == 0 && half % n == 0;
     RopeArgs a = {x, y, positions, inv_freq, rows, x_stride, y_stride, heads, head_dim, half,
-                  0, 0, 0, scale};
+                  0, 0, scale};
     const int step = wide ? n : 1;
     a.turn_units = half / step;
     a.units = a.turn_units + (x == y ? 0 : (head_dim - rot_dim) / step);
-    // Heads a thread turns: as many as leave 512 threads a CU, up to eight. One
-    // and eight: 6.6 us with eight against 3.6 for 4 rows of 40 heads of 64; 35.8
-    // with one against 35.7 for 8192 rows of 128 (the memory bounds both).
-    const int64_t all = rows * a.units * heads;
-    const int64_t each = std::min<int64_t>(8, std::max<int64_t>(1, all / (256 * 512)));
-    a.head_groups = (int)((heads + each - 1) / each);
-    const int64_t blocks = (rows * a.units * a.head_groups + 255) / 256;
-    if (blocks > 0x7FFFFFFF) return NCM_E_SHAPE;
+    const int64_t blocks = (rows * a.units * heads + 255) / 256;
     const DeviceScope scope(ncm_ctx_device(ctx));
     int rc = step_hip(scope.error(), "rope_positions device");
     if (rc) return rc;

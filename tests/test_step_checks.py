@@ -114,7 +114,7 @@ def test_library_refuses(ncm):
         ("ctx", "x", "y", "pos", "inv", "rows", "heads", "hd", "rot", "xs", "ys", "lay", "scale",
          "dt")])
     assert R(ctx=no) == NCM_E_NULL and R(x=no) == NCM_E_NULL and R(inv=no) == NCM_E_NULL
-    for bad in (dict(rows=-1), dict(rows=1 << 31), dict(rot=63), dict(rot=66), dict(rot=0),
+    for bad in (dict(rows=-1), dict(rows=1 << 31), dict(rows=(1 << 25) + 1), dict(rot=63), dict(rot=66), dict(rot=0),
                 dict(xs=127), dict(ys=127), dict(heads=-1), dict(hd=0)):
         assert R(**bad) == NCM_E_SHAPE, bad
     for bad in (dict(lay=2), dict(dt=1), dict(ys=130)):
