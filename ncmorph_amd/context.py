@@ -4,7 +4,7 @@ from __future__ import annotations
 import ctypes as C
 import threading
 
-from ._lib import check, lib
+from ._lib import NCM_E_ARG, NcmError, check, lib
 
 
 _raw_stream = None
@@ -79,11 +79,15 @@ def stream_context(device, ctx: Context | None = None) -> Context:
     changes of stream need no event, and a call can be captured into a graph
     whatever the default context has done before (but for a thread's very first
     call on a device, which creates the context)."""
-    if ctx is None:
+    index = device.index or 0
+    if ctx is not None:
+        if ctx.device != index:
+            raise NcmError(NCM_E_ARG, "ctx", f"a context of device {ctx.device} cannot run on "
+                                             f"tensors of {device}")
+    else:
         ctxs = getattr(_tls, "stream_ctxs", None)
         if ctxs is None:
             ctxs = _tls.stream_ctxs = {}
-        index = device.index or 0
         ctx = ctxs.get(index)
         if ctx is None:
             import torch

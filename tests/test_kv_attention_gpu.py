@@ -261,6 +261,32 @@ def test_rows_of_no_request_and_other_columns_stay(ncm, cuda):
     assert bool((buf.cpu()[rest] == 9.0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layers_in_one_buffer_and_a_slice_of_a_table(ncm, cuda, dtype):
+    """K, V and scales as parts of wider buffers that hold NaN elsewhere, the
+    page table as columns of a wider one."""
+    step = f64.Step(23, [3, 1, 6], [200, 90, 0], 2, 64, 32, dtype)
+    q = queries(step, 4, cuda)
+    kv, table, offs, starts = step.to(cuda)
+    ref = cache.attention(q, kv, 4, table, offs, starts)
+    held(ref, step, 4, *f64.attention(step, q.cpu(), 4, f64.chain(step.new)))
+    pages = kv.k.shape[0]
+    byte = torch.full((pages, 3, 2, *kv.k.shape[1:]), 127, dtype=torch.uint8, device=cuda)
+    wide = byte.view(dtype) if dtype != BF16 else torch.full(byte.shape, math.nan, dtype=BF16,
+                                                              device=cuda)
+    wide[:, 1, 0], wide[:, 1, 1] = kv.k, kv.v
+    scales = (None, None)
+    if dtype != BF16:
+        sc = torch.full((pages, 2, 2, *kv.k_scale.shape[1:]), math.nan, device=cuda)
+        sc[:, 1, 0], sc[:, 1, 1] = kv.k_scale, kv.v_scale
+        scales = sc[:, 1, 0], sc[:, 1, 1]
+    part = cache.KvCache(wide[:, 1, 0], wide[:, 1, 1], *scales)
+    cols = torch.full((3, table.shape[1] + 5), 2**31 - 1, dtype=torch.int32, device=cuda)
+    cols[:, 2:2 + table.shape[1]] = table
+    out = cache.attention(q, part, 4, cols[:, 2:2 + table.shape[1]], offs, starts)
+    assert torch.equal(out, ref)
+
+
 def test_many_requests(ncm, cuda):
     """More requests than a workgroup has threads, most of them short."""
     rng = np.random.default_rng(3)

@@ -78,6 +78,14 @@ def test_step_tensors():
     _raises(NCM_E_SHAPE, att, z(3, 192), kv, 3, t, o, s)             # 3 heads over 2
 
 
+def test_context_of_another_device():
+    from types import SimpleNamespace
+
+    from ncmorph_amd.context import stream_context
+
+    _raises(NCM_E_ARG, stream_context, torch.device("cuda", 0), SimpleNamespace(device=1))
+
+
 def test_rope_and_logits_checks():
     x, p, f = z(5, 128), z(5, dtype=i32), z(32, dtype=f32)
     r = kernels.rope_positions
