@@ -433,10 +433,12 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
             const bf16x8_t v = __builtin_bit_cast(bf16x8_t, u32x4_t{w[n][0], w[n][1], w[n][2], w[n][3]});
 #pragma unroll
             for (int rr = 0; rr < R; ++rr)
-                st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rr], st.o[rr][4 * f + n], 0, 0, 0);
+                st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    v, p[rr], st.o[rr][4 * f + n], 0, 0, 0);
 #pragma unroll
             for (int rr = 0; rr < R; ++rr)
-                st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest[rr], st.o[rr][4 * f + n], 0, 0, 0);
+                st.o[rr][4 * f + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    v, rest[rr], st.o[rr][4 * f + n], 0, 0, 0);
         }
     }
     next_v();
