@@ -684,7 +684,8 @@ int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
  *   x = x + (the sum, in list order, of bias_values[r][e] with bias_ids[r][e] == t)
  *   bit t % 32 of allowed[row][t / 32] clear: x = -infinity
  * and one rounding. Ids outside [0, vocab) are ignored; lengths are clamped
- * to [0, history_width]. */
+ * to [0, history_width]. history_width, with draft_tokens plus rows, is below
+ * 2^30 (a count has 30 bits). */
 typedef struct ncm_logit_rules {
     const int32_t* offsets;       /* [requests + 1] */
     const int32_t* history;       /* [requests][history_width] */

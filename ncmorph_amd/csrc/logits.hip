@@ -262,6 +262,9 @@ extern "C" int ncm_adjust_logits_dev(ncm_ctx_t* ctx, const ncm_logit_rules_t* ru
         u.history_width > kMaxRows || u.bias_count < 0 || u.bias_count > kMaxRows ||
         u.mask_words < 0 || u.mask_words > kMaxRows)
         return NCM_E_SHAPE;
+    // A token that stands in every entry still leaves the word's marks alone.
+    if ((u.history ? u.history_width : 0) + (u.draft_tokens ? rows : 0) > (int64_t)kCount)
+        return NCM_E_SHAPE;
     if (dtype != NCM_OUT_F32 && dtype != NCM_OUT_BF16) return NCM_E_ARG;
     if (u.offsets ? u.requests > kMaxRequests : u.requests != rows) return NCM_E_SHAPE;
     if ((u.draft_tokens && !u.offsets) || !u.bias_ids != !u.bias_values) return NCM_E_NULL;
