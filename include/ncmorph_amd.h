@@ -660,10 +660,10 @@ int ncm_kv_read_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_ba
  * q_stride], query head h at column h * head_dim reading K/V head h /
  * (q_heads / kv_heads); out: bf16 bits [rows, out_stride]. Strides multiples
  * of 8, 16-byte aligned. tree_mask: uint64 [rows, mask_words]; new tokens past
- * 64 * mask_words are not seen. workspace: at least the bytes that
- * ncm_kv_attention_workspace gives for the same cache, batch and q_heads,
- * 16-byte aligned; the call leaves nothing there that a later one needs, and
- * no two calls that may run at once can share it. Device pointers. */
+ * 64 * mask_words are not seen (with mask_words 0, none). workspace: at least
+ * the bytes that ncm_kv_attention_workspace gives for the same cache, batch and
+ * q_heads, 16-byte aligned; the call leaves nothing there that a later one
+ * needs, and no two calls that may run at once can share it. Device pointers. */
 int ncm_kv_attention_workspace(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                                int q_heads, size_t* bytes);
 int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
@@ -677,7 +677,8 @@ int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
  * is request r's. For token t of a row, count is how often t stands in
  * history[r][prompt_lens[r] .. history_lens[r]) and on the row's drafted path
  * (draft_tokens of the request's rows j whose bit is set in the row's
- * tree_mask; tree_mask NULL: rows up to and including its own), and t is seen
+ * tree_mask, none where mask_words is 0; tree_mask NULL: rows up to and
+ * including its own), and t is seen
  * when count > 0 or it stands in history[r][0 .. prompt_lens[r]). In fp32:
  *   seen:  x = x > 0 ? x / repetition[r] : x * repetition[r]
  *   x = x - frequency[r] * count, then x = x - presence[r] where count > 0

@@ -198,6 +198,8 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
     if tree_mask is not None:
         _, words = _ck.dims(tree_mask, "tree_mask", W, 2)
     pm = a.dev(tree_mask, "tree_mask", _ck.U64, (rows, words), optional=True)
+    if tree_mask is not None and words == 0:
+        pm = b.offsets  # a mask of no words has no address of its own; nothing is read there
     pp = a.dev(positions, "positions", _ck.I32, (rows,), optional=True)
     need = C.c_size_t()
     check(lib().ncm_kv_attention_workspace(C.byref(kv.struct), C.byref(b), q_heads,

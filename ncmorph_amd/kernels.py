@@ -662,6 +662,8 @@ def adjust_logits(logits, history=None, prompt_lens=None, history_lens=None, rep
         opt(draft_tokens, "draft_tokens", i32, (rows,), True),
         opt(tree_mask, "tree_mask", _ck.U64, (rows, words), True),
         requests, width, nb, words)
+    if tree_mask is not None and words == 0:
+        rules.tree_mask = rules.offsets  # a mask of no words has no address; nothing is read there
     if out is None:
         out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
         po, os_ = out.data_ptr(), vocab
