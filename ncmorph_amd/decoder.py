@@ -203,8 +203,11 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: dict | None = None):
       "yarn"     pairs that turn less than beta_slow (1) times in
                  original_max_position_embeddings divided by factor, those that
                  turn more than beta_fast (32) times kept, a linear ramp over
-                 the pairs between; sines and cosines times attention_factor
-                 (0.1 ln factor + 1)."""
+                 the pairs between (its ends rounded outwards to whole pairs,
+                 unless truncate is false); sines and cosines times
+                 attention_factor: with mscale and mscale_all_dim (together)
+                 the first's 0.1 m ln factor + 1 over the second's, else
+                 0.1 ln factor + 1; 1 where factor is at most 1."""
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError("rot_dim must be even and positive")
     if not theta > 1.0:
@@ -237,12 +240,19 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: dict | None = None):
     def pair(turns):  # the pair that turns so many times in the trained length
         return rot_dim * math.log(length / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
 
-    first = max(math.floor(pair(float(scaling.get("beta_fast", 32.0)))), 0)
-    last = min(math.ceil(pair(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+    first = pair(float(scaling.get("beta_fast", 32.0)))
+    last = pair(float(scaling.get("beta_slow", 1.0)))
+    if scaling.get("truncate") is not False:
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rot_dim - 1)
     ramp = np.clip((p - first) / max(last - first, 0.001), 0.0, 1.0)
     scale = scaling.get("attention_factor")
     if scale is None:
-        scale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        m, all_dim = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        if (m is None) != (all_dim is None):
+            raise ValueError("mscale and mscale_all_dim come together")
+        log = 0.1 * math.log(factor) if factor > 1.0 else 0.0
+        scale = log + 1.0 if m is None else (m * log + 1.0) / (all_dim * log + 1.0)
     return (inv * (1.0 - ramp) + inv / factor * ramp).astype(np.float32), float(scale)
 
 
