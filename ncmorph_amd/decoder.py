@@ -231,17 +231,25 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: dict | None = None):
         base = theta * factor ** (rot_dim / (rot_dim - 2.0))
         return (base ** (-2.0 * p / rot_dim)).astype(np.float32), 1.0
     length = float(scaling["original_max_position_embeddings"])
+    if not length > 0.0:
+        raise ValueError("original_max_position_embeddings must be positive")
     if kind == "llama3":
         low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not high > low:
+            raise ValueError("high_freq_factor must be above low_freq_factor")
         turns = length * inv / (2.0 * math.pi)
         keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
         return (inv * (keep + (1.0 - keep) / factor)).astype(np.float32), 1.0
 
+    fast = float(scaling.get("beta_fast", 32.0))
+    slow = float(scaling.get("beta_slow", 1.0))
+    if not fast >= slow > 0.0:
+        raise ValueError("beta_fast and beta_slow must be positive, the former not below the latter")
+
     def pair(turns):  # the pair that turns so many times in the trained length
         return rot_dim * math.log(length / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
 
-    first = pair(float(scaling.get("beta_fast", 32.0)))
-    last = pair(float(scaling.get("beta_slow", 1.0)))
+    first, last = pair(fast), pair(slow)
     if scaling.get("truncate") is not False:
         first, last = math.floor(first), math.ceil(last)
     first, last = max(first, 0), min(last, rot_dim - 1)

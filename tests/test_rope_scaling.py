@@ -39,3 +39,19 @@ def test_yarn_without_whole_pairs():
     assert not np.array_equal(whole, inv)
     same, _ = decoder.rope_frequencies(128, 10000.0, dict(YARN, truncate=True))
     assert np.array_equal(same, whole)
+
+
+L3 = dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+          original_max_position_embeddings=8192)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(L3, high_freq_factor=1.0), dict(L3, high_freq_factor=0.5), dict(L3, low_freq_factor=4.0),
+    dict(L3, high_freq_factor=math.nan), dict(L3, original_max_position_embeddings=0),
+    dict(L3, original_max_position_embeddings=-8192), dict(YARN, original_max_position_embeddings=0),
+    dict(YARN, original_max_position_embeddings=math.nan), dict(YARN, beta_slow=0.0),
+    dict(YARN, beta_fast=0.0), dict(YARN, beta_fast=1.0, beta_slow=32.0),
+    dict(YARN, beta_fast=math.nan)])
+def test_scalings_of_no_meaning_are_refused(bad):
+    with pytest.raises(ValueError):
+        decoder.rope_frequencies(64, 10000.0, bad)
