@@ -39,3 +39,26 @@ def test_a_tree_mask_of_no_words_counts_no_drafts(ncm, cuda):
               frequency=torch.ones(2, device=cuda), presence=torch.ones(2, device=cuda))
     y = kernels.adjust_logits(x, tree_mask=torch.zeros(5, 0, dtype=torch.int64, device=cuda), **kw)
     assert torch.equal(y, x)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8, I8])
+@pytest.mark.parametrize("form", ["chain", "tree", "positions"])
+def test_windows_behind_a_short_table(ncm, cuda, dtype, form):
+    """The table ends before the requests' own rows: their windows still end at
+    their positions, not at the table's end."""
+    step = f64.Step(9, [2, 3, 1], [100, 70, 300], 1, 64, 16, dtype)
+    kv, table, offs, starts = step.to(cuda)
+    q = torch.randn(6, 128, generator=torch.Generator().manual_seed(2)).to(BF16).to(cuda)
+    allowed = f64.chain(step.new) if form == "chain" else f64.tree(2, step.new)
+    mask = None if form == "chain" else f64.bits(allowed, 6, 1).to(cuda)
+    pos = None
+    if form == "positions":
+        pos = torch.tensor([100, 103, 70, -1, 75, 280], dtype=I32)
+    missing = [(r, p) for r in range(3) for p in range(4, 30)]
+    for window in (1, 50, 90, 260):
+        out = cache.attention(q, kv, 2, table[:, :4].contiguous(), offs, starts, tree_mask=mask,
+                              window=window, positions=None if pos is None else pos.to(cuda))
+        ref, mag = f64.attention(step, q.cpu(), 2, allowed, window=window, positions=pos,
+                                 missing=missing, chained=form == "chain")
+        err = (out.cpu().double().view(6, 2, 64) - ref).abs()
+        assert bool((err <= f64.attention_bound(ref, mag)).all()), window
