@@ -3,7 +3,8 @@
 // One pass with a running maximum and sum of the softmax:
 //   s_j = scale q.k_j (times the scale of k_j), m' >= max(m, max s_j) - 8,
 //   l' = l 2^(m - m') + sum 2^(s_j - m'), o' = o 2^(m - m') + sum 2^(s_j - m') v_j
-// with log2(e) folded into the scale. The query heads of a K/V head and the
+// with log2(e) folded into the scale (which for bf16 caches multiplies the
+// differences s_j - m in place of the products). The query heads of a K/V head and the
 // rows of a request stand together: R times 16 (row, head) pairs are the
 // columns of v_mfma_f32_16x16x32_bf16 products, tokens the rows of S^T = K Q^T
 // and the summed index of O^T = V^T P^T.
@@ -332,8 +333,9 @@ __device__ __forceinline__ void clean_values(const AttnArgs& a, int h, int key, 
 template <bool FULL, int HD, int CODES, int R, typename NextK, typename NextV>
 __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int h,
                                            Tile<HD, CODES>& t, State<HD, R>& st, int key, int page0,
-                                           int page1, uint32_t there, float to_log2, int lane,
-                                           const Lds<HD, R>& lds, NextK next_k, NextV next_v) {
+                                           int page1, uint32_t there, float to_log2, float lag,
+                                           int lane, const Lds<HD, R>& lds, NextK next_k,
+                                           NextV next_v) {
     const int g = lane >> 4;
     float s[R][8];
     // The queries are read from LDS each round: hoisted out of the loop they
@@ -379,15 +381,17 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
 #pragma unroll
         for (int i = 1; i < 8; ++i) top = fmaxf(top, s[rr][i]);
         top = max_over_groups(top);
-        // bf16 caches: s is the plain product, the scale is in the exponent's fma.
-        if constexpr (CODES == NCM_KV_BF16) top = top * to_log2;
         // m follows the maximum once that has grown by 2^8: sums in fp32 and
         // the rounding of p, a relative one, are as good to 2^8 as to 1, and o
         // is seldom touched after the first tiles. The comparison fails for a
-        // pair that has seen nothing yet.
-        if (__any(top > st.m[rr] + 8.0f)) {
+        // pair that has seen nothing yet. bf16 caches: s and m are plain
+        // products, their difference takes the scale: scaled first, two large
+        // scores would differ by their products' roundings, and 2^31 is enough
+        // for that to leave the exponent's range.
+        if (__any(top > st.m[rr] + (CODES == NCM_KV_BF16 ? lag : 8.0f))) {
             top = fmaxf(top, st.m[rr]);
-            const float f = __builtin_amdgcn_exp2f(st.m[rr] - top);
+            const float d = st.m[rr] - top;
+            const float f = __builtin_amdgcn_exp2f(CODES == NCM_KV_BF16 ? d * to_log2 : d);
             st.m[rr] = top;
             st.l[rr] *= f;
 #pragma unroll
@@ -396,8 +400,8 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            s[rr][i] = __builtin_amdgcn_exp2f(CODES == NCM_KV_BF16 ? fmaf(s[rr][i], to_log2, -st.m[rr])
-                                                                   : s[rr][i] - st.m[rr]);
+            const float d = s[rr][i] - st.m[rr];
+            s[rr][i] = __builtin_amdgcn_exp2f(CODES == NCM_KV_BF16 ? d * to_log2 : d);
             // A scale of 0 times -inf, and 0 times a V scale that is NaN.
             if constexpr (!FULL) s[rr][i] = (see[rr] >> i) & 1u ? s[rr][i] : 0.0f;
             sum += s[rr][i];
@@ -460,6 +464,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     // products is that of the scores.
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
     const float to_log2 = fabsf(a.scale) * 1.4426950408889634f;
+    const float lag = 8.0f / to_log2;  // 2^8 in plain products
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
         const int pair = block * 16 * R + min(16 * rr + c, pairs - 1);
@@ -518,8 +523,8 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
         if (s2 != s && (s2 & 31) == 0) look_up(s2);
         p0 = page(s2, 0), p1 = page(s2, 1);
         add_tokens<decltype(full)::value, HD, CODES, R>(
-            a, d, h, t, st, key, max(q0, 0), max(q1, 0), there, to_log2, lane,
-            lds, [&] { t.load_k(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); },
+            a, d, h, t, st, key, max(q0, 0), max(q1, 0), there, to_log2, lag, lane, lds,
+            [&] { t.load_k(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); },
             [&] { t.load_v(a.cache, h, key2, max(p0, 0), max(p1, 0), lane); });
         ++s;
     };
@@ -534,6 +539,9 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
         st.l[rr] = sum_over_groups(st.l[rr]);
+        // Maxima of plain products to exponents of 2, but for a pair that saw nothing.
+        if (CODES == NCM_KV_BF16 && st.m[rr] > kNoMax)
+            st.m[rr] = fmaxf(st.m[rr] * to_log2, kNoMax);
         if (g == 0) lds.m[wave][16 * rr + c] = st.m[rr];
     }
     __syncthreads();

@@ -62,3 +62,55 @@ def test_windows_behind_a_short_table(ncm, cuda, dtype, form):
                                  missing=missing, chained=form == "chain")
         err = (out.cpu().double().view(6, 2, 64) - ref).abs()
         assert bool((err <= f64.attention_bound(ref, mag)).all()), window
+
+
+def equal_keys(seed, new, before, hd, dtype, key):
+    """A step whose K hold `key` in every place; an equal score for all tokens."""
+    step = f64.Step(seed, new, before, 1, hd, 16, dtype)
+    for x in step.tokens[0]:
+        x.fill_(key)
+    codes, sc = f64.quantise(torch.full((1, hd), key).to(BF16), dtype)
+    if dtype == BF16:
+        step.pages[0][:] = codes[0]
+    else:
+        step.pages[0].view(torch.uint8)[:] = codes[0].view(torch.uint8)
+        step.scales[0].fill_(float(sc[0]))
+    return step
+
+
+def means(out, step, hd):
+    """Equal scores: every row is the mean of the V that it sees."""
+    out = out.cpu().double().view(-1, 2, hd)
+    V, i = step.cached(1), 0
+    for r, (n, c) in enumerate(zip(step.new, step.before)):
+        for j in range(n):
+            v = V[r][:c + j + 1, 0]
+            ref, mag = v.mean(0), v.abs().mean(0)
+            assert bool(((out[i] - ref).abs() <= f64.attention_bound(ref, mag)).all()), (r, j)
+            i += 1
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8, I8])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("key", [2.0 ** 5, -2.0 ** 15, 2.0 ** 30, -2.0 ** 50, 2.0 ** 60])
+def test_scores_of_any_size(ncm, cuda, dtype, hd, key):
+    """Scores of 2^28 to 2^84, of both signs, the same bits for every token; of
+    mantissas whose products with the scale are rounded."""
+    step = equal_keys(5, [2, 1, 30], [0, 300, 2000], hd, dtype, 1.2890625 * key)
+    kv, table, offs, starts = step.to(cuda)
+    q = torch.full((33, 2 * hd), 1.5703125 * 2.0 ** 20, dtype=BF16, device=cuda)
+    means(cache.attention(q, kv, 2, table, offs, starts), step, hd)
+
+
+@pytest.mark.parametrize("far", [-2.0 ** 40, -2.0 ** 70, -2.0 ** 100])
+def test_far_scores_beside_moderate_ones(ncm, cuda, far):
+    """Tokens far below the others count for nothing, whole tiles of them too."""
+    step = f64.Step(6, [1], [900], 1, 64, 16, BF16)
+    step.tokens[0][0][50:] = 1.2890625 * far
+    for t in range(50, 901):
+        step.pages[0][int(step.table[0, t // 16]), 0, t % 16] = 1.2890625 * far
+    kv, table, offs, starts = step.to(cuda)
+    q = torch.full((1, 64), 1.5703125, dtype=BF16, device=cuda)
+    out = cache.attention(q, kv, 1, table, offs, starts).cpu().double().view(1, 1, 64)
+    ref, mag = f64.attention(step, q.cpu(), 1, f64.chain([1]))
+    assert bool(((out - ref).abs() <= f64.attention_bound(ref, mag)).all())
