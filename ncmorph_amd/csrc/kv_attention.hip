@@ -4,10 +4,10 @@
 //   s_j = scale q.k_j (times the scale of k_j), m' >= max(m, max s_j) - 8,
 //   l' = l 2^(m - m') + sum 2^(s_j - m'), o' = o 2^(m - m') + sum 2^(s_j - m') v_j
 // with log2(e) folded into the scale (which for bf16 caches multiplies the
-// differences s_j - m in place of the products). The query heads of a K/V head and the
-// rows of a request stand together: R times 16 (row, head) pairs are the
-// columns of v_mfma_f32_16x16x32_bf16 products, tokens the rows of S^T = K Q^T
-// and the summed index of O^T = V^T P^T.
+// differences s_j - m in place of the products). The query heads of a K/V head
+// and the rows of a request stand together: R times 16 (row, head) pairs are
+// the columns of v_mfma_f32_16x16x32_bf16 products, tokens the rows of S^T =
+// K Q^T and the summed index of O^T = V^T P^T.
 //
 // Bound by the cache's bytes for one token a request, so K and V go from
 // memory to registers, each read once, without LDS between: the lane layout of
@@ -40,7 +40,8 @@ namespace {
 
 constexpr int kTile = 128;     // tokens of a tile, 32 per wavefront
 constexpr int kCus = 256;
-constexpr float kNoMax = -1e30f;  // a finite start: 2^(-inf - m) stays 0
+// No score is below this start but -inf, and 2^(-inf - m) stays 0 as it is finite.
+constexpr float kNoMax = -3.40282347e38f;
 
 struct AttnArgs {
     KvView cache;

@@ -114,3 +114,15 @@ def test_far_scores_beside_moderate_ones(ncm, cuda, far):
     out = cache.attention(q, kv, 1, table, offs, starts).cpu().double().view(1, 1, 64)
     ref, mag = f64.attention(step, q.cpu(), 1, f64.chain([1]))
     assert bool(((out - ref).abs() <= f64.attention_bound(ref, mag)).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8, I8])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("key", [-2.0 ** 42, -2.0 ** 50, -2.0 ** 57])
+def test_scores_far_below_zero(ncm, cuda, dtype, hd, key):
+    """All of a row's scores below -1e30, down to where 128 products of about
+    2^118 still have a sum in fp32's range."""
+    step = equal_keys(7, [2, 1, 30], [0, 300, 2000], hd, dtype, key)
+    kv, table, offs, starts = step.to(cuda)
+    q = torch.full((33, 2 * hd), 1.5703125 * 2.0 ** 60, dtype=BF16, device=cuda)
+    means(cache.attention(q, kv, 2, table, offs, starts), step, hd)
