@@ -636,8 +636,8 @@ typedef struct ncm_kv_batch {
 
 /* Writes the K and V rows of a step into the cache, quantised. k, v: bf16
  * bits [rows, stride], kv_heads heads from column 0; strides multiples of 8,
- * 16-byte aligned. What a place holds that two rows name is not defined.
- * Device pointers. */
+ * 16-byte aligned; fewer than 2^26 - 3 rows. What a place holds that two rows
+ * name is not defined. Device pointers. */
 int ncm_kv_write_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                      const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride);
 
@@ -659,7 +659,9 @@ int ncm_kv_read_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_ba
  * does not reach it, not even an infinity or a NaN. q: bf16 bits [rows,
  * q_stride], query head h at column h * head_dim reading K/V head h /
  * (q_heads / kv_heads); out: bf16 bits [rows, out_stride]. Strides multiples
- * of 8, 16-byte aligned. tree_mask: uint64 [rows, mask_words]; new tokens past
+ * of 8, 16-byte aligned. rows * q_heads is below 2^31, and units (of 32 rows
+ * and heads, one K/V head and one request; of 16 where requests have no more on
+ * average) below 2^24. tree_mask: uint64 [rows, mask_words]; new tokens past
  * 64 * mask_words are not seen (with mask_words 0, none). workspace: at least
  * the bytes that ncm_kv_attention_workspace gives for the same cache, batch and
  * q_heads, 16-byte aligned; the call leaves nothing there that a later one
@@ -708,7 +710,8 @@ typedef struct ncm_logit_rules {
 
 /* out = the rules applied to logits: float (dtype NCM_OUT_F32) or bf16 bits
  * (NCM_OUT_BF16) [rows, stride]; out may be logits, and must not overlap them
- * otherwise. Rows of no request are left as they were. */
+ * otherwise. Rows of no request are left as they were. Rows times slices of
+ * 8192 tokens, rounded up: below 2^23. */
 int ncm_adjust_logits_dev(ncm_ctx_t* ctx, const ncm_logit_rules_t* rules, const void* logits,
                           void* out, int64_t rows, int64_t vocab, int64_t in_stride,
                           int64_t out_stride, int dtype);

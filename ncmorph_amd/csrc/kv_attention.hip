@@ -819,6 +819,8 @@ int check_attention(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch, in
     if (q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads ||
         batch->rows * q_heads > 0x7FFFFFFF)
         return NCM_E_SHAPE;
+    // The join's launch has a workgroup per unit.
+    if (layout_of(*cache, *batch, q_heads).units > kMaxBlocks) return NCM_E_SHAPE;
     a->q_heads = q_heads;
     a->group = q_heads / cache->kv_heads;
     return NCM_OK;
@@ -862,7 +864,7 @@ extern "C" int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
     // in 64 bits, times the workgroups.
     const double most = ((double)batch->rows * q_heads / 16 + cache->kv_heads) * batch->requests *
                         ((double)a.batch.capacity / kTile + 1);
-    if (most > 0x1p50 || s.units > 0x7FFFFFFF) return NCM_E_SHAPE;
+    if (most > 0x1p50) return NCM_E_SHAPE;
     if (!workspace) return NCM_E_NULL;
     if (workspace_bytes < s.bytes) return NCM_E_LENGTH;
     if ((uintptr_t)workspace % 16) return NCM_E_ARG;

@@ -229,6 +229,7 @@ int move_rows(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_batch_t*
     if (rc) return rc;
     rc = check_batch(batch, a.cache.page_log2, &a.batch);
     if (rc) return rc;
+    if (batch->rows > 4 * kMaxBlocks) return NCM_E_SHAPE;  // four rows a workgroup
     if (batch->rows == 0 || batch->requests == 0) return NCM_OK;
     const int64_t width = (int64_t)cache->kv_heads * cache->head_dim;
     rc = check_rows(k, k_stride, width);

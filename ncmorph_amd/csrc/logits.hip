@@ -268,22 +268,21 @@ extern "C" int ncm_adjust_logits_dev(ncm_ctx_t* ctx, const ncm_logit_rules_t* ru
     if (dtype != NCM_OUT_F32 && dtype != NCM_OUT_BF16) return NCM_E_ARG;
     if (u.offsets ? u.requests > kMaxRequests : u.requests != rows) return NCM_E_SHAPE;
     if ((u.draft_tokens && !u.offsets) || !u.bias_ids != !u.bias_values) return NCM_E_NULL;
+    const bool bf16 = dtype == NCM_OUT_BF16;
+    const int size = bf16 ? 2 : 4, slice = slice_of(rows, vocab);
+    const int slices = (int)((vocab + 16 / size - 1 + slice - 1) / slice);
+    if (rows * slices > kMaxThreads / threads_of(bf16, slice)) return NCM_E_SHAPE;
     if (rows == 0 || vocab == 0 || u.requests == 0) return NCM_OK;
     if (!logits || !out) return NCM_E_NULL;
-    const bool bf16 = dtype == NCM_OUT_BF16;
-    const int size = bf16 ? 2 : 4;
     if ((uintptr_t)logits % size || (uintptr_t)out % size) return NCM_E_ARG;
     if (logits == out && in_stride != out_stride) return NCM_E_ARG;
     const bool wide = ((uintptr_t)logits - (uintptr_t)out) % 16 == 0 &&
                       (in_stride - out_stride) * size % 16 == 0;
     const bool counts = (u.history && u.history_width > 0) || u.draft_tokens ||
                         (u.bias_ids && u.bias_count > 0);
-    LogitArgs a = {u, logits, out, in_stride, out_stride, (int)rows, (int)vocab, 0,
+    LogitArgs a = {u, logits, out, in_stride, out_stride, (int)rows, (int)vocab, slices,
                    (int)((vocab + 31) / 32)};
-    const int slice = slice_of(rows, vocab);
-    a.slices = (int)((vocab + 16 / size - 1 + slice - 1) / slice);
-    if (rows * a.slices > 0x7FFFFFFF) return NCM_E_SHAPE;
-    const uint32_t blocks = (uint32_t)(rows * a.slices);
+    const uint32_t blocks = (uint32_t)(rows * slices);
     const DeviceScope scope(ncm_ctx_device(ctx));
     const int rc = step_hip(scope.error(), "adjust_logits device");
     if (rc) return rc;

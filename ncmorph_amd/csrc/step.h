@@ -90,6 +90,8 @@ __device__ __forceinline__ int page_of(const BatchView& b, const KvView& c, int6
 constexpr int64_t kMaxRequests = 65535;
 constexpr int64_t kMaxRows = int64_t(1) << 30;
 constexpr int64_t kMaxTokens = int64_t(1) << 30;  // of a sequence
+constexpr int64_t kMaxThreads = 0xFFFFFFFF;       // of a launch, along x
+constexpr int64_t kMaxBlocks = kMaxThreads / 256;
 
 inline int check_cache(const ncm_kv_cache_t* c, KvView* view) {
     if (!c) return NCM_E_NULL;
