@@ -710,8 +710,8 @@ typedef struct ncm_logit_rules {
 
 /* out = the rules applied to logits: float (dtype NCM_OUT_F32) or bf16 bits
  * (NCM_OUT_BF16) [rows, stride]; out may be logits, and must not overlap them
- * otherwise. Rows of no request are left as they were. Rows times slices of
- * 8192 tokens, rounded up: below 2^23. */
+ * otherwise. Rows of no request are left as they were. rows times
+ * (vocab + 7) / 8192 + 1 is below 2^23. */
 int ncm_adjust_logits_dev(ncm_ctx_t* ctx, const ncm_logit_rules_t* rules, const void* logits,
                           void* out, int64_t rows, int64_t vocab, int64_t in_stride,
                           int64_t out_stride, int dtype);

@@ -581,9 +581,11 @@ def rope_positions(x, positions, inv_freq, heads: int, head_dim: int, layout: st
     else:
         po, os_ = a.rows(out, "out", (_ck._dtype(x),), n_rows, width)
     a.done()
+    if n_rows < 2:  # one row has no stride
+        xs = os_ = width
     ctx = stream_context(x.device, ctx)
     check(lib().ncm_rope_positions_dev(ctx.handle, px, po, pp, pf, n_rows, heads, head_dim,
-                                       2 * half, max(xs, width), max(os_, width),
+                                       2 * half, xs, os_,
                                        _ROPE_LAYOUTS[layout], scale,
                                        NCM_OUT_BF16 if x.dtype == torch.bfloat16 else NCM_OUT_F32),
           W)
@@ -670,9 +672,10 @@ def adjust_logits(logits, history=None, prompt_lens=None, history_lens=None, rep
     else:
         po, os_ = a.rows(out, "out", (_ck._dtype(logits),), rows, vocab)
     a.done()
+    if rows < 2:  # one row has no stride
+        ls = os_ = vocab
     ctx = stream_context(logits.device, ctx)
-    check(lib().ncm_adjust_logits_dev(ctx.handle, C.byref(rules), pl, po, rows, vocab,
-                                      max(ls, vocab), max(os_, vocab),
+    check(lib().ncm_adjust_logits_dev(ctx.handle, C.byref(rules), pl, po, rows, vocab, ls, os_,
                                       NCM_OUT_BF16 if logits.dtype == torch.bfloat16
                                       else NCM_OUT_F32), W)
     return out

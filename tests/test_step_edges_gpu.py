@@ -126,3 +126,20 @@ def test_scores_far_below_zero(ncm, cuda, dtype, hd, key):
     kv, table, offs, starts = step.to(cuda)
     q = torch.full((33, 2 * hd), 1.5703125 * 2.0 ** 60, dtype=BF16, device=cuda)
     means(cache.attention(q, kv, 2, table, offs, starts), step, hd)
+
+
+def test_one_row_in_place_under_two_strides(ncm, cuda):
+    """A single row has no stride: two views of it may name different ones."""
+    buf = torch.randn(2, 200, generator=torch.Generator().manual_seed(2)).to(cuda)
+    x, y = buf[:1, :128], buf.view(-1)[:128].view(1, 128)
+    assert x.stride(0) != y.stride(0)
+    pos = torch.tensor([1234], dtype=I32, device=cuda)
+    inv = torch.rand(32, device=cuda)
+    ref = kernels.rope_positions(x, pos, inv, 2, 64)
+    assert kernels.rope_positions(x, pos, inv, 2, 64, out=y) is y
+    assert torch.equal(x, ref)
+    bias = dict(bias_ids=torch.tensor([[3, 90]], dtype=I32, device=cuda),
+                bias_values=torch.tensor([[1.0, -2.0]], device=cuda))
+    ref = kernels.adjust_logits(x, **bias)
+    assert kernels.adjust_logits(x, out=y, **bias) is y
+    assert torch.equal(x, ref)
