@@ -143,3 +143,52 @@ def test_one_row_in_place_under_two_strides(ncm, cuda):
     ref = kernels.adjust_logits(x, **bias)
     assert kernels.adjust_logits(x, out=y, **bias) is y
     assert torch.equal(x, ref)
+
+
+@pytest.mark.parametrize("new,before", [([1, 1], [3000, 20]), ([70, 3], [100, 900])])
+def test_attention_into_its_queries(ncm, cuda, new, before):
+    """A unit's queries are read by the units that write their places alone, the
+    parts of one that is cut before its join."""
+    step = f64.Step(7, new, before, 2, 64, 16, BF16)
+    kv, table, offs, starts = step.to(cuda)
+    buf = torch.randn(step.rows, 400, generator=torch.Generator().manual_seed(2)).to(BF16).to(cuda)
+    q = buf[:, 8:264]
+    ref = cache.attention(q, kv, 4, table, offs, starts)
+    was = buf.clone()
+    assert cache.attention(q, kv, 4, table, offs, starts, out=q) is q
+    assert torch.equal(q, ref)
+    assert torch.equal(buf[:, :8], was[:, :8]) and torch.equal(buf[:, 264:], was[:, 264:])
+
+
+def test_rows_before_the_first_request(ncm, cuda):
+    """offsets that begin past 0: the rows ahead are no request's."""
+    step = f64.Step(11, [3, 2], [40, 7], 2, 64, 16, BF16, extra_rows=4)
+    kv, table, offs, starts = step.to(cuda)
+    offs = offs + 3
+    q = torch.randn(9, 256, generator=torch.Generator().manual_seed(2)).to(BF16).to(cuda)
+    out = torch.full((9, 256), 5.0, dtype=BF16, device=cuda)
+    cache.attention(q, kv, 4, table, offs, starts, out=out)
+    ref, mag = f64.attention(step, q.cpu()[3:], 4, f64.chain(step.new))
+    err = (out.cpu().double()[3:8].view(5, 4, 64) - ref[:5]).abs()
+    assert bool((err <= f64.attention_bound(ref[:5], mag[:5])).all())
+    k, v = (torch.full((9, 128), 5.0, dtype=BF16, device=cuda) for _ in range(2))
+    cache.read(kv, table, offs, starts, 9, out=(k, v))
+    for w, t in enumerate((k, v)):
+        want = torch.cat([step.tokens[w][0][40:], step.tokens[w][1][7:]]).reshape(5, 128)
+        assert torch.equal(t.cpu()[3:8], want)
+    fresh = cache.allocate(kv.k.shape[0], 2, 16, 64, BF16, cuda)
+    cache.write(fresh, k, v, table, offs, starts)
+    x = torch.randn(9, 77, device=cuda)
+    y = torch.full((9, 77), 5.0, device=cuda)
+    one = torch.ones(2, device=cuda)
+    kernels.adjust_logits(x, offsets=offs, out=y, presence=one,
+                          history=torch.tensor([[3], [4]], dtype=I32, device=cuda))
+    z = x.clone()
+    z[3:6, 3] -= 1
+    z[6:8, 4] -= 1
+    assert torch.equal(y[3:8], z[3:8])
+    for t in (out, k, v, y):
+        assert bool((t[[0, 1, 2, 8]] == 5.0).all())
+    k2, _ = cache.read(fresh, table, offs, starts, 9)
+    assert torch.equal(k2[3:8], k[3:8])
+    assert int((fresh.k != 0).any(-1).sum()) == 10     # five tokens of two heads
