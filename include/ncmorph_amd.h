@@ -655,11 +655,13 @@ int ncm_kv_read_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache, const ncm_kv_ba
  *   counts as c);
  *   the request's new token c + j where bit j % 64 of tree_mask[row][j / 64]
  *   is set, or, where tree_mask is NULL, with j <= i and in the window too.
- * A row that sees nothing gets zeros, and a value that a row does not see
- * does not reach it, not even an infinity or a NaN. q: bf16 bits [rows,
- * q_stride], query head h at column h * head_dim reading K/V head h /
- * (q_heads / kv_heads); out: bf16 bits [rows, out_stride]. Strides multiples
- * of 8, 16-byte aligned. rows * q_heads is below 2^31, and units (of 32 rows
+ * A row that sees nothing, or nothing but scores of -infinity, gets zeros, and
+ * a value that a row does not see does not reach it, not even an infinity or a
+ * NaN. Sums run unnormalised: 2^8 times the sum of the |v| that a row sees has
+ * to stay in fp32's range. q: bf16 bits [rows, q_stride], query head h at column
+ * h * head_dim reading K/V head h / (q_heads / kv_heads); out: bf16 bits [rows,
+ * out_stride]; out may be q where the strides are equal, and must not overlap it
+ * otherwise. Strides multiples of 8, 16-byte aligned. rows * q_heads is below 2^31, and units (of 32 rows
  * and heads, one K/V head and one request; of 16 where requests have no more on
  * average) below 2^24. tree_mask: uint64 [rows, mask_words]; new tokens past
  * 64 * mask_words are not seen (with mask_words 0, none). workspace: at least
@@ -680,8 +682,8 @@ int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
  * history[r][prompt_lens[r] .. history_lens[r]) and on the row's drafted path
  * (draft_tokens of the request's rows j whose bit is set in the row's
  * tree_mask, none where mask_words is 0; tree_mask NULL: rows up to and
- * including its own), and t is seen
- * when count > 0 or it stands in history[r][0 .. prompt_lens[r]). In fp32:
+ * including its own), and t is seen when count > 0 or it stands in history[r]
+ * [0 .. prompt_lens[r]). In fp32:
  *   seen:  x = x > 0 ? x / repetition[r] : x * repetition[r]
  *   x = x - frequency[r] * count, then x = x - presence[r] where count > 0
  *   x = x + (the sum, in list order, of bias_values[r][e] with bias_ids[r][e] == t)

@@ -62,7 +62,8 @@ class KvCache:
     torch.bfloat16 (as given), torch.float8_e4m3fn or torch.int8 (codes, with
     float32 k_scale and v_scale [pages, kv_heads, page_size]). Pages may lie
     apart, as those of one layer of a buffer [pages, layers, ...] do.
-    page_size: a power of two, 16 to 1024; head_dim 64 or 128."""
+    page_size: a power of two, 16 to 1024; head_dim 64 or 128. It keeps the
+    tensors' addresses: where one gets another storage, make a new KvCache."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "struct", "named")
 
@@ -184,8 +185,9 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
     window > 0: of the tokens before (without a tree_mask, of all tokens) those
     less than window positions back from the row's position, positions[row]
     (int32) or starts + its index. Rows that see nothing get zeros.
-    scale: head_dim ** -0.5 by default. workspace: uint8 scratch, taken from
-    torch's allocator where not given."""
+    scale: head_dim ** -0.5 by default. out may be q; a new one's rows of no
+    request are not initialised. workspace: uint8 scratch, taken from torch's
+    allocator where not given."""
     import torch
 
     W = "cache.attention"

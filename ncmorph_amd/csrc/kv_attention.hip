@@ -26,13 +26,17 @@
 // that is cut go to the workspace, and kv_attention_join_kernel adds them in
 // order.
 //
-// 64 requests of 1024 to 8192 tokens, one row each, 32 heads over 8 of 128, fp8:
-// 105 us (4.7 TB/s; a copy runs at 5.1). Trees of 25 rows over 2000 to 4000
-// tokens, int8, 8 requests: 36 us; chunks of 256 rows over 8000, bf16, 2
-// requests: 143 us (290 TFLOP/s of unmasked products). Those two are bound by the
-// instructions around the products: per 32 tokens and 32 pairs some 300 vector
-// instructions (exponentials, maxima, regrouping, widening) beside 48 MFMAs, two
-// wavefronts a SIMD.
+// 64 requests of 1044 to 8192 tokens, one row each, 32 heads over 8 of 128, fp8:
+// 101 us (4.9 TB/s; a copy runs at 5.1), its join 4.7. 8 trees of 13 to 25 rows
+// over 523 to 4000 tokens, int8: 34 us, join 5.3. Chunks of 256 rows over 8000
+// tokens and of 186 over 2160, bf16: 129 us (318 TFLOP/s of unmasked products),
+// join 7.0. Those two are bound by latency, in runs of a few tiles for the trees:
+// per 32 tokens and 32 pairs a wavefront issues 305 (bf16) or 606 (int8) vector
+// instructions, all included, and 48 MFMAs, which keep the vector pipes busy for
+// 30% of the time and the matrix cores for 17 or 9%; wavefronts, 1.4 or 1.1 a
+// SIMD, wait for loads, LDS or barriers for 36 or 39% of theirs. (head_dim 128,
+// bf16, 32 pairs: all 256 registers and 10 spilled, none touched in the loop over
+// tiles that every pair sees whole.)
 #include "step.h"
 
 namespace ncm {
@@ -620,10 +624,10 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     __syncthreads();
 }
 
-// Two workgroups a CU. (Three, in 168 registers: 122 us against 105 for 64
+// Two workgroups a CU. (Three, in 168 registers: 122 us against 105 then for 64
 // requests of up to 8192 tokens, fp8: the runs are shorter, and a run begins
 // with a chain of loads. Both of a tile's loads a round ahead, in a second
-// tile's registers: 105, and 163 against 142 us for chunks of 256 rows.)
+// tile's registers: 105, and 163 against 142 then for chunks of 256 rows.)
 template <int HD, int CODES, int R>
 __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttnArgs a) {
     __shared__ Lds<HD, R> lds;
@@ -774,10 +778,11 @@ Layout layout_of(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int q_heads) 
     const int64_t some = std::max<int64_t>(1, std::min(b.requests, b.rows));
     // 16 R pairs a unit. R = 2 where requests have more than 16 on average: each
     // token's codes are loaded and widened once for twice the pairs. R = 1 and 2:
-    // 41 and 36 us for 8 trees of 25 rows and 4 heads over 4000 tokens, int8, 235
-    // and 143 for 256-row chunks over 8000, bf16; with one row a request, 105 and
-    // 116 for 64 of them, fp8, 8.0 and 10.1 for one over 777 tokens. (R = 4, one
-    // wavefront a SIMD: 53 for the trees, 148 for the chunks.)
+    // 38 and 34 us for 8 trees of up to 25 rows and 4 heads over up to 4000 tokens,
+    // int8, 212 and 129 for chunks of 256 and 186 rows over 8000 and 2160, bf16;
+    // with one row a request, 101 and 112 for 64 of them, fp8, 7.5 and 9.6 for one
+    // over 777 tokens. (R = 4, one wavefront a SIMD, when R = 2 took 36 and 143: 53
+    // for the trees, 148 for the chunks.)
     s.r16 = pairs <= 16 * some ? 1 : 2;
     s.some = some;
     s.units = (pairs / (16 * s.r16) + some) * c.kv_heads;

@@ -7,9 +7,9 @@
 // of a correctly rounded quotient of exact operands (a bf16 value times 127 has
 // 15 bits), so x = m / 2, a tie, rounds as it does in real numbers.
 //
-// Memory bound: a bf16 value in and its code out, or the other way. 14700 rows of
-// 8 heads of 128, e4m3: written in 24 us (3.8 TB/s of values, codes and scales),
-// read in 19 (4.8).
+// Memory bound: a bf16 value in and its code out, or the other way. 14720 rows of
+// 8 heads of 128, e4m3: written in 23 us (4.0 TB/s of values, codes and scales),
+// read in 19 (4.9).
 #include "step.h"
 
 namespace ncm {
@@ -200,10 +200,10 @@ void start(const ReadArgs& a, uint32_t blocks, hipStream_t st) {
 }
 
 // Rows a workgroup: four where that leaves four workgroups a CU, for one search
-// and its chain of loads for four times the bytes. One, four and eight: 90, 74
-// and 77 us for 49500 rows of 8 heads of 128, int8, read back (143 with a search
-// by every head), 27, 24 and 25 for 14700 rows, e4m3, written; one and four: 4.2
-// and 7.7 us for 48 rows written.
+// and its chain of loads for four times the bytes. One and four: 88 and 74 us for
+// 53607 rows of 8 heads of 128, int8, read back (143 with a search by every head,
+// 77 with eight rows), 25.5 and 23 for 14720 rows, e4m3, written (25 with eight);
+// 3.6 and 6.3 us for 48 rows written.
 template <int HD, int CODES, typename Args>
 void start_rows(const Args& a, hipStream_t st) {
     const int64_t rows = a.batch.rows;

@@ -8,7 +8,7 @@
 // that entries of one token are summed in list order.
 //
 // Memory bound: logits in and out and a bit a token; the history is read once
-// per slice, from the L2 after the first. 200 rows of 151936 float32 with
+// per slice, from the L2 after the first. 143 rows of 151936 float32 with
 // histories of 4000, masks and 300 biases: 47 us (3.7 TB/s).
 #include "step.h"
 
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(threads_of(BF16, SLICE)) void adjust_logits_kernel(
                 for (int i = 0; i < 4; ++i)
                     o[i] = BF16 ? bf16x2_bits_rne(x[(2 * i) % N], x[(2 * i + 1) % N])
                                 : __float_as_uint(x[i]);
-                // Large outputs past the caches: 51 us against 54 for 200 rows
+                // Large outputs past the caches: 51 us against 54 for 143 rows
                 // of 151936 float32.
                 if constexpr (SLICE == 8192) __builtin_nontemporal_store(o, (u32x4_t*)(out + t));
                 else *(u32x4_t*)(out + t) = o;
@@ -234,8 +234,8 @@ __global__ __launch_bounds__(threads_of(BF16, SLICE)) void adjust_logits_kernel(
 }
 
 // Slices of 8192 tokens where that leaves four workgroups a CU: the history is
-// read once a slice. 8192 and 2048: 51 and 71 us for 200 rows of 151936 float32,
-// 8.1 and 6.4 for 4 rows of 128256.
+// read once a slice. 8192 and 2048: 48 and 70 us for 143 rows of 151936 float32,
+// 7.4 and 6.1 for 4 rows of 128256.
 int slice_of(int64_t rows, int64_t vocab) {
     return rows * (vocab / 8192 + 1) >= 1024 ? 8192 : 2048;
 }

@@ -9,7 +9,7 @@
 //
 // Memory bound: rows * heads * head_dim values in and out. A thread turns 32
 // bytes of one head, sines and all: sharing them among eight heads of a row gave
-// nothing for 8192 rows of 40 heads of 128, bf16, interleaved (33.5 us, 5.0 TB/s; a
+// nothing for 8192 rows of 40 heads of 128, bf16, interleaved (33.3 us, 5.0 TB/s; a
 // copy runs at 5.1), and took 6.6 us against 3.5 for 4 rows.
 #include "step.h"
 

@@ -621,7 +621,9 @@ def adjust_logits(logits, history=None, prompt_lens=None, history_lens=None, rep
       seen:  x / repetition where x > 0, else x * repetition
       x - frequency * count, then x - presence where count > 0
       x + biases;  -infinity where not allowed
-    in float32, rounded once. out may be logits; new without one."""
+    in float32, rounded once. Ids outside the vocabulary are ignored; a
+    bias_ids that repeats ids takes time by the square of n. out may be logits;
+    a new one's rows of no request are not initialised."""
     import torch
 
     W = "adjust_logits"
