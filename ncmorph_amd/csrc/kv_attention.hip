@@ -468,8 +468,12 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     // A negative scale turns the queries' signs, so that the maximum of the
     // products is that of the scores.
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-    const float to_log2 = fabsf(a.scale) * 1.4426950408889634f;
-    const float lag = 8.0f / to_log2;  // 2^8 in plain products
+    // For a scale of 0 the least above it: the difference of m's start to a large
+    // product is an infinity, which 0 would turn into NaN.
+    const float to_log2 = a.scale == 0.0f ? 1.4e-45f : fabsf(a.scale) * 1.4426950408889634f;
+    // 2^8 in plain products; low enough for the first of them to move m, whatever
+    // the scale: no product less the start may leave fp32's range upwards.
+    const float lag = fminf(8.0f / to_log2, 1e30f);
 #pragma unroll
     for (int rr = 0; rr < R; ++rr) {
         const int pair = block * 16 * R + min(16 * rr + c, pairs - 1);

@@ -192,3 +192,14 @@ def test_rows_before_the_first_request(ncm, cuda):
     k2, _ = cache.read(fresh, table, offs, starts, 9)
     assert torch.equal(k2[3:8], k[3:8])
     assert int((fresh.k != 0).any(-1).sum()) == 10     # five tokens of two heads
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8, I8])
+@pytest.mark.parametrize("scale", [0.0, 1e-45, -1e-38])
+@pytest.mark.parametrize("key", [1.0, 2.0 ** 57, -2.0 ** 57])
+def test_scales_of_nothing(ncm, cuda, dtype, scale, key):
+    """Scores of 0 or next to it, also of products next to fp32's end."""
+    step = equal_keys(8, [2, 1, 30], [0, 300, 2000], 64, dtype, 1.2890625 * key)
+    kv, table, offs, starts = step.to(cuda)
+    q = torch.full((33, 128), 1.5703125 * max(abs(key) * 8, 1.0), dtype=BF16, device=cuda)
+    means(cache.attention(q, kv, 2, table, offs, starts, scale=scale), step, 64)
