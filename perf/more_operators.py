@@ -106,6 +106,7 @@ def draw(rng):
         # listed case.
         most = 256 * 16000 * 32 * 128 // 2 // (groups * members * tokens * hq * hd)
         values = 14_000_000 // (hkv * hd * groups)
+        page = min(page, 32) if groups * members > 60 else page   # tokens in no whole page
         return dict(kind=kind, groups=groups, members=members,
                     common=_log(rng, 16, max(17, min(most, values, 20000))),
                     context=_log(rng, 1, max(1, min(most, values // members, 2000))),
