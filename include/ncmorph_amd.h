@@ -676,6 +676,64 @@ int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
                          int64_t window, const int32_t* positions, const uint64_t* tree_mask,
                          int64_t mask_words, void* workspace, size_t workspace_bytes);
 
+/* The pages of a cache that belong to nobody, and who holds the others. Device
+ * memory; a new pool has free = any order of all pages, count = pages, refs 0
+ * and marks INT64_MAX. free is a stack: pages are taken from free[count - 1]
+ * downwards. A page goes back to it when its last holder releases it. */
+typedef struct ncm_page_pool {
+    int32_t* free;    /* [pages] */
+    int32_t* count;   /* [1] pages on the stack */
+    int32_t* refs;    /* [pages] table entries that hold a page */
+    int64_t* marks;   /* [pages] of a release's own use between calls INT64_MAX */
+    int64_t pages;    /* at most 2^30 */
+} ncm_page_pool_t;
+
+/* The page tables of sequences, [requests][table_stride] int32 as
+ * ncm_kv_batch_t has them, where a sequence of t tokens holds the first
+ * ceil(t / page_size) entries of its row, at most table_width; what the others
+ * say is not read. page_size: a power of two, 16 .. 1024. The arrays of lengths
+ * are device int32 [requests], read on the stream; negative lengths count as 0,
+ * those above 2^30 as 2^30. Calls on one pool are ordered by the caller (one
+ * stream, or events). An entry outside the pool holds nothing. */
+
+/* Request r holds, besides sources[r], the pages that the first tokens[r] tokens
+ * of that request's sequence fill (tokens[r] / page_size, rounded down: the
+ * next page of either is its own, and what the source has there is not copied).
+ * A source that is r or no request leaves r as it was; what row r's first
+ * entries held before is not released. A row must not be a source and get pages
+ * in one call. */
+int ncm_pages_share_dev(ncm_ctx_t* ctx, const ncm_page_pool_t* pool, int32_t* page_table,
+                        const int32_t* sources, const int32_t* tokens, int64_t requests,
+                        int64_t table_width, int64_t table_stride, int page_size);
+
+/* The step that adds added[r] tokens behind starts[r] of every request: offsets
+ * [requests + 1] (ncm_kv_batch_t's; tokens past `rows` are not added), per row
+ * its position, starts[r] + i for row i of request r, or with a tree_mask
+ * (uint64 [rows][mask_words], as ncm_kv_attention_dev's) starts[r] + the number
+ * of its ancestors (bits set among the request's rows, less its own; at least
+ * 0), and its slot, page * page_size + token % page_size of token starts[r] + i,
+ * or -1 where that token is not there. Rows of no request get position 0 and
+ * slot -1. The pages that the tokens begin are taken from the pool in the order
+ * of requests and tokens; missing[0] is how many the pool did not have (their
+ * entries become -1: those tokens are not there). pool NULL: no page is taken,
+ * the table has them already. workspace: int32 [requests + 2]. */
+int ncm_pages_extend_dev(ncm_ctx_t* ctx, const ncm_page_pool_t* pool, const int32_t* added,
+                         const int32_t* starts, int32_t* page_table, int64_t requests,
+                         int64_t table_width, int64_t table_stride, int page_size, int64_t rows,
+                         const uint64_t* tree_mask, int64_t mask_words, int32_t* offsets,
+                         int32_t* positions, int64_t* slots, int32_t* missing, int32_t* workspace);
+
+/* Sequences of lens[r] tokens become keep[r] long (no change where that is not
+ * less): the pages behind are released, their entries become -1. Pages without
+ * a holder go back to the stack in the order of requests and tokens, the first
+ * on top: a release of what an extension took leaves the pool as it was.
+ * Entries of a page beyond its holders release nothing. workspace: int32
+ * [requests + 2]. */
+int ncm_pages_release_dev(ncm_ctx_t* ctx, const ncm_page_pool_t* pool, int32_t* page_table,
+                          const int32_t* lens, const int32_t* keep, int64_t requests,
+                          int64_t table_width, int64_t table_stride, int page_size,
+                          int32_t* workspace);
+
 /* Rules on logits; every pointer may be NULL (its rule is off), device memory.
  * Request r's rows are offsets[r] .. offsets[r + 1] - 1; offsets NULL: row r
  * is request r's. For token t of a row, count is how often t stands in

@@ -75,6 +75,10 @@ SIGNATURES = [
     ("ncm_kv_attention_workspace", i32, [vp, vp, i32, C.POINTER(sz)]),
     ("ncm_kv_attention_dev", i32, [vp, vp, vp, vp, vp, i32, i64, i64, C.c_float, i64, vp, vp, i64,
                                    vp, sz]),
+    ("ncm_pages_share_dev", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i32]),
+    ("ncm_pages_extend_dev", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i32, i64, vp, i64, vp, vp,
+                                   vp, vp, vp]),
+    ("ncm_pages_release_dev", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]),
     ("ncm_adjust_logits_dev", i32, [vp, vp, vp, vp, i64, i64, i64, i64, i32]),
     ("ncm_rvq_prepare", i32, [vp, vp, i64, i64, i64, vp]),
     ("ncm_rvq_encode", i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp]),

@@ -2,7 +2,10 @@
 prefill. A step hands over the new rows of some requests (one token each, a
 drafted tree of tokens, a chunk of a prompt): `write` puts their K and V into
 the cache, `attention` lets their queries read it, `read` gives cached tokens
-back as dense rows.
+back as dense rows. Which pages hold what is kept on the device too, in a
+PagePool: `extend` takes the pages of a step's new tokens and makes its offsets,
+positions and slots, `share` lets sequences hold the pages of a common prefix,
+`release` gives pages back.
 
 Every call takes the step's requests as three int32 device tensors: offsets
 [requests + 1] (request r's rows are offsets[r] .. offsets[r + 1] - 1), starts
@@ -16,6 +19,7 @@ ncm_kv_cache_t and ncm_kv_batch_t say the rest. The reference has no cache
 """
 from __future__ import annotations
 
+import collections
 import ctypes as C
 
 from . import _check as _ck
@@ -38,6 +42,11 @@ class _Batch(C.Structure):
     _fields_ = [("offsets", C.c_void_p), ("starts", C.c_void_p), ("page_table", C.c_void_p),
                 ("requests", C.c_int64), ("rows", C.c_int64), ("table_width", C.c_int64),
                 ("table_stride", C.c_int64)]
+
+
+class _Pool(C.Structure):
+    _fields_ = [("free", C.c_void_p), ("count", C.c_void_p), ("refs", C.c_void_p),
+                ("marks", C.c_void_p), ("pages", C.c_int64)]
 
 
 def _page_stride(t, name, shape, size, where):
@@ -223,3 +232,123 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
                                      pm, words, pw,
                                      workspace.numel()), W)
     return out
+
+
+class PagePool:
+    """The pages of a cache (of all its layers) that belong to nobody, and who
+    holds the others: free int32 [pages], a stack whose first count[0] entries
+    (int32 [1]) are the free pages, taken from its top, and refs int32 [pages],
+    how many table entries hold each page. It keeps the tensors' addresses.
+    Calls on one pool belong on one stream, or are ordered by the caller."""
+
+    __slots__ = ("free", "count", "refs", "marks", "struct", "named")
+
+    def __init__(self, free, count, refs):
+        import torch
+
+        a = _ck.Args("PagePool")
+        (pages,) = _ck.dims(free, "free", a.where, 1)
+        if not 0 < pages <= 1 << 30:
+            raise NcmError(NCM_E_SHAPE, a.where, "a pool has 1 to 2^30 pages")
+        pf = a.dev(free, "free", _ck.I32, (pages,))
+        pc = a.dev(count, "count", _ck.I32, (1,))
+        pr = a.dev(refs, "refs", _ck.I32, (pages,))
+        self.free, self.count, self.refs = free, count, refs
+        self.marks = torch.full((pages,), (1 << 63) - 1, dtype=torch.int64, device=free.device)
+        self.struct = _Pool(pf, pc, pr, self.marks.data_ptr(), pages)
+        self.named = tuple(a.seen)
+
+
+def page_pool(pages: int, device) -> PagePool:
+    """A PagePool whose pages are all free, page 0 on top."""
+    import torch
+
+    return PagePool(torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device),
+                    torch.full((1,), pages, dtype=torch.int32, device=device),
+                    torch.zeros(pages, dtype=torch.int32, device=device))
+
+
+StepTables = collections.namedtuple("StepTables", "offsets positions slots missing")
+
+
+def _tables(a, pool, page_table, lengths, names, optional=False):
+    """Addresses of the per-request int32 tensors and (requests, width, row
+    stride) of the table; the pool's tensors join the call's."""
+    requests, width = _ck.dims(page_table, "page_table", a.where, 2)
+    got = [a.dev(t, n, _ck.I32, (requests,)) for t, n in zip(lengths, names)]
+    pt, stride = a.rows(page_table, "page_table", _ck.I32, requests, width)
+    if pool is not None or not optional:
+        if not isinstance(pool, PagePool):
+            raise NcmError(NCM_E_ARG, a.where, "pool must be a PagePool")
+        a.seen += pool.named
+    return got, pt, requests, width, max(stride, width) if requests > 1 else width
+
+
+def share(pool: PagePool, page_table, sources, tokens, page_size: int, ctx=None):
+    """Lets request r hold the whole pages of the first tokens[r] tokens of
+    request sources[r] (int32 [requests]; its own number or -1: nothing) besides
+    that one, in the first entries of its row of page_table, which must hold no
+    pages. tokens[r] // page_size pages; r's sequence goes on behind them. A row
+    cannot be a source and get pages in one call."""
+    a = _ck.Args("cache.share")
+    got, pt, n, width, stride = _tables(a, pool, page_table, (sources, tokens),
+                                        ("sources", "tokens"))
+    a.done()
+    ctx = stream_context(page_table.device, ctx)
+    check(lib().ncm_pages_share_dev(ctx.handle, C.byref(pool.struct), pt, *got, n, width, stride,
+                                    page_size), a.where)
+
+
+def extend(pool, page_table, new, starts, rows: int, page_size: int, tree_mask=None,
+           ctx=None) -> StepTables:
+    """A step that adds new[r] tokens behind starts[r] of every request (int32
+    [requests]), its tensors of `rows` rows: takes the pages that they begin
+    from the pool into page_table, in the order of requests and tokens, and
+    returns offsets (int32 [requests + 1]), positions (int32 [rows]: starts +
+    index, or the depth in the tree_mask that `attention` takes in place of the
+    index), slots (int64 [rows]: page * page_size + token % page_size; -1 where
+    the token is not there) and missing (int32 [1]: pages that the pool did not
+    have; their tokens are not there). Rows of no request get position 0 and
+    slot -1. pool None: page_table has every page already."""
+    import torch
+
+    W = "cache.extend"
+    a = _ck.Args(W)
+    got, pt, n, width, stride = _tables(a, pool, page_table, (new, starts), ("new", "starts"), True)
+    words = 0
+    if tree_mask is not None:
+        _, words = _ck.dims(tree_mask, "tree_mask", W, 2)
+    pm = a.dev(tree_mask, "tree_mask", _ck.U64, (rows, words), optional=True)
+    a.done()
+    dev = page_table.device
+    # One allocation for what is int32, slots apart.
+    ints = torch.empty(2 * n + 4 + rows, dtype=torch.int32, device=dev)
+    slots = torch.empty(rows, dtype=torch.int64, device=dev)
+    offsets, positions = ints[:n + 1], ints[n + 1:n + 1 + rows]
+    missing = ints[n + 1 + rows:n + 2 + rows]
+    p = ints.data_ptr()
+    if tree_mask is not None and words == 0:
+        pm = p  # a mask of no words has no address of its own; nothing is read there
+    ctx = stream_context(dev, ctx)
+    check(lib().ncm_pages_extend_dev(
+        ctx.handle, None if pool is None else C.byref(pool.struct), *got, pt, n, width, stride,
+        page_size, rows, pm, words, p, p + 4 * (n + 1), slots.data_ptr(), p + 4 * (n + 1 + rows),
+        p + 4 * (n + 2 + rows)), W)
+    return StepTables(offsets, positions, slots, missing)
+
+
+def release(pool: PagePool, page_table, lens, keep, page_size: int, ctx=None):
+    """Cuts sequences of lens[r] tokens to keep[r] (int32 [requests]; no change
+    where that is not less): page_table's entries behind become -1, and pages
+    that no table holds any more go back to the pool. Drafted tokens that were
+    rejected: keep the accepted; finished requests: keep 0. What an `extend` took
+    leaves the pool, released, as it was before."""
+    import torch
+
+    a = _ck.Args("cache.release")
+    got, pt, n, width, stride = _tables(a, pool, page_table, (lens, keep), ("lens", "keep"))
+    a.done()
+    space = torch.empty(n + 2, dtype=torch.int32, device=page_table.device)
+    ctx = stream_context(page_table.device, ctx)
+    check(lib().ncm_pages_release_dev(ctx.handle, C.byref(pool.struct), pt, *got, n, width, stride,
+                                      page_size, space.data_ptr()), a.where)
