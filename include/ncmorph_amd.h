@@ -776,6 +776,45 @@ int ncm_adjust_logits_dev(ncm_ctx_t* ctx, const ncm_logit_rules_t* rules, const 
                           void* out, int64_t rows, int64_t vocab, int64_t in_stride,
                           int64_t out_stride, int dtype);
 
+/* How tokens are drawn; every pointer but offsets is device memory [requests]
+ * and may be NULL (its rule is off). Request r's rows are offsets[r] ..
+ * offsets[r + 1] - 1; offsets NULL: row r is request r's. A row's tokens stand
+ * in the order (logit descending, id ascending), w = exp((x - max) / T), with
+ * NaN and -infinity not among them and infinity the largest finite value:
+ *   top_k[r] > 0: the first top_k[r] of them;
+ *   top_p[r] < 1: of those, the fewest whose sum is at least top_p[r] times
+ *   their sum (one at least);
+ *   min_p[r] > 0: of those, the ones with w >= min_p[r] (1 at most);
+ *   the token is the first whose cumulative weight is above u times the sum of
+ *   those kept.
+ * temperature 0, below it or NaN: the first token of all. (One above 0 but
+ * below 2^-96 counts as that.) NaN turns top_p and min_p off. */
+typedef struct ncm_sample_rules {
+    const int32_t* offsets;     /* [requests + 1] */
+    const float* temperature;   /* NULL: 1 */
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int64_t requests;
+} ncm_sample_rules_t;
+
+/* tokens[row] (int32): the token that uniform[row] (float or double, by
+ * uniform_bits 32 or 64, in [0, 1); others count as the nearest of these) draws
+ * from logits, float (dtype NCM_OUT_F32) or bf16 bits (NCM_OUT_BF16) [rows,
+ * stride], or -1 where none is there; probabilities[row] (float, or NULL): its
+ * share of the kept tokens' sum, 1 for a greedy row, 0 for -1. Weights are taken
+ * in 64 bits, rounded to multiples of 2^-43 of the largest and summed exactly:
+ * the same logits draw the same token wherever they stand. Rows of no request
+ * are left as they were. vocab at most 2^20, rows below 2^22. workspace: at
+ * least the bytes that ncm_sample_workspace gives, 16-byte aligned; the call
+ * leaves nothing there that a later one needs, and no two calls that may run at
+ * once can share it. Device pointers. */
+int ncm_sample_workspace(int64_t rows, int64_t vocab, size_t* bytes);
+int ncm_sample_dev(ncm_ctx_t* ctx, const ncm_sample_rules_t* rules, const void* logits,
+                   int64_t rows, int64_t vocab, int64_t stride, int dtype, const void* uniform,
+                   int uniform_bits, int32_t* tokens, float* probabilities, void* workspace,
+                   size_t workspace_bytes);
+
 /* ---- multiscale residual vector quantization ---- */
 
 /* csq[l * v + k] = squared norm of codebook row (l, k), in the fixed fp32

@@ -80,6 +80,8 @@ SIGNATURES = [
                                    vp, vp, vp]),
     ("ncm_pages_release_dev", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]),
     ("ncm_adjust_logits_dev", i32, [vp, vp, vp, vp, i64, i64, i64, i64, i32]),
+    ("ncm_sample_workspace", i32, [i64, i64, C.POINTER(sz)]),
+    ("ncm_sample_dev", i32, [vp, vp, vp, i64, i64, i64, i32, vp, i32, vp, vp, vp, sz]),
     ("ncm_rvq_prepare", i32, [vp, vp, i64, i64, i64, vp]),
     ("ncm_rvq_encode", i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp]),
     ("ncm_rvq_encode_counts", i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp, vp,

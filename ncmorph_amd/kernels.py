@@ -10,9 +10,9 @@ ABI; nothing here computes on the CPU.
 already in HBM, bf16 (or fp32) operands, fp32 (or bf16) output,
 stream-ordered on torch's current stream.
 
-`rope_positions` and `adjust_logits` belong to a step that continues sequences
-over ncmorph_amd.cache: they take torch tensors, use no workspace and can be
-captured into a graph.
+`rope_positions`, `adjust_logits` and `sample` belong to a step that continues
+sequences over ncmorph_amd.cache: they take torch tensors, use no workspace of
+the context and can be captured into a graph.
 """
 from __future__ import annotations
 
@@ -681,3 +681,70 @@ def adjust_logits(logits, history=None, prompt_lens=None, history_lens=None, rep
                                       NCM_OUT_BF16 if logits.dtype == torch.bfloat16
                                       else NCM_OUT_F32), W)
     return out
+
+
+class _SampleRules(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("offsets", "temperature", "top_k", "top_p", "min_p")]
+    _fields_ += [("requests", C.c_int64)]
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, offsets=None,
+           probabilities: bool = False, out=None, workspace=None, ctx=None):
+    """The tokens, int32 [rows], that uniform (float32 or float64 [rows], in [0,
+    1)) draws from logits (torch.float32 or bfloat16 [rows, vocab], rows may be
+    strided; adjust_logits' output). Row r is request r, or, with offsets (int32
+    [requests + 1], as in ncmorph_amd.cache), the rows of request r are
+    offsets[r] .. offsets[r + 1] - 1. Per request, every one optional:
+    temperature (float32; 0 or less: the largest logit, no draw), top_k (int32;
+    0 or less: off), top_p and min_p (float32; 1, and 0: off). In the order
+    (logit descending, id ascending), with weights w = exp((x - max) / T):
+      the first top_k tokens,
+      of those the fewest with a sum of at least top_p times theirs,
+      of those the ones with w >= min_p;
+      the first of them whose cumulative weight is above uniform * their sum.
+    Weights are summed exactly in 64 bits. NaN and -infinity are no tokens;
+    where there is none the result is -1. probabilities: returns (tokens,
+    float32 [rows] shares of the tokens drawn). out: int32 [rows]; a new one's
+    rows of no request are not initialised, nor are probabilities there.
+    workspace: uint8 scratch, taken from torch's allocator where not given."""
+    import torch
+
+    W = "sample"
+    a = _ck.Args(W)
+    rows, vocab = _ck.dims(logits, "logits", W, 2)
+    requests = rows
+    if offsets is not None:
+        requests = _ck.dims(offsets, "offsets", W, 1)[0] - 1
+        if requests < 0:
+            raise NcmError(-2, W, "offsets must have requests + 1 entries")
+    pl, stride = a.rows(logits, "logits", ("float32", "bfloat16"), rows, vocab)
+    pu = a.dev(uniform, "uniform", ("float32", "float64"), (rows,))
+    per = (requests,)
+    rules = _SampleRules(
+        a.dev(offsets, "offsets", _ck.I32, (requests + 1,), True),
+        a.dev(temperature, "temperature", _ck.F32, per, True),
+        a.dev(top_k, "top_k", _ck.I32, per, True), a.dev(top_p, "top_p", _ck.F32, per, True),
+        a.dev(min_p, "min_p", _ck.F32, per, True), requests)
+    need = C.c_size_t()
+    check(lib().ncm_sample_workspace(rows, vocab, C.byref(need)), W)
+    dv = logits.device
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=dv)
+        po = out.data_ptr()
+    else:
+        po = a.dev(out, "out", _ck.I32, (rows,))
+    chance = torch.empty(rows, dtype=torch.float32, device=dv) if probabilities else None
+    if workspace is None:
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=dv)
+        pw = workspace.data_ptr()
+    else:
+        pw = a.dev(workspace, "workspace", ("uint8",))
+    a.done()
+    ctx = stream_context(dv, ctx)
+    check(lib().ncm_sample_dev(ctx.handle, C.byref(rules), pl, rows, vocab,
+                               stride if rows > 1 else vocab,
+                               NCM_OUT_BF16 if logits.dtype == torch.bfloat16 else NCM_OUT_F32, pu,
+                               64 if uniform.dtype == torch.float64 else 32, po,
+                               chance.data_ptr() if probabilities else None, pw,
+                               workspace.numel()), W)
+    return (out, chance) if probabilities else out
