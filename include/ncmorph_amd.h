@@ -189,6 +189,53 @@ int ncm_linear_bf16_swiglu(ncm_ctx_t* ctx, const uint16_t* x, const uint16_t* w,
                            const uint16_t* bias, uint16_t* y, int64_t m, int64_t k,
                            int64_t n2);
 
+/* A weight matrix [n, k] in 4-bit codes, in the order in which ncm_linear_int4
+ * reads it (ncm_int4_pack_dev): weight = (code - zero) * scale, codes and zeros 0
+ * .. 15, one bf16 scale (and one zero, or 8 for all) per output and group of 32,
+ * 64 or 128 inputs. n up to 2^28, k a multiple of 8 up to 2^24 (the last group
+ * may be short), and ceil(n / 16) * ceil(k / 128) below 2^24. */
+typedef struct ncm_int4_weight {
+    const void* codes;   /* ncm_int4_bytes' bytes, 16-byte aligned */
+    const void* scales;  /* likewise */
+    int64_t n;
+    int64_t k;
+    int32_t group;
+    int32_t has_zeros;   /* packed with zeros */
+} ncm_int4_weight_t;
+
+/* Bytes of both packed arrays. */
+int ncm_int4_bytes(int64_t n, int64_t k, int group, int has_zeros, size_t* codes, size_t* scales);
+/* codes (a byte each, the low four bits) [n, k], scales (bf16 bits) and zeros
+ * (a byte each, or NULL) [n, ceil(k / group)] into the packed arrays. Device
+ * pointers. */
+int ncm_int4_pack_dev(ncm_ctx_t* ctx, const uint8_t* codes, const uint16_t* scales,
+                      const uint8_t* zeros, int64_t n, int64_t k, int group, void* packed_codes,
+                      void* packed_scales);
+/* Codes and scales of a bf16 matrix w [n, stride]: per group, zeros NULL: scale
+ * = bf16(max |w| / 7), code = rint(w / scale) + 8; else, with lo = min(w, 0) and
+ * hi = max(w, 0), scale = bf16(hi / 15 - lo / 15), zero = rint(-lo / scale),
+ * code = rint(w / scale) + zero; codes and zeros clamped to 0 .. 15, quotients in
+ * fp32. A group that holds a NaN or an infinity gets the scale NaN; one without
+ * a value other than 0 (or too small for a bf16 scale) the scale 0; both the
+ * codes (and zero) 8. Device pointers. */
+int ncm_int4_quantise_dev(ncm_ctx_t* ctx, const uint16_t* w, int64_t n, int64_t k, int64_t stride,
+                          int group, uint8_t* codes, uint16_t* scales, uint8_t* zeros);
+/* y[m, n] = sum_k x[m, k] * weight[n, k] (+ bias[n]) (+ residual[m, n]): the bf16
+ * activations times the exact 4-bit integers in fp32, the fp32 sums of a group
+ * times its scale, all sums in fp32 and one rounding to the output's type.
+ * Inside, codes stand as 128 + code and the sum of x takes the excess off: the
+ * rounding of an output is that of sums of (128 + code) |x| scale, those sums
+ * have to stay in fp32's range, and a row of x that holds an infinity or a NaN
+ * gives NaN. x: bf16 bits [m, x_stride], stride a multiple of 8, 16-byte aligned;
+ * bias: bf16 [n] or NULL; residual: float [m, n] or NULL, which y may be for the
+ * float modes; y: float [m, n] (out_mode F32, BF16_F32) or bf16 bits (BF16). m up
+ * to 2^20: made for the rows of a decode step; from some hundred rows on
+ * ncm_linear_bf16 of the widened weights takes less time. Uses no workspace.
+ * Device pointers. */
+int ncm_linear_int4(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride,
+                    const ncm_int4_weight_t* w, const uint16_t* bias, const float* residual,
+                    void* y, int64_t m, int out_mode);
+
 /* The q|k|v projection and the RoPE rotation of its q and k heads
  * (root.zig:497-530) in one pass, for head_dim 64: y = the bf16 output of
  * ncm_linear_bf16 (BF16), with every 64-wide head in columns [0, rot_cols)

@@ -1,0 +1,385 @@
+// Products with 4-bit weights (ncm_linear_int4) and what makes them.
+//
+//   y[m, n] = sum_g s[n, g] sum_{k in g} (q[n, k] - z[n, g]) x[m, k]
+//
+// A code becomes the bf16 value 128 + q by setting its four bits into 0x4300,
+// one operation for two codes, and enters v_mfma_f32_16x16x32_bf16 with the
+// bf16 rows of x, weights the rows and tokens the columns of the product. A
+// product with ones gives the sum of x over the same k, so that per group
+//   y += s (sum (128 + q) x - (128 + z) sum x)
+// in fp32: scales and zero points meet fp32 sums, and nothing is rounded to 16
+// bits but the output. The difference costs a factor of 143 / 8 of the rounding
+// of a plain fp32 sum at most.
+//
+// Bound by the weights' bytes for few rows. They are packed once in the order
+// of the lanes: 16 outputs and 128 inputs are 1 KB, a wavefront's 16-byte load.
+// A workgroup makes 16 NT outputs of 16 MT rows, its eight wavefronts taking
+// every eighth 128 inputs; their sums are added in order through LDS.
+#include "step.h"
+
+namespace ncm {
+namespace {
+
+constexpr int kWaves = 8;
+
+struct Int4Args {
+    const uint16_t* x;
+    const u32x4_t* codes;
+    const char* scales;
+    const uint16_t* bias;
+    const float* residual;
+    void* y;
+    int64_t x_stride;
+    int m, n, k, blocks;  // of 128 inputs
+    bool wide;            // 4 outputs of a row in one access
+};
+
+// Scales of 16 outputs, a block of 128 inputs: [128 / GROUP][16], two bytes, or
+// with zero points four: 128 + z in the low half, both bf16.
+template <int GROUP, bool ZEROS>
+constexpr int scale_bytes() { return 128 / GROUP * 16 * (ZEROS ? 4 : 2); }
+
+template <int GROUP, bool ZEROS, int NT, int MT>
+struct Stage {
+    static constexpr int G = 128 / GROUP;
+    u32x4_t w[NT];
+    u32x4_t x[MT][4];
+    uint32_t s[NT][G][ZEROS ? 4 : 2];
+};
+
+template <int GROUP, bool ZEROS, int NT, int MT, int OUT>
+__global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
+    typedef Stage<GROUP, ZEROS, NT, MT> S;
+    constexpr int G = S::G, STEPS = 4 / G;  // MFMA steps of a group
+    __shared__ f32x4_t parts[kWaves][NT * MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int64_t tile0 = (int64_t)blockIdx.x * NT;
+    const int tiles = (a.n + 15) / 16, m0 = blockIdx.y * 16 * MT;
+
+    auto load = [&](S& s, int b) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int64_t at = min(tile0 + t, (int64_t)tiles - 1) * a.blocks + b;
+            s.w[t] = a.codes[at * 64 + lane];
+            const char* p = a.scales + at * scale_bytes<GROUP, ZEROS>() + g * (ZEROS ? 16 : 8);
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < (ZEROS ? 4 : 2); ++j)
+                    s.s[t][i][j] = ((const uint32_t*)(p + i * (ZEROS ? 64 : 32)))[j];
+        }
+#pragma unroll
+        for (int r = 0; r < MT; ++r) {
+            const int row = m0 + 16 * r + c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = 128 * b + 32 * i + 8 * g;
+                s.x[r][i] = u32x4_t{0, 0, 0, 0};
+                if (row < a.m && k < a.k) s.x[r][i] = *(const u32x4_t*)(a.x + row * a.x_stride + k);
+            }
+        }
+    };
+
+    f32x4_t sum[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < MT; ++r) sum[t][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const u32x4_t one_bits = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, one_bits);
+    auto add = [&](const S& s) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            f32x4_t of_x[MT], of_q[NT][MT];
+#pragma unroll
+            for (int r = 0; r < MT; ++r) {
+                of_x[r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) of_q[t][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int e = STEPS * i; e < STEPS * (i + 1); ++e) {
+#pragma unroll
+                for (int r = 0; r < MT; ++r)
+                    of_x[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        ones, __builtin_bit_cast(bf16x8_t, s.x[r][e]), of_x[r], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    u32x4_t q;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) q[j] = ((s.w[t][e] >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+#pragma unroll
+                    for (int r = 0; r < MT; ++r)
+                        of_q[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8_t, q), __builtin_bit_cast(bf16x8_t, s.x[r][e]),
+                            of_q[t][r], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t word = s.s[t][i][ZEROS ? j : j / 2];
+                    const float scale = __uint_as_float(!ZEROS && j % 2 == 0 ? word << 16 : word & 0xFFFF0000u);
+                    const float zero = ZEROS ? __uint_as_float(word << 16) : 136.0f;
+#pragma unroll
+                    for (int r = 0; r < MT; ++r)
+                        sum[t][r][j] = fmaf(scale, fmaf(-zero, of_x[r][j], of_q[t][r][j]), sum[t][r][j]);
+                }
+        }
+    };
+
+    S now, next;
+    int b = wave;
+    if (b < a.blocks) load(now, b);
+    while (b < a.blocks) {
+        const int after = b + kWaves;
+        if (after < a.blocks) load(next, after);
+        add(now);
+        now = next;
+        b = after;
+    }
+
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < MT; ++r) parts[wave][t * MT + r][lane] = sum[t][r];
+    __syncthreads();
+    for (int i = wave; i < NT * MT; i += kWaves) {
+        f32x4_t v = parts[0][i][lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            const f32x4_t p = parts[w][i][lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = v[j] + p[j];
+        }
+        const int row = m0 + 16 * (i % MT) + c;
+        const int64_t col = (tile0 + i / MT) * 16 + 4 * g;
+        if (row >= a.m) continue;
+        const int64_t at = (int64_t)row * a.n + col;
+        const int left = (int)min((int64_t)4, a.n - col);
+        if (left <= 0) continue;
+        if (a.wide) {
+            if (a.bias) {
+                const u32x2_t bits = *(const u32x2_t*)(a.bias + col);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[j] += __uint_as_float(j % 2 ? bits[j / 2] & 0xFFFF0000u : bits[j / 2] << 16);
+            }
+            if (a.residual) v += *(const f32x4_t*)(a.residual + at);
+            if constexpr (OUT == NCM_OUT_BF16) {
+                *(u32x2_t*)((uint16_t*)a.y + at) =
+                    u32x2_t{bf16x2_bits_rne(v[0], v[1]), bf16x2_bits_rne(v[2], v[3])};
+            } else {
+                if constexpr (OUT == NCM_OUT_BF16_F32)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(bf16_bits_rne(v[j]) << 16);
+                *(f32x4_t*)((float*)a.y + at) = v;
+            }
+        } else {
+            for (int j = 0; j < left; ++j) {
+                float f = v[j];
+                if (a.bias) f += __uint_as_float((uint32_t)a.bias[col + j] << 16);
+                if (a.residual) f += a.residual[at + j];
+                if constexpr (OUT == NCM_OUT_BF16) ((uint16_t*)a.y)[at + j] = (uint16_t)bf16_bits_rne(f);
+                else ((float*)a.y)[at + j] =
+                    OUT == NCM_OUT_F32 ? f : __uint_as_float(bf16_bits_rne(f) << 16);
+            }
+        }
+    }
+}
+
+// Codes, a byte each, into the products' order; outputs past n and inputs past
+// k as codes 0 with scales 0.
+__global__ __launch_bounds__(256) void int4_pack_kernel(const uint8_t* codes, const uint16_t* scales,
+                                                        const uint8_t* zeros, int64_t n, int64_t k,
+                                                        int group, int64_t blocks, uint32_t* to,
+                                                        char* scales_to) {
+    const int64_t block = (int64_t)blockIdx.x;  // 16 outputs, 128 inputs
+    const int64_t tile = block / blocks, b = block - tile * blocks;
+    const int lane = threadIdx.x & 63, e = threadIdx.x >> 6;
+    const int64_t row = 16 * tile + (lane & 15), k0 = 128 * b + 32 * e + 8 * (lane >> 4);
+    uint32_t word = 0;
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t q = row < n && k0 + i < k ? codes[row * k + k0 + i] & 15u : 0u;
+        word |= q << (4 * (i / 2) + 16 * (i % 2));
+    }
+    to[(block * 64 + lane) * 4 + e] = word;
+    const int per = 128 / group, all = (int)((k + group - 1) / group);
+    if ((int)threadIdx.x < per * 16) {
+        const int i = threadIdx.x / 16;
+        const int64_t r = 16 * tile + threadIdx.x % 16, at = b * per + i;
+        const bool in = r < n && at < all;
+        const uint32_t s = in ? scales[r * all + at] : 0u;
+        const int64_t slot = block * per * 16 + threadIdx.x;
+        if (zeros) {
+            const float z = 128.0f + (in ? (float)(zeros[r * all + at] & 15) : 0.0f);
+            ((uint32_t*)scales_to)[slot] = s << 16 | __float_as_uint(z) >> 16;
+        } else {
+            ((uint16_t*)scales_to)[slot] = (uint16_t)s;
+        }
+    }
+}
+
+// A wavefront per group of a row.
+__global__ __launch_bounds__(256) void int4_quantise_kernel(const uint16_t* w, int64_t n, int64_t k,
+                                                            int64_t stride, int group, uint8_t* codes,
+                                                            uint16_t* scales, uint8_t* zeros) {
+    const int64_t all = (k + group - 1) / group;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (at >= n * all) return;
+    const int64_t row = at / all, k0 = (at - row * all) * group;
+    const int len = (int)min((int64_t)group, k - k0);
+    float v[2], lo = 0.0f, hi = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = lane + 64 * i;
+        v[i] = j < len ? __uint_as_float((uint32_t)w[row * stride + k0 + j] << 16) : 0.0f;
+        bad |= !(fabsf(v[i]) <= 3.40282347e38f);
+        lo = fminf(lo, v[i]), hi = fmaxf(hi, v[i]);
+    }
+    for (int x = 32; x; x >>= 1) lo = fminf(lo, __shfl_xor(lo, x)), hi = fmaxf(hi, __shfl_xor(hi, x));
+    bad = __any(bad);
+    // Divided before they are added: the range of the largest values has no float.
+    const float unit = zeros ? hi / 15.0f - lo / 15.0f : fmaxf(hi, -lo) / 7.0f;
+    const uint32_t bits = bad ? 0x7FC0u : bf16_bits_rne(unit);
+    const float s = __uint_as_float(bits << 16);
+    const bool none = bad || s == 0.0f;
+    const float z = none ? 8.0f : zeros ? fminf(fmaxf(rintf(-lo / s), 0.0f), 15.0f) : 8.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = lane + 64 * i;
+        if (j < len)
+            codes[row * k + k0 + j] =
+                (uint8_t)(none ? z : fminf(fmaxf(rintf(v[i] / s) + z, 0.0f), 15.0f));
+    }
+    if (lane == 0) {
+        scales[at] = (uint16_t)bits;
+        if (zeros) zeros[at] = (uint8_t)z;
+    }
+}
+
+int check_int4(int64_t n, int64_t k, int group) {
+    if (n < 0 || n > (1 << 28) || k < 8 || k > (1 << 24) || k % 8 ||
+        (group != 32 && group != 64 && group != 128))
+        return NCM_E_SHAPE;
+    // A workgroup per 16 outputs and 128 inputs packs them.
+    return (n + 15) / 16 * ((k + 127) / 128) > kMaxBlocks ? NCM_E_SHAPE : NCM_OK;
+}
+
+template <int GROUP, bool ZEROS, int NT, int MT>
+void launch_out(const Int4Args& a, int out, dim3 grid, hipStream_t st) {
+    if (out == NCM_OUT_F32) linear_int4_kernel<GROUP, ZEROS, NT, MT, NCM_OUT_F32><<<grid, 64 * kWaves, 0, st>>>(a);
+    else if (out == NCM_OUT_BF16) linear_int4_kernel<GROUP, ZEROS, NT, MT, NCM_OUT_BF16><<<grid, 64 * kWaves, 0, st>>>(a);
+    else linear_int4_kernel<GROUP, ZEROS, NT, MT, NCM_OUT_BF16_F32><<<grid, 64 * kWaves, 0, st>>>(a);
+}
+
+template <int GROUP, bool ZEROS>
+void launch(const Int4Args& a, int out, hipStream_t st) {
+    const int64_t tiles = (a.n + 15) / 16;
+    auto go = [&](auto nt, auto mt) {
+        constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value;
+        launch_out<GROUP, ZEROS, NT, MT>(
+            a, out, dim3((uint32_t)((tiles + NT - 1) / NT), (uint32_t)((a.m + 16 * MT - 1) / (16 * MT))), st);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 4> four;
+    if (a.m <= 16) go(one, one);
+    else if (a.m <= 32) go(two, two);
+    else go(two, four);
+}
+
+}  // namespace
+}  // namespace ncm
+
+extern "C" int ncm_int4_bytes(int64_t n, int64_t k, int group, int has_zeros, size_t* codes,
+                              size_t* scales) {
+    using namespace ncm;
+    if (!codes || !scales) return NCM_E_NULL;
+    *codes = *scales = 0;
+    const int rc = check_int4(n, k, group);
+    if (rc) return rc;
+    const size_t blocks = (size_t)((n + 15) / 16) * (size_t)((k + 127) / 128);
+    *codes = blocks * 1024;
+    *scales = blocks * (128 / group) * 16 * (has_zeros ? 4 : 2);
+    return NCM_OK;
+}
+
+extern "C" int ncm_int4_quantise_dev(ncm_ctx_t* ctx, const uint16_t* w, int64_t n, int64_t k,
+                                     int64_t stride, int group, uint8_t* codes, uint16_t* scales,
+                                     uint8_t* zeros) {
+    using namespace ncm;
+    if (!ctx) return NCM_E_NULL;
+    int rc = check_int4(n, k, group);
+    if (rc) return rc;
+    if (stride < k || stride > (int64_t(1) << 40)) return NCM_E_SHAPE;
+    const int64_t groups = (k + group - 1) / group;
+    if ((n * groups + 3) / 4 > kMaxBlocks) return NCM_E_SHAPE;
+    if (n == 0) return NCM_OK;
+    if (!w || !codes || !scales) return NCM_E_NULL;
+    const DeviceScope scope(ncm_ctx_device(ctx));
+    rc = step_hip(scope.error(), "int4_quantise device");
+    if (rc) return rc;
+    int4_quantise_kernel<<<(uint32_t)((n * groups + 3) / 4), 256, 0, ncm_ctx_stream(ctx)>>>(
+        w, n, k, stride, group, codes, scales, zeros);
+    return step_hip(hipGetLastError(), "int4_quantise launch");
+}
+
+extern "C" int ncm_int4_pack_dev(ncm_ctx_t* ctx, const uint8_t* codes, const uint16_t* scales,
+                                 const uint8_t* zeros, int64_t n, int64_t k, int group,
+                                 void* packed_codes, void* packed_scales) {
+    using namespace ncm;
+    if (!ctx) return NCM_E_NULL;
+    int rc = check_int4(n, k, group);
+    if (rc || n == 0) return rc;
+    if (!codes || !scales || !packed_codes || !packed_scales) return NCM_E_NULL;
+    if ((uintptr_t)packed_codes % 16 || (uintptr_t)packed_scales % 16) return NCM_E_ARG;
+    const DeviceScope scope(ncm_ctx_device(ctx));
+    rc = step_hip(scope.error(), "int4_pack device");
+    if (rc) return rc;
+    const int64_t blocks = (k + 127) / 128;
+    int4_pack_kernel<<<(uint32_t)((n + 15) / 16 * blocks), 256, 0, ncm_ctx_stream(ctx)>>>(
+        codes, scales, zeros, n, k, group, blocks, (uint32_t*)packed_codes, (char*)packed_scales);
+    return step_hip(hipGetLastError(), "int4_pack launch");
+}
+
+extern "C" int ncm_linear_int4(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride,
+                               const ncm_int4_weight_t* w, const uint16_t* bias,
+                               const float* residual, void* y, int64_t m, int out_mode) {
+    using namespace ncm;
+    if (!ctx || !w) return NCM_E_NULL;
+    int rc = check_int4(w->n, w->k, w->group);
+    if (rc) return rc;
+    if (m < 0 || m > (1 << 20)) return NCM_E_SHAPE;
+    if (out_mode != NCM_OUT_F32 && out_mode != NCM_OUT_BF16 && out_mode != NCM_OUT_BF16_F32)
+        return NCM_E_ARG;
+    if (m == 0 || w->n == 0) return NCM_OK;
+    rc = check_rows(x, x_stride, w->k);
+    if (rc) return rc;
+    if (!w->codes || !w->scales || !y) return NCM_E_NULL;
+    const int size = out_mode == NCM_OUT_BF16 ? 2 : 4;
+    if ((uintptr_t)w->codes % 16 || (uintptr_t)w->scales % 16 || (uintptr_t)y % size ||
+        (uintptr_t)bias % 2 || (uintptr_t)residual % 4)
+        return NCM_E_ARG;
+    if (residual == y && size == 2) return NCM_E_ARG;
+    const bool wide = w->n % 4 == 0 && (uintptr_t)y % (4 * size) == 0 && (uintptr_t)bias % 8 == 0 &&
+                      (uintptr_t)residual % 16 == 0;
+    const Int4Args a = {x, (const u32x4_t*)w->codes, (const char*)w->scales, bias, residual, y,
+                        x_stride, (int)m, (int)w->n, (int)w->k, (int)((w->k + 127) / 128), wide};
+    const DeviceScope scope(ncm_ctx_device(ctx));
+    rc = step_hip(scope.error(), "linear_int4 device");
+    if (rc) return rc;
+    const hipStream_t st = ncm_ctx_stream(ctx);
+    auto go = [&](auto group) {
+        constexpr int GROUP = decltype(group)::value;
+        w->has_zeros ? launch<GROUP, true>(a, out_mode, st) : launch<GROUP, false>(a, out_mode, st);
+    };
+    if (w->group == 32) go(std::integral_constant<int, 32>());
+    else if (w->group == 64) go(std::integral_constant<int, 64>());
+    else go(std::integral_constant<int, 128>());
+    return step_hip(hipGetLastError(), "linear_int4 launch");
+}

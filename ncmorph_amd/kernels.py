@@ -298,6 +298,107 @@ def linear_bf16_rope64(x, w, rot_cols: int, seq_len: int, cosine, sine, bias=Non
     return out
 
 
+class _Int4(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("n", C.c_int64),
+                ("k", C.c_int64), ("group", C.c_int32), ("has_zeros", C.c_int32)]
+
+
+class Int4Weight:
+    """A weight matrix [n, k] in 4-bit codes, packed for linear_int4 (pack_int4
+    makes it). It keeps the addresses of its two buffers."""
+
+    __slots__ = ("codes", "scales", "n", "k", "group", "struct", "named")
+
+    def __init__(self, codes, scales, n: int, k: int, group: int, has_zeros: bool):
+        a = _ck.Args("Int4Weight")
+        need = C.c_size_t(), C.c_size_t()
+        check(lib().ncm_int4_bytes(n, k, group, int(has_zeros), *map(C.byref, need)), a.where)
+        pc = a.dev(codes, "codes", ("uint8",), (need[0].value,))
+        ps = a.dev(scales, "scales", ("uint8",), (need[1].value,))
+        self.codes, self.scales, self.n, self.k, self.group = codes, scales, n, k, group
+        self.struct = _Int4(pc, ps, n, k, group, int(has_zeros))
+        self.named = tuple(a.seen)
+
+
+def pack_int4(codes, scales, group: int, zeros=None, ctx=None) -> Int4Weight:
+    """The Int4Weight of codes (uint8 [n, k], 0 to 15), scales (torch.bfloat16
+    [n, ceil(k / group)]) and zeros (uint8, likewise; None: 8 everywhere):
+    weight = (code - zero) * scale. group: 32, 64 or 128; k a multiple of 8."""
+    import torch
+
+    W = "pack_int4"
+    a = _ck.Args(W)
+    n, k = _ck.dims(codes, "codes", W, 2)
+    need = C.c_size_t(), C.c_size_t()
+    check(lib().ncm_int4_bytes(n, k, group, int(zeros is not None), *map(C.byref, need)), W)
+    groups = (k + group - 1) // group
+    pc = a.dev(codes, "codes", ("uint8",), (n, k))
+    ps = a.dev(scales, "scales", _ck.BF16, (n, groups))
+    pz = a.dev(zeros, "zeros", ("uint8",), (n, groups), optional=True)
+    a.done()
+    packed = [torch.empty(s.value, dtype=torch.uint8, device=codes.device) for s in need]
+    ctx = stream_context(codes.device, ctx)
+    check(lib().ncm_int4_pack_dev(ctx.handle, pc, ps, pz, n, k, group, packed[0].data_ptr(),
+                                  packed[1].data_ptr()), W)
+    return Int4Weight(*packed, n, k, group, zeros is not None)
+
+
+def quantise_int4(w, group: int, symmetric: bool = True, ctx=None):
+    """(codes, scales, zeros) of a bf16 matrix w [n, >= k] with contiguous rows,
+    as pack_int4 takes them. symmetric: scale = bf16(max |w| / 7) of a group,
+    code = rint(w / scale) + 8 and zeros None; else the range from min(w, 0) to
+    max(w, 0) in 15 steps. A group with a NaN or an infinity gets the scale NaN."""
+    import torch
+
+    W = "quantise_int4"
+    a = _ck.Args(W)
+    n, k = _ck.dims(w, "w", W, 2)
+    need = C.c_size_t(), C.c_size_t()
+    check(lib().ncm_int4_bytes(n, k, group, int(not symmetric), *map(C.byref, need)), W)
+    pw, stride = a.rows(w, "w", _ck.BF16, n, k)
+    a.done()
+    groups, dv = (k + group - 1) // group, w.device
+    codes = torch.empty(n, k, dtype=torch.uint8, device=dv)
+    scales = torch.empty(n, groups, dtype=torch.bfloat16, device=dv)
+    zeros = None if symmetric else torch.empty(n, groups, dtype=torch.uint8, device=dv)
+    ctx = stream_context(dv, ctx)
+    check(lib().ncm_int4_quantise_dev(ctx.handle, pw, n, k, stride if n > 1 else k, group,
+                                      codes.data_ptr(), scales.data_ptr(),
+                                      None if symmetric else zeros.data_ptr()), W)
+    return codes, scales, zeros
+
+
+def linear_int4(x, w: Int4Weight, bias=None, residual=None, out=None, out_mode: str = "f32",
+                ctx=None):
+    """y = x @ weight.T (+ bias) (+ residual) with 4-bit weights: x
+    torch.bfloat16 [m, >= k] with contiguous rows, bias bf16 [n], residual
+    float32 [m, n], sums in fp32 and one rounding; out [m, n] float32 ("f32",
+    "bf16_f32") or torch.bfloat16 ("bf16"), for the float modes residual itself
+    if wanted. For the rows of a decode step; it uses no workspace."""
+    import torch
+
+    W = "linear_int4"
+    a = _ck.Args(W)
+    if not isinstance(w, Int4Weight):
+        raise NcmError(-7, W, "w must be an Int4Weight")
+    m, _ = _ck.dims(x, "x", W, 2)
+    n, mode = w.n, _mode(out_mode, W)
+    px, stride = a.rows(x, "x", _ck.BF16, m, w.k)
+    pb = a.dev(bias, "bias", _ck.BF16, (n,), optional=True)
+    pr = a.dev(residual, "residual", _ck.F32, (m, n), optional=True)
+    if out is None:
+        out = _new_out(torch, mode, (m, n), x.device)
+        po = out.data_ptr()
+    else:
+        po = a.dev(out, "out", _out_dtypes(mode), (m, n))
+    a.seen += w.named
+    a.done()
+    ctx = stream_context(x.device, ctx)
+    check(lib().ncm_linear_int4(ctx.handle, px, stride if m > 1 else (w.k + 7) // 8 * 8,
+                                C.byref(w.struct), pb, pr, po, m, mode), W)
+    return out
+
+
 def linear_f32(x, w, out=None, ctx=None):
     """y = x @ w.T with float32 operands [m, k] and [n, k] (k % 4 == 0) on
     the fp32 MFMA, on torch's current stream."""
