@@ -723,6 +723,24 @@ int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
                          int64_t window, const int32_t* positions, const uint64_t* tree_mask,
                          int64_t mask_words, void* workspace, size_t workspace_bytes);
 
+/* ncm_kv_attention_dev of requests that share prefixes: the requests
+ * groups[g] .. groups[g + 1] - 1 of group g (device int32 [n_groups + 1],
+ * ascending; n_groups at most requests) hold the same tokens 0 .. shared[g] - 1
+ * (int32 [n_groups]), and what is before shared[g] in a request's own tokens
+ * (before its rows, that is) is read through the page table's row of the group's
+ * first request, once for all of them. A request of no group, of a group of one
+ * or with shared[g] <= 0 reads its own row alone. All else is as there; the sums
+ * are made in another order. */
+int ncm_kv_attention_shared_workspace(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
+                                      int64_t n_groups, int q_heads, size_t* bytes);
+int ncm_kv_attention_shared_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
+                                const ncm_kv_batch_t* batch, const int32_t* groups,
+                                const int32_t* shared, int64_t n_groups, const uint16_t* q,
+                                uint16_t* out, int q_heads, int64_t q_stride, int64_t out_stride,
+                                float scale, int64_t window, const int32_t* positions,
+                                const uint64_t* tree_mask, int64_t mask_words, void* workspace,
+                                size_t workspace_bytes);
+
 /* The pages of a cache that belong to nobody, and who holds the others. Device
  * memory; a new pool has free = any order of all pages, count = pages, refs 0
  * and marks INT64_MAX. free is a stack: pages are taken from free[count - 1]

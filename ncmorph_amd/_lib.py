@@ -79,6 +79,9 @@ SIGNATURES = [
     ("ncm_kv_attention_workspace", i32, [vp, vp, i32, C.POINTER(sz)]),
     ("ncm_kv_attention_dev", i32, [vp, vp, vp, vp, vp, i32, i64, i64, C.c_float, i64, vp, vp, i64,
                                    vp, sz]),
+    ("ncm_kv_attention_shared_workspace", i32, [vp, vp, i64, i32, C.POINTER(sz)]),
+    ("ncm_kv_attention_shared_dev", i32, [vp, vp, vp, vp, vp, i64, vp, vp, i32, i64, i64,
+                                          C.c_float, i64, vp, vp, i64, vp, sz]),
     ("ncm_pages_share_dev", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i32]),
     ("ncm_pages_extend_dev", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i32, i64, vp, i64, vp, vp,
                                    vp, vp, vp]),

@@ -184,7 +184,7 @@ def read(kv: KvCache, page_table, offsets, starts, rows: int, out=None, ctx=None
 
 def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_mask=None,
               window: int = 0, positions=None, scale: float | None = None, out=None,
-              workspace=None, ctx=None):
+              workspace=None, ctx=None, groups=None, shared=None):
     """Attention of a step's queries, torch.bfloat16 [rows, >= q_heads *
     head_dim] with contiguous rows, over the cache, which holds the step's own
     K and V already; torch.bfloat16 [rows, q_heads * head_dim]. A row sees the
@@ -196,7 +196,11 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
     (int32) or starts + its index. Rows that see nothing get zeros.
     scale: head_dim ** -0.5 by default. out may be q; a new one's rows of no
     request are not initialised. workspace: uint8 scratch, taken from torch's
-    allocator where not given."""
+    allocator where not given.
+    groups (int32 [n + 1], ascending) and shared (int32 [n]): requests groups[g]
+    .. groups[g + 1] - 1 hold the same first shared[g] tokens; of the tokens
+    before a request's rows those are read through the page table's row of its
+    group's first request, once for the whole group."""
     import torch
 
     W = "cache.attention"
@@ -212,9 +216,18 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
     if tree_mask is not None and words == 0:
         pm = b.offsets  # a mask of no words has no address of its own; nothing is read there
     pp = a.dev(positions, "positions", _ck.I32, (rows,), optional=True)
+    if (groups is None) != (shared is None):
+        raise NcmError(-1, W, "groups and shared come together")
     need = C.c_size_t()
-    check(lib().ncm_kv_attention_workspace(C.byref(kv.struct), C.byref(b), q_heads,
-                                           C.byref(need)), W)
+    if groups is None:
+        check(lib().ncm_kv_attention_workspace(C.byref(kv.struct), C.byref(b), q_heads,
+                                               C.byref(need)), W)
+    else:
+        (n_groups,) = _ck.dims(shared, "shared", W, 1)
+        pg = a.dev(groups, "groups", _ck.I32, (n_groups + 1,))
+        psh = a.dev(shared, "shared", _ck.I32, (n_groups,))
+        check(lib().ncm_kv_attention_shared_workspace(C.byref(kv.struct), C.byref(b), n_groups,
+                                                      q_heads, C.byref(need)), W)
     if out is None:
         out = torch.empty(rows, q_heads * hd, dtype=torch.bfloat16, device=q.device)
         po, os_ = out.data_ptr(), q_heads * hd
@@ -227,10 +240,15 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
         pw = a.dev(workspace, "workspace", ("uint8",))
     a.done()
     ctx = stream_context(q.device, ctx)
-    check(lib().ncm_kv_attention_dev(ctx.handle, C.byref(kv.struct), C.byref(b), pq, po, q_heads,
-                                     qs, os_, hd ** -0.5 if scale is None else scale, window, pp,
-                                     pm, words, pw,
-                                     workspace.numel()), W)
+    scale = hd ** -0.5 if scale is None else scale
+    if groups is None:
+        check(lib().ncm_kv_attention_dev(ctx.handle, C.byref(kv.struct), C.byref(b), pq, po,
+                                         q_heads, qs, os_, scale, window, pp, pm, words, pw,
+                                         workspace.numel()), W)
+    else:
+        check(lib().ncm_kv_attention_shared_dev(
+            ctx.handle, C.byref(kv.struct), C.byref(b), pg, psh, n_groups, pq, po, q_heads, qs,
+            os_, scale, window, pp, pm, words, pw, workspace.numel()), W)
     return out
 
 
