@@ -9,19 +9,20 @@
 // where 64-bit arithmetic puts it.
 //
 // Few tokens matter to a row: those next to its cuts and to its draw. Where they
-// stand is found from sums over 2048 bins of 1/64 of (max - x) / T, the last of
-// them for what is too far below to have a weight:
-//   1. the first token of each slice of a row;
+// stand is found from sums over 2048 bins of (max - x) / T, equally wide over the
+// row's range or over the 31 units in which tokens have weights:
+//   1. the largest logit of every segment (1 KB) of a row, by many workgroups;
 //   2. weights (and numbers, for top-k) of its bins, in LDS, then added to the
-//      row's in memory;
+//      row's in memory; segments whose largest logit is behind the k-th largest
+//      of the segments', or too weak for min-p, are left out;
 //   3. the bins that a cut or the draw can fall into, from the row's bins, and
-//      their tokens into a list;
+//      their tokens into a list, from the segments that can have some;
 //   4. each listed token's cumulative weight, exactly, from its bin's and the
 //      listed tokens of its bin; cuts and draw are minima over these.
-// A row whose list would be longer than 1024 (many equal logits, a temperature
-// that puts thousands of tokens into a bin) is done digit by digit of the
-// token's 52-bit place in the order (32 bits of the logit, 20 of the id): sums of
-// the tokens by their next digit, then the digit where the target is passed.
+// A row that lists more than 1024 (many equal logits) is done digit by digit
+// of the token's 52-bit place in the order (32 bits of the logit, 20 of the id):
+// sums of the tokens by their next digit, then the digit where the target is
+// passed.
 #include "step.h"
 
 namespace ncm {
@@ -52,7 +53,7 @@ struct RowRule {
     double top_p;    // 1: off
     double min_p;    // 0: off
     double uniform;
-    float bins;      // 64 / T: bins a unit of logit
+    float bins;      // bins a unit of logit, at least
     int top_k;       // 0: off
     int greedy;
     int request;     // -1: none
@@ -67,6 +68,8 @@ struct Ranges {
     int strong;         // bins below it hold only tokens of at least min_p
     int pad;
 
+    __device__ __forceinline__ int first() const { return min(min(lo[0], lo[1]), min(lo[2], lo[3])); }
+    __device__ __forceinline__ int last() const { return max(max(hi[0], hi[1]), max(hi[2], hi[3])); }
     __device__ __forceinline__ bool has(int b) const {
         bool in = false;
 #pragma unroll
@@ -79,27 +82,29 @@ struct Ranges {
 struct RowSpace {
     RowRule* rule;
     uint64_t* sums;     // [kBins]
+    uint32_t* counts;   // [kBins]
+    uint2* ends;        // [slices]: the first and the last key of a slice
+    Ranges* ranges;
     uint64_t* list;     // [kList]: places
     uint64_t* below;    // [kList]: the sum of the bins below the place's
     uint32_t* ahead;    // [kList]: their number
-    Ranges* ranges;
-    uint64_t* firsts;   // [slices]: each slice's first place
-    uint32_t* counts;   // [kBins]
     uint32_t* listed;   // places there are for the list
+    uint32_t* firsts;   // [segments]: the first key of a segment
 };
 
 __device__ __forceinline__ RowSpace row_space(const SampleArgs& a, int row) {
     char* p = a.space + row * a.row_bytes;
     RowSpace r;
     r.rule = (RowRule*)p;
-    r.sums = (uint64_t*)(p + sizeof(RowRule));
+    r.ranges = (Ranges*)(p + sizeof(RowRule));
+    r.sums = (uint64_t*)(r.ranges + 1);
     r.list = r.sums + kBins;
     r.below = r.list + kList;
-    r.firsts = r.below + kList;
-    r.ranges = (Ranges*)(r.firsts + a.slices);
-    r.counts = (uint32_t*)(r.ranges + 1);
+    r.ends = (uint2*)(r.below + kList);
+    r.counts = (uint32_t*)(r.ends + a.slices);
     r.ahead = r.counts + kBins;
     r.listed = r.ahead + kList;
+    r.firsts = r.listed + 1;
     return r;
 }
 
@@ -146,23 +151,35 @@ __device__ __forceinline__ float value_of(float x) {
     x = x == x ? fminf(x, 3.40282347e38f) : -INFINITY;
     return x == 0.0f ? 0.0f : x;
 }
-// Ascending in the order.
-__device__ __forceinline__ uint64_t place_of(float x, int id) {
+// A logit's key, and with its id its place: both ascending in the order. No key
+// is kNoKey, that of the NaN of all ones.
+constexpr uint32_t kNoKey = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t b = __float_as_uint(x);
-    const uint32_t up = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return ((uint64_t)~up << 20) | (uint32_t)id;
+    return b & 0x80000000u ? b : ~(b | 0x80000000u);
 }
-constexpr uint64_t kNowhere = (uint64_t)0xFFFFFFFFu << 20;  // above every place: NaN's bits
-__device__ __forceinline__ float place_value(uint64_t p) {
-    const uint32_t up = ~(uint32_t)(p >> 20);
-    return __uint_as_float(up & 0x80000000u ? up & 0x7FFFFFFFu : ~up);
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7FFFFFFFu);
 }
+__device__ __forceinline__ uint64_t place_of(float x, int id) {
+    return ((uint64_t)key_of(x) << 20) | (uint32_t)id;
+}
+__device__ __forceinline__ float place_value(uint64_t p) { return key_value((uint32_t)(p >> 20)); }
 __device__ __forceinline__ int place_id(uint64_t p) { return (int)(p & 0xFFFFFu); }
 
-// 2^(j / 32), in LDS.
+// 2^(j / 32), and in LDS.
+__device__ const double kPowers[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 typedef double Powers[32];
 __device__ __forceinline__ void fill(Powers& powers) {
-    if (threadIdx.x < 32) powers[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+    if (threadIdx.x < 32) powers[threadIdx.x] = kPowers[threadIdx.x];
 }
 
 // rint(2^43 exp((x - top) / T)), per = 32 log2(e) / T: a power of 2^(1 / 32) times
@@ -192,14 +209,6 @@ __device__ __forceinline__ uint64_t share_of(double f, uint64_t total, bool& mor
     return (hi << 11) | (lo >> 53);
 }
 
-template <bool BF16>
-__device__ __forceinline__ float load_logit(const SampleArgs& a, int row, int i) {
-    const int64_t at = (int64_t)row * a.stride + i;
-    const float x = BF16 ? __uint_as_float((uint32_t)((const uint16_t*)a.logits)[at] << 16)
-                         : ((const float*)a.logits)[at];
-    return value_of(x);
-}
-
 // The cumulative weight at which a part p of `total` is reached, and a draw's.
 __device__ __forceinline__ uint64_t cut_at(double p, uint64_t total) {
     bool more;
@@ -217,49 +226,77 @@ __device__ __forceinline__ void put_token(const SampleArgs& a, int row, uint64_t
     if (a.probabilities) a.probabilities[row] = (float)((double)weight / (double)kept);
 }
 
-// Accesses ahead: 16 logits.
+// A row in accesses of 16 bytes, aligned in memory, N logits each, and in segments
+// of 64 such accesses; the first and the last access may hold values that are not
+// the row's.
 template <bool BF16>
-constexpr int kAhead = BF16 ? 2 : 4;
+struct Row {
+    static constexpr int SIZE = BF16 ? 2 : 4, N = 16 / SIZE;
+    const char* base;
+    int skip;      // values ahead of the row in its first access
+    int vocab;
+    int segments;
 
-// The logits of a slice of a row, N of a 16-byte access at a time: f(values, id
-// of the first); values that are not the row's are -infinity.
-template <bool BF16, int AHEAD, typename F>
-__device__ __forceinline__ void each_logit(const SampleArgs& a, int row, int slice, int slices, F f) {
-    constexpr int SIZE = BF16 ? 2 : 4, N = 16 / SIZE;
-    const char* base = (const char*)a.logits + (int64_t)row * a.stride * SIZE;
-    const int skip = (int)((uintptr_t)base % 16) / SIZE;  // values ahead of the row in its first access
-    const int vectors = (a.vocab + skip + N - 1) / N;
-    const int v0 = (int)((int64_t)vectors * slice / slices);
-    const int v1 = (int)((int64_t)vectors * (slice + 1) / slices);
-    for (int v = v0 + (int)threadIdx.x; v < v1; v += kThreads * AHEAD) {
-        u32x4_t raw[AHEAD];
+    __device__ __forceinline__ Row(const SampleArgs& a, int row) {
+        base = (const char*)a.logits + (int64_t)row * a.stride * SIZE;
+        skip = (int)((uintptr_t)base % 16) / SIZE;
+        vocab = a.vocab;
+        segments = (vocab + skip + 64 * N - 1) / (64 * N);
+    }
+    // The id of the lane's first value of a segment.
+    __device__ __forceinline__ int first(int segment) const {
+        return (segment * 64 + (int)(threadIdx.x & 63)) * N - skip;
+    }
+    __device__ __forceinline__ bool whole(int segment) const {
+        return first(segment) >= 0 && first(segment) + N <= vocab;
+    }
+    __device__ __forceinline__ u32x4_t load(int segment) const {
+        u32x4_t raw = {0, 0, 0, 0};
+        if (whole(segment)) raw = *(const u32x4_t*)(base + (int64_t)first(segment) * SIZE);
+        return raw;
+    }
+    static __device__ __forceinline__ float raw_value(const u32x4_t& raw, int i) {
+        return BF16 ? __uint_as_float(i % 2 ? raw[i / 2] & 0xFFFF0000u : raw[i / 2] << 16)
+                    : __uint_as_float(raw[BF16 ? 0 : i]);
+    }
+    __device__ __forceinline__ float one(int id) const {
+        return value_of(BF16 ? __uint_as_float((uint32_t)((const uint16_t*)base)[id] << 16)
+                             : ((const float*)base)[id]);
+    }
+    // -infinity where there is no value of the row.
+    __device__ __forceinline__ void values(int segment, const u32x4_t& raw, float (&x)[N]) const {
+        if (whole(segment)) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int at = v + k * kThreads, first = at * N - skip;
-            if (at < v1 && first >= 0 && first + N <= a.vocab)
-                raw[k] = *(const u32x4_t*)(base + (int64_t)first * SIZE);
-        }
+            for (int i = 0; i < N; ++i)
+                x[i] = value_of(raw_value(raw, i));
+        } else {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int at = v + k * kThreads, first = at * N - skip;
-            if (at >= v1) break;
-            float x[N];
-            if (first >= 0 && first + N <= a.vocab) {
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    x[i] = value_of(BF16 ? __uint_as_float(i % 2 ? raw[k][i / 2] & 0xFFFF0000u
-                                                                 : raw[k][i / 2] << 16)
-                                         : __uint_as_float(raw[k][BF16 ? 0 : i]));
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    x[i] = first + i >= 0 && first + i < a.vocab ? load_logit<BF16>(a, row, first + i)
-                                                                 : -INFINITY;
+            for (int i = 0; i < N; ++i) {
+                const int id = first(segment) + i;
+                x[i] = id >= 0 && id < vocab ? one(id) : -INFINITY;
             }
-            f(x, first);
         }
     }
-}
+    // f(values, the lane's first id, segment) for segments s0 .. s1 - 1, one of
+    // every wavefront at a time and AHEAD of them loaded together.
+    template <int AHEAD, typename F>
+    __device__ __forceinline__ void each(int s0, int s1, F f) const {
+        for (int s = s0 + (int)(threadIdx.x >> 6); s < s1; s += kWavesOf * AHEAD) {
+            u32x4_t raw[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (s + k * kWavesOf < s1) raw[k] = load(s + k * kWavesOf);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int at = s + k * kWavesOf;
+                if (at >= s1) break;
+                float x[N];
+                values(at, raw[k], x);
+                f(x, first(at), at);
+            }
+        }
+    }
+};
 
 // Sums and numbers by a place's next digit.
 struct Digits {
@@ -274,7 +311,7 @@ struct Digits {
 // The first place whose cumulative weight (COUNT: number) is at least `target`;
 // sum: the cumulative weight there. False where all together is less.
 template <bool BF16, bool COUNT>
-__device__ bool find_place(const SampleArgs& a, int row, float top, const RowRule& q,
+__device__ bool find_place(const Row<BF16>& logits, float top, const RowRule& q,
                            const Powers& powers, uint64_t target, Digits& s, uint64_t& place,
                            uint64_t& sum) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -286,10 +323,9 @@ __device__ bool find_place(const SampleArgs& a, int row, float top, const RowRul
         for (int i = tid; i < 2048; i += kThreads) s.sums[i] = 0, s.counts[i] = 0;
         if (tid == 0) s.found = 0;
         __syncthreads();
-        each_logit<BF16, kAhead<BF16>>(a, row, 0, 1, [&](const auto& x, int first) {
-            constexpr int N = sizeof(x) / sizeof(float);
+        logits.template each<2>(0, logits.segments, [&](const auto& x, int first, int) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
+            for (int i = 0; i < Row<BF16>::N; ++i) {
                 const uint64_t p = place_of(x[i], first + i);
                 if (x[i] == -INFINITY || (p >> low) != prefix) continue;
                 const int digit = (int)((p >> next) & ((1 << bits) - 1));
@@ -368,10 +404,10 @@ __device__ __noinline__ void pick_by_digits(const SampleArgs& a, int row, const 
                                const Powers& powers, Digits& s) {
     const uint64_t least = least_weight(q);
     uint64_t all = 0, strong = 0;  // all weights, and those of at least min_p
-    each_logit<BF16, kAhead<BF16>>(a, row, 0, 1, [&](const auto& x, int) {
-        constexpr int N = sizeof(x) / sizeof(float);
+    const Row<BF16> logits(a, row);
+    logits.template each<2>(0, logits.segments, [&](const auto& x, int, int) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < Row<BF16>::N; ++i) {
             const uint64_t w = weight_of(x[i], top, q.per, powers);
             all += w;
             strong += w >= least ? w : 0;
@@ -380,25 +416,49 @@ __device__ __noinline__ void pick_by_digits(const SampleArgs& a, int row, const 
     all = total_of(all, s.wave_sums);
     strong = total_of(strong, s.wave_counts);
     uint64_t place, sum;
-    if (q.top_k && find_place<BF16, true>(a, row, top, q, powers, q.top_k, s, place, sum)) all = sum;
+    if (q.top_k && find_place<BF16, true>(logits, top, q, powers, q.top_k, s, place, sum)) all = sum;
     uint64_t kept = all;
     if (q.top_p < 1.0 &&
-        find_place<BF16, false>(a, row, top, q, powers, cut_at(q.top_p, all), s, place, sum))
+        find_place<BF16, false>(logits, top, q, powers, cut_at(q.top_p, all), s, place, sum))
         kept = min(kept, sum);
     kept = min(kept, strong);
-    find_place<BF16, false>(a, row, top, q, powers, draw_at(q.uniform, kept), s, place, sum);
+    find_place<BF16, false>(logits, top, q, powers, draw_at(q.uniform, kept), s, place, sum);
     if (threadIdx.x == 0)
         put_token(a, row, place, weight_of(place_value(place), top, q.per, powers), kept);
 }
 
-__device__ __forceinline__ int bin_of(float x, float top, const RowRule& q) {
-    return (int)fminf((top - x) * q.bins, (float)(kBins - 1));
+// The row's bins: at least 64 a unit of (max - x) / T, or 2047 over all its
+// values where these lie closer.
+struct Bins {
+    float top, per;
+    __device__ __forceinline__ int of(float x) const {
+        return (int)fminf((top - x) * per, (float)(kBins - 1));
+    }
+};
+
+// What all of a row's slices say: its first and its last value.
+__device__ __forceinline__ uint2 ends_of(const RowSpace& sp, int slices) {
+    const int lane = threadIdx.x & 63;
+    const uint2 e = lane < slices ? sp.ends[lane] : make_uint2(kNoKey, 0u);
+    return make_uint2(wave_min_xor(e.x), ~wave_min_xor(~e.y));
+}
+__device__ __forceinline__ Bins bins_of(uint2 ends, const RowRule& q) {
+    const float top = key_value(ends.x), range = top - key_value(ends.y);
+    return {top, range > 0.0f ? fmaxf(q.bins, fminf(2047.0f / range, 0x1p100f)) : q.bins};
+}
+
+// The bin where weights fall below min_p.
+__device__ __forceinline__ int weak_bin(const Bins& bins, const RowRule& q) {
+    // log(min_p) T of the logits' distance from the largest, in bins.
+    const double d = -log(q.min_p) * (32.0 * 1.44269504088896340736) / q.per * (double)bins.per;
+    return (int)fmin(d, (double)kBins);
 }
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads) void sample_first_kernel(SampleArgs a) {
-    __shared__ uint64_t waves[kWavesOf];
+    __shared__ uint2 waves[kWavesOf];
     const int row = (int)(blockIdx.x / (uint32_t)a.slices), slice = (int)(blockIdx.x % (uint32_t)a.slices);
+    const int lane = threadIdx.x & 63;
     const RowSpace sp = row_space(a, row);
     // What the row's next kernels start from.
     if (a.slices > 1)
@@ -408,48 +468,145 @@ __global__ __launch_bounds__(kThreads) void sample_first_kernel(SampleArgs a) {
         const RowRule q = rule_of(a, row);
         if (threadIdx.x == 0) *sp.rule = q, *sp.listed = 0;
     }
-    float top = -INFINITY;
-    int id = 0x7FFFFFFF;
-    each_logit<BF16, kAhead<BF16>>(a, row, slice, a.slices, [&](const auto& x, int first) {
-        constexpr int N = sizeof(x) / sizeof(float);
+    const Row<BF16> logits(a, row);
+    uint32_t first = kNoKey, last = 0;
+    logits.template each<4>((int)((int64_t)logits.segments * slice / a.slices),
+                            (int)((int64_t)logits.segments * (slice + 1) / a.slices),
+                            [&](const auto& x, int, int segment) {
+        uint32_t least = kNoKey;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            id = x[i] > top ? first + i : id;
-            top = fmaxf(top, x[i]);
+        for (int i = 0; i < Row<BF16>::N; ++i) {
+            const uint32_t key = key_of(x[i]);
+            const bool there = x[i] != -INFINITY;
+            least = min(least, there ? key : kNoKey);
+            last = max(last, there ? key : 0u);
         }
+        least = wave_min_xor(least);
+        if (lane == 0) sp.firsts[segment] = least;
+        first = min(first, least);
     });
-    const uint64_t place = least_of(top == -INFINITY ? kNowhere : place_of(top, id), waves);
-    if (threadIdx.x == 0) sp.firsts[slice] = place;
+    last = ~wave_min_xor(~last);
+    if (lane == 0) waves[threadIdx.x >> 6] = make_uint2(first, last);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kWavesOf; ++w) first = min(first, waves[w].x), last = max(last, waves[w].y);
+        sp.ends[slice] = make_uint2(first, last);
+    }
 }
 
-// The row's first place, from its slices'.
-__device__ __forceinline__ uint64_t first_of(const RowSpace& sp, int slices) {
+// The bin that holds the target'th of `counts` (kBins - 1 where there are fewer),
+// by one wavefront.
+__device__ __forceinline__ int bin_reaching(const uint32_t* counts, uint32_t target) {
     const int lane = threadIdx.x & 63;
-    return wave_least(lane < slices ? sp.firsts[lane] : kNowhere);
+    uint32_t n = 0;
+    for (int i = 0; i < 32; ++i) n += counts[32 * lane + (i + lane) % 32];
+    uint32_t at = n;
+    for (int x = 1; x < 64; x <<= 1) {
+        const uint32_t o = __shfl_up(at, x);
+        if (lane >= x) at += o;
+    }
+    const uint64_t there = __ballot(at >= target);
+    if (!there) return kBins - 1;
+    const int l = __ffsll((unsigned long long)there) - 1;
+    uint32_t c = lane < 32 ? counts[32 * l + lane] : 0;
+    for (int x = 1; x < 32; x <<= 1) {
+        const uint32_t o = __shfl_up(c, x);
+        if (lane >= x) c += o;
+    }
+    const uint32_t before = __shfl(at - n, l);
+    return 32 * l + __ffsll((unsigned long long)__ballot(lane < 32 && before + c >= target)) - 1;
 }
+
+// Segments that are looked at, in any order.
+struct Wanted {
+    int n;
+    uint16_t at[kMaxVocab / 256 + 1];
+
+    // Those of s0 .. s1 - 1 that begin at bin `far` or ahead of it; n is 0 before.
+    __device__ __forceinline__ void fill(const RowSpace& sp, const Bins& bins, int s0, int s1, int far) {
+        for (int i = s0 + (int)threadIdx.x; i < s1; i += kThreads) {
+            const uint32_t key = sp.firsts[i];
+            if (key != kNoKey && bins.of(key_value(key)) <= far) at[atomicAdd(&n, 1)] = (uint16_t)i;
+        }
+    }
+    // f(values, the lane's first id), as Row::each, of segments where some lane's
+    // access has ok(value).
+    template <int AHEAD, bool BF16, typename Ok, typename F>
+    __device__ __forceinline__ void each(const Row<BF16>& logits, Ok ok, F f) const {
+        for (int i = threadIdx.x >> 6; i < n; i += kWavesOf * AHEAD) {
+            u32x4_t raw[AHEAD];
+            int segment[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (i + k * kWavesOf < n) {
+                    segment[k] = __builtin_amdgcn_readfirstlane(at[i + k * kWavesOf]);
+                    raw[k] = logits.load(segment[k]);
+                }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                if (i + k * kWavesOf >= n) break;
+                bool some = !logits.whole(segment[k]);
+#pragma unroll
+                for (int e = 0; e < Row<BF16>::N; ++e) some |= ok(Row<BF16>::raw_value(raw[k], e));
+                if (!__any(some)) continue;
+                float x[Row<BF16>::N];
+                logits.values(segment[k], raw[k], x);
+                f(x, logits.first(segment[k]));
+            }
+        }
+    }
+};
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) {
     __shared__ uint64_t sums[kBins];
     __shared__ uint32_t counts[kBins];
     __shared__ Powers powers;
+    __shared__ int reach;
+    __shared__ Wanted wanted;
     const int row = (int)(blockIdx.x / (uint32_t)a.slices), slice = (int)(blockIdx.x % (uint32_t)a.slices);
     const RowSpace sp = row_space(a, row);
     const RowRule q = *sp.rule;
-    const uint64_t place = first_of(sp, a.slices);
-    if (q.request < 0 || q.greedy || place == kNowhere) return;
-    const float top = place_value(place);
+    const uint2 ends = ends_of(sp, a.slices);
+    if (q.request < 0 || q.greedy || ends.x == kNoKey) return;
+    const Bins bins = bins_of(ends, q);
+    const Row<BF16> logits(a, row);
     fill(powers);
     for (int i = threadIdx.x; i < kBins; i += kThreads) sums[i] = 0, counts[i] = 0;
+    if (threadIdx.x == 0) wanted.n = 0;
     __syncthreads();
-    each_logit<BF16, kAhead<BF16> / 2>(a, row, slice, a.slices, [&](const auto& x, int) {
-        constexpr int N = sizeof(x) / sizeof(float);
+    // Segments that begin behind bin `far` have nothing that counts.
+    int far = kBins;
+    if (q.top_k && q.top_k < logits.segments) {
+        // The k first of the segments' first tokens are k tokens: the k-th of all
+        // is not behind them.
+        for (int i = threadIdx.x; i < logits.segments; i += kThreads) {
+            const uint32_t key = sp.firsts[i];
+            if (key != kNoKey) atomicAdd(&counts[bins.of(key_value(key))], 1u);
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int b = bin_reaching(counts, (uint32_t)q.top_k);
+            if (threadIdx.x == 0) reach = b;
+        }
+        __syncthreads();
+        far = reach;
+        for (int i = threadIdx.x; i < kBins; i += kThreads) counts[i] = 0;
+        __syncthreads();
+    } else if (q.min_p > 0.0 && !q.top_k && q.top_p == 1.0) {
+        far = weak_bin(bins, q) + 1;
+    }
+    wanted.fill(sp, bins, (int)((int64_t)logits.segments * slice / a.slices),
+                (int)((int64_t)logits.segments * (slice + 1) / a.slices), far);
+    __syncthreads();
+    wanted.template each<BF16 ? 1 : 2>(logits, [](float) { return true; }, [&](const auto& x, int) {
+        constexpr int N = Row<BF16>::N;
         uint64_t w[N];
         int b[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = weight_of(x[i], top, q.per, powers);
+        for (int i = 0; i < N; ++i) w[i] = weight_of(x[i], bins.top, q.per, powers);
 #pragma unroll
-        for (int i = 0; i < N; ++i) b[i] = bin_of(x[i], top, q);
+        for (int i = 0; i < N; ++i) b[i] = bins.of(x[i]);
         if (q.top_k)
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -476,19 +633,29 @@ struct Cumulative {
     uint64_t wave_sums[4];
     uint32_t wave_counts[4];
 
-    // By the workgroup's first four wavefronts.
-    __device__ __forceinline__ void load(const RowSpace& sp) {
-        constexpr int PER = kBins / 256;
+    // By the workgroup's first four wavefronts, from what fetch() has read.
+    static constexpr int PER = kBins / 256;
+    struct Part {
+        uint64_t s[PER];
+        uint32_t n[PER];
+    };
+    static __device__ __forceinline__ Part fetch(const RowSpace& sp) {
+        Part f = {};
+        if (threadIdx.x < 256) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) f.s[i] = sp.sums[threadIdx.x * PER + i];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) f.n[i] = sp.counts[threadIdx.x * PER + i];
+        }
+        return f;
+    }
+    __device__ __forceinline__ void load(const Part& f) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-        uint64_t s[PER], w = 0, w_at = 0;
-        uint32_t n[PER], c = 0, c_at = 0;
+        uint64_t w = 0, w_at = 0;
+        uint32_t c = 0, c_at = 0;
         if (tid < 256) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) s[i] = sp.sums[tid * PER + i];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) n[i] = sp.counts[tid * PER + i];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) w += s[i], c += n[i];
+            for (int i = 0; i < PER; ++i) w += f.s[i], c += f.n[i];
             w_at = w, c_at = c;
             for (int x = 1; x < 64; x <<= 1) {
                 const uint64_t ow = __shfl_up((unsigned long long)w_at, x);
@@ -504,7 +671,7 @@ struct Cumulative {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 sums[tid * PER + i] = w_at, counts[tid * PER + i] = c_at;
-                w_at += s[i], c_at += n[i];
+                w_at += f.s[i], c_at += f.n[i];
             }
             if (tid == 255) sums[kBins] = w_at, counts[kBins] = c_at;
         }
@@ -523,7 +690,7 @@ struct Cumulative {
     }
 };
 
-__device__ __forceinline__ Ranges ranges_of(const Cumulative& c, const RowRule& q) {
+__device__ __forceinline__ Ranges ranges_of(const Cumulative& c, const Bins& bins, const RowRule& q) {
     typedef Cumulative C;
     Ranges g;
 #pragma unroll
@@ -549,7 +716,7 @@ __device__ __forceinline__ Ranges ranges_of(const Cumulative& c, const RowRule& 
     g.strong = kBins, g.sure = 0, g.pad = 0;
     if (q.min_p > 0.0) {
         // A bin to either side for the rounding of logarithm and bins.
-        const int b = (int)fminf(-logf((float)q.min_p) * 64.0f, (float)kBins);
+        const int b = weak_bin(bins, q);
         const int low = max(b - 1, 0), high = min(b + 1, kBins - 1);
         if (c.sums[low] < most) {
             g.lo[2] = low, g.hi[2] = high, g.strong = low, g.sure = c.sums[low];
@@ -564,17 +731,21 @@ __device__ __forceinline__ Ranges ranges_of(const Cumulative& c, const RowRule& 
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 8) void sample_list_kernel(SampleArgs a) {
-    __shared__ Cumulative bins;
+    __shared__ Cumulative sums;
     __shared__ Ranges ranges;
+    __shared__ Wanted wanted;
     const int row = (int)(blockIdx.x / (uint32_t)a.slices), slice = (int)(blockIdx.x % (uint32_t)a.slices);
     const RowSpace sp = row_space(a, row);
+    const Cumulative::Part part = Cumulative::fetch(sp);
     const RowRule q = *sp.rule;
-    const uint64_t first = first_of(sp, a.slices);
-    if (q.request < 0 || q.greedy || first == kNowhere) return;
-    const float top = place_value(first);
-    bins.load(sp);
+    const uint2 ends = ends_of(sp, a.slices);
+    if (q.request < 0 || q.greedy || ends.x == kNoKey) return;
+    const Row<BF16> logits(a, row);
+    const Bins bins = bins_of(ends, q);
+    if (threadIdx.x == 0) wanted.n = 0;
+    sums.load(part);
     if (threadIdx.x < 64) {
-        const Ranges g = ranges_of(bins, q);
+        const Ranges g = ranges_of(sums, bins, q);
         if (threadIdx.x == 0) {
             ranges = g;
             if (slice == 0) *sp.ranges = g;
@@ -582,16 +753,25 @@ __global__ __launch_bounds__(kThreads, 8) void sample_list_kernel(SampleArgs a) 
     }
     __syncthreads();
     const Ranges g = ranges;
-    each_logit<BF16, kAhead<BF16>>(a, row, slice, a.slices, [&](const auto& x, int id) {
-        constexpr int N = sizeof(x) / sizeof(float);
+    wanted.fill(sp, bins, (int)((int64_t)logits.segments * slice / a.slices),
+                (int)((int64_t)logits.segments * (slice + 1) / a.slices), g.last());
+    __syncthreads();
+    // Distances that can be in one of the ranges; infinity's, which counts as the
+    // largest, is -infinity here.
+    const float near = g.first() > 0 ? (float)g.first() : -INFINITY, far = (float)(g.last() + 1);
+    auto ok = [&](float x) {
+        const float d = (bins.top - x) * bins.per;
+        return d >= near && (d < far || far == (float)kBins);
+    };
+    wanted.template each<BF16 ? 2 : 4>(logits, ok, [&](const auto& x, int first) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int bin = bin_of(x[i], top, q);
-            if (x[i] == -INFINITY || !g.has(bin)) continue;
+        for (int e = 0; e < Row<BF16>::N; ++e) {
+            const int bin = bins.of(x[e]);
+            if (x[e] == -INFINITY || !g.has(bin)) continue;
             const uint32_t at = atomicAdd(sp.listed, 1u);
             if (at < kList)
-                sp.list[at] = place_of(x[i], id + i), sp.below[at] = bins.sums[bin],
-                sp.ahead[at] = bins.counts[bin];
+                sp.list[at] = place_of(x[e], first + e), sp.below[at] = sums.sums[bin],
+                sp.ahead[at] = sums.counts[bin];
         }
     });
 }
@@ -612,35 +792,57 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
         Digits digits;
     } s;
     __shared__ Powers powers;
-    const int row = blockIdx.x, tid = threadIdx.x;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const RowSpace sp = row_space(a, row);
+    const uint32_t listed = *sp.listed;
     const RowRule q = *sp.rule;
-    const uint64_t first = first_of(sp, a.slices);
-    const int n = (int)min(*sp.listed, (uint32_t)kList + 1);
     const Ranges g = *sp.ranges;
+    const uint2 ends = ends_of(sp, a.slices);
+    fill(powers);
     if (q.request < 0) return;
-    if (q.greedy || first == kNowhere) {
+    if (ends.x == kNoKey) {
         if (tid == 0) {
-            a.tokens[row] = first == kNowhere ? -1 : place_id(first);
-            if (a.probabilities) a.probabilities[row] = first == kNowhere ? 0.0f : 1.0f;
+            a.tokens[row] = -1;
+            if (a.probabilities) a.probabilities[row] = 0.0f;
         }
         return;
     }
-    const float top = place_value(first);
-    fill(powers);
-    __syncthreads();
-    if (n > kList) {
-        pick_by_digits<BF16>(a, row, q, top, powers, s.digits);
+    const Row<BF16> logits(a, row);
+    if (q.greedy) {
+        // The first segment that begins with the row's first key.
+        uint64_t at = ~0ull;
+        for (int i = tid; i < logits.segments; i += kThreads)
+            if (sp.firsts[i] == ends.x) at = min(at, (uint64_t)i);
+        at = least_of(at, s.digits.wave_sums);
+        if (tid >= 64) return;
+        float x[Row<BF16>::N];
+        logits.values((int)at, logits.load((int)at), x);
+        uint32_t id = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = Row<BF16>::N - 1; i >= 0; --i)
+            if (key_of(x[i]) == ends.x && x[i] != -INFINITY) id = (uint32_t)(logits.first((int)at) + i);
+        id = wave_min_xor(id);
+        if (tid == 0) {
+            a.tokens[row] = (int)id;
+            if (a.probabilities) a.probabilities[row] = 1.0f;
+        }
         return;
     }
+    const Bins bins = bins_of(ends, q);
+    __syncthreads();
+    if (listed > kList) {
+        pick_by_digits<BF16>(a, row, q, bins.top, powers, s.digits);
+        return;
+    }
+    const int n = (int)listed;
     uint64_t sum = 0, mine = 0;
     uint32_t count = 0;
     if (tid < n) {
         const uint64_t place = sp.list[tid];
         sum = sp.below[tid], count = sp.ahead[tid];
         const float x = place_value(place);
-        mine = (uint64_t)bin_of(x, top, q) << 52 | place;
-        s.p.list[tid] = Listed{mine, weight_of(x, top, q.per, powers)};
+        mine = (uint64_t)bins.of(x) << 52 | place;
+        s.p.list[tid] = Listed{mine, weight_of(x, bins.top, q.per, powers)};
     }
     __syncthreads();
     // The listed token's cumulative weight and number: its bin's tokens up to it
@@ -662,20 +864,20 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
     const uint64_t none = ~0ull;
     auto reaches = [&](uint64_t target) {  // the least sum of at least that
         uint64_t v = none;
-        for (int i = tid; i < n; i += 64) v = s.p.sums[i] >= target ? min(v, s.p.sums[i]) : v;
+        for (int i = lane; i < n; i += 64) v = s.p.sums[i] >= target ? min(v, s.p.sums[i]) : v;
         return wave_least(v);
     };
     uint64_t kept = g.all;
     if (g.lo[0] <= g.hi[0]) {
         uint64_t v = none;
-        for (int i = tid; i < n; i += 64) v = s.p.counts[i] == (uint32_t)q.top_k ? s.p.sums[i] : v;
+        for (int i = lane; i < n; i += 64) v = s.p.counts[i] == (uint32_t)q.top_k ? s.p.sums[i] : v;
         kept = wave_least(v);
     }
     if (q.top_p < 1.0) kept = min(kept, reaches(cut_at(q.top_p, kept)));
     if (g.strong < kBins) {
         const uint64_t least = least_weight(q);
         uint64_t v = 0;
-        for (int i = tid; i < n; i += 64) {
+        for (int i = lane; i < n; i += 64) {
             const Listed l = s.p.list[i];
             const int bin = (int)(l.place >> 52);
             v += bin >= g.lo[2] && bin <= g.hi[2] && l.weight >= least ? l.weight : 0;
@@ -683,7 +885,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
         kept = min(kept, g.sure + wave_total(v));
     }
     const uint64_t drawn = reaches(draw_at(q.uniform, kept));
-    for (int i = tid; i < n; i += 64) {
+    for (int i = lane; i < n; i += 64) {
         const Listed l = s.p.list[i];
         // One token of a weight has this sum.
         if (s.p.sums[i] == drawn && l.weight)
@@ -696,9 +898,10 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
 int64_t slices_of(int64_t rows, int64_t vocab) {
     return std::max<int64_t>(1, std::min<int64_t>((vocab + 16383) / 16384, 512 / std::max<int64_t>(rows, 1)));
 }
-static_assert(kMaxVocab / 16384 <= 64, "first_of has a lane per slice");
-int64_t row_bytes_of(int64_t slices) {
-    return (sizeof(RowRule) + sizeof(Ranges) + kBins * 12 + kList * 20 + slices * 8 + 4 + 15) / 16 * 16;
+static_assert(kMaxVocab / 16384 <= 64, "ends_of has a lane per slice");
+int64_t row_bytes_of(int64_t slices, int64_t vocab) {
+    const int64_t segments = vocab / 256 + 2;
+    return (sizeof(RowRule) + sizeof(Ranges) + kBins * 12 + kList * 20 + slices * 8 + (segments + 1) * 4 + 15) / 16 * 16;
 }
 
 template <bool BF16>
@@ -719,7 +922,7 @@ extern "C" int ncm_sample_workspace(int64_t rows, int64_t vocab, size_t* bytes) 
     if (!bytes) return NCM_E_NULL;
     *bytes = 0;
     if (rows < 0 || rows >= kMaxBlocks / 4 || vocab < 0 || vocab > kMaxVocab) return NCM_E_SHAPE;
-    if (rows > 0) *bytes = (size_t)rows * row_bytes_of(slices_of(rows, vocab));
+    if (rows > 0) *bytes = (size_t)rows * row_bytes_of(slices_of(rows, vocab), vocab);
     return NCM_OK;
 }
 
@@ -746,7 +949,7 @@ extern "C" int ncm_sample_dev(ncm_ctx_t* ctx, const ncm_sample_rules_t* rules, c
         return NCM_E_ARG;
     const int64_t slices = slices_of(rows, vocab);
     const SampleArgs a = {*rules, logits, uniform, tokens, probabilities, stride, (int)rows, (int)vocab,
-                          uniform_bits == 64, (char*)workspace, row_bytes_of(slices), (int)slices};
+                          uniform_bits == 64, (char*)workspace, row_bytes_of(slices, vocab), (int)slices};
     const DeviceScope scope(ncm_ctx_device(ctx));
     rc = step_hip(scope.error(), "sample device");
     if (rc) return rc;
