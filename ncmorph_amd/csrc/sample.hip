@@ -31,6 +31,10 @@ namespace {
 constexpr double kOne = 0x1p43;  // the largest weight
 constexpr int64_t kMaxVocab = int64_t(1) << 20;
 constexpr int kThreads = 1024, kWavesOf = kThreads / 64;
+// Of the row's last kernel: few enough for its rare part to have all the registers
+// that it wants (1024 threads of 128: scratch memory, 12 us in place of 5 for 4
+// rows that have no use for that part).
+constexpr int kPickThreads = 256, kPickWaves = kPickThreads / 64;
 constexpr int kBins = 2048, kList = 1024;
 
 struct SampleArgs {
@@ -279,16 +283,16 @@ struct Row {
     }
     // f(values, the lane's first id, segment) for segments s0 .. s1 - 1, one of
     // every wavefront at a time and AHEAD of them loaded together.
-    template <int AHEAD, typename F>
+    template <int AHEAD, int WAVES, typename F>
     __device__ __forceinline__ void each(int s0, int s1, F f) const {
-        for (int s = s0 + (int)(threadIdx.x >> 6); s < s1; s += kWavesOf * AHEAD) {
+        for (int s = s0 + (int)(threadIdx.x >> 6); s < s1; s += WAVES * AHEAD) {
             u32x4_t raw[AHEAD];
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k)
-                if (s + k * kWavesOf < s1) raw[k] = load(s + k * kWavesOf);
+                if (s + k * WAVES < s1) raw[k] = load(s + k * WAVES);
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k) {
-                const int at = s + k * kWavesOf;
+                const int at = s + k * WAVES;
                 if (at >= s1) break;
                 float x[N];
                 values(at, raw[k], x);
@@ -302,8 +306,8 @@ struct Row {
 struct Digits {
     uint64_t sums[2048];
     uint32_t counts[2048];
-    uint64_t wave_sums[kWavesOf];
-    uint64_t wave_counts[kWavesOf];
+    uint64_t wave_sums[kPickWaves];
+    uint64_t wave_counts[kPickWaves];
     uint64_t place, sum, count;
     int found;
 };
@@ -314,16 +318,17 @@ template <bool BF16, bool COUNT>
 __device__ bool find_place(const Row<BF16>& logits, float top, const RowRule& q,
                            const Powers& powers, uint64_t target, Digits& s, uint64_t& place,
                            uint64_t& sum) {
+    constexpr int PER = 2048 / kPickThreads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t prefix = 0, done_sum = 0, done_count = 0;
     int low = 52;  // digits above it are fixed
     while (low > 0) {
         const int bits = low > 30 ? 11 : 10, next = low - bits;
         __syncthreads();
-        for (int i = tid; i < 2048; i += kThreads) s.sums[i] = 0, s.counts[i] = 0;
+        for (int i = tid; i < 2048; i += kPickThreads) s.sums[i] = 0, s.counts[i] = 0;
         if (tid == 0) s.found = 0;
         __syncthreads();
-        logits.template each<2>(0, logits.segments, [&](const auto& x, int first, int) {
+        logits.template each<4, kPickWaves>(0, logits.segments, [&](const auto& x, int first, int) {
 #pragma unroll
             for (int i = 0; i < Row<BF16>::N; ++i) {
                 const uint64_t p = place_of(x[i], first + i);
@@ -335,26 +340,29 @@ __device__ bool find_place(const Row<BF16>& logits, float top, const RowRule& q,
             }
         });
         __syncthreads();
-        const uint64_t c0 = s.counts[2 * tid], c1 = s.counts[2 * tid + 1];
-        const uint64_t s0 = s.sums[2 * tid], s1 = s.sums[2 * tid + 1];
-        uint64_t c = c0 + c1, w = s0 + s1;
+        uint64_t c = 0, w = 0;
+        for (int i = 0; i < PER; ++i) c += s.counts[PER * tid + i], w += s.sums[PER * tid + i];
+        uint64_t c_at = c, w_at = w;
         for (int x = 1; x < 64; x <<= 1) {
-            const uint64_t oc = __shfl_up((unsigned long long)c, x), ow = __shfl_up((unsigned long long)w, x);
-            if (lane >= x) c += oc, w += ow;
+            const uint64_t oc = __shfl_up((unsigned long long)c_at, x);
+            const uint64_t ow = __shfl_up((unsigned long long)w_at, x);
+            if (lane >= x) c_at += oc, w_at += ow;
         }
-        if (lane == 63) s.wave_sums[wave] = w, s.wave_counts[wave] = c;
+        if (lane == 63) s.wave_sums[wave] = w_at, s.wave_counts[wave] = c_at;
         __syncthreads();
-        c += done_count, w += done_sum;
-        for (int v = 0; v < wave; ++v) c += s.wave_counts[v], w += s.wave_sums[v];
-        // Cumulative values ahead of, between and behind the thread's two digits.
-        const uint64_t c_at = c - c0 - c1, w_at = w - s0 - s1;
-        const uint64_t before = COUNT ? c_at : w_at, mid = COUNT ? c_at + c0 : w_at + s0;
-        if (before < target && target <= (COUNT ? c : w)) {
-            const bool second = mid < target;
-            s.found = 1;
-            s.place = (prefix << bits) | (uint64_t)(2 * tid + second);
-            s.sum = second ? w_at + s0 : w_at;
-            s.count = second ? c_at + c0 : c_at;
+        c_at += done_count - c, w_at += done_sum - w;
+        for (int v = 0; v < wave; ++v) c_at += s.wave_counts[v], w_at += s.wave_sums[v];
+        // The thread's digits from here on, the target among them or not.
+        for (int i = 0; i < PER; ++i) {
+            const uint64_t n = s.counts[PER * tid + i], m = s.sums[PER * tid + i];
+            const uint64_t before = COUNT ? c_at : w_at, after = before + (COUNT ? n : m);
+            if (before < target && target <= after) {
+                s.found = 1;
+                s.place = (prefix << bits) | (uint64_t)(PER * tid + i);
+                s.sum = w_at;
+                s.count = c_at;
+            }
+            c_at += n, w_at += m;
         }
         __syncthreads();
         if (!s.found) return false;
@@ -375,21 +383,21 @@ __device__ __forceinline__ uint64_t wave_total(uint64_t v) {
     return v;
 }
 // Of a workgroup's values.
-__device__ __forceinline__ uint64_t least_of(uint64_t v, uint64_t (&waves)[kWavesOf]) {
+__device__ __forceinline__ uint64_t least_of(uint64_t v, uint64_t (&waves)[kPickWaves]) {
     v = wave_least(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
     __syncthreads();
-    for (int w = 0; w < kWavesOf; ++w) v = min(v, waves[w]);
+    for (int w = 0; w < kPickWaves; ++w) v = min(v, waves[w]);
     return v;
 }
-__device__ __forceinline__ uint64_t total_of(uint64_t v, uint64_t (&waves)[kWavesOf]) {
+__device__ __forceinline__ uint64_t total_of(uint64_t v, uint64_t (&waves)[kPickWaves]) {
     v = wave_total(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
-    for (int w = 0; w < kWavesOf; ++w) v += waves[w];
+    for (int w = 0; w < kPickWaves; ++w) v += waves[w];
     return v;
 }
 
@@ -400,12 +408,12 @@ __device__ __forceinline__ uint64_t least_weight(const RowRule& q) {
 
 // A row by its places' digits.
 template <bool BF16>
-__device__ __noinline__ void pick_by_digits(const SampleArgs& a, int row, const RowRule& q, float top,
+__device__ void pick_by_digits(const SampleArgs& a, int row, const RowRule& q, float top,
                                const Powers& powers, Digits& s) {
     const uint64_t least = least_weight(q);
     uint64_t all = 0, strong = 0;  // all weights, and those of at least min_p
     const Row<BF16> logits(a, row);
-    logits.template each<2>(0, logits.segments, [&](const auto& x, int, int) {
+    logits.template each<4, kPickWaves>(0, logits.segments, [&](const auto& x, int, int) {
 #pragma unroll
         for (int i = 0; i < Row<BF16>::N; ++i) {
             const uint64_t w = weight_of(x[i], top, q.per, powers);
@@ -470,7 +478,7 @@ __global__ __launch_bounds__(kThreads) void sample_first_kernel(SampleArgs a) {
     }
     const Row<BF16> logits(a, row);
     uint32_t first = kNoKey, last = 0;
-    logits.template each<4>((int)((int64_t)logits.segments * slice / a.slices),
+    logits.template each<4, kWavesOf>((int)((int64_t)logits.segments * slice / a.slices),
                             (int)((int64_t)logits.segments * (slice + 1) / a.slices),
                             [&](const auto& x, int, int segment) {
         uint32_t least = kNoKey;
@@ -600,20 +608,23 @@ __global__ __launch_bounds__(kThreads, 8) void sample_bins_kernel(SampleArgs a) 
                 (int)((int64_t)logits.segments * (slice + 1) / a.slices), far);
     __syncthreads();
     wanted.template each<BF16 ? 1 : 2>(logits, [](float) { return true; }, [&](const auto& x, int) {
-        constexpr int N = Row<BF16>::N;
-        uint64_t w[N];
-        int b[N];
+        // Four weights side by side.
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = weight_of(x[i], bins.top, q.per, powers);
+        for (int h = 0; h < Row<BF16>::N; h += 4) {
+            uint64_t w[4];
+            int b[4];
 #pragma unroll
-        for (int i = 0; i < N; ++i) b[i] = bins.of(x[i]);
-        if (q.top_k)
+            for (int i = 0; i < 4; ++i) w[i] = weight_of(x[h + i], bins.top, q.per, powers);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (x[i] != -INFINITY) atomicAdd(&counts[b[i]], 1u);
+            for (int i = 0; i < 4; ++i) b[i] = bins.of(x[h + i]);
+            if (q.top_k)
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (w[i]) atomicAdd((unsigned long long*)&sums[b[i]], (unsigned long long)w[i]);
+                for (int i = 0; i < 4; ++i)
+                    if (x[h + i] != -INFINITY) atomicAdd(&counts[b[i]], 1u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (w[i]) atomicAdd((unsigned long long*)&sums[b[i]], (unsigned long long)w[i]);
+        }
     });
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
@@ -782,7 +793,7 @@ struct Listed {
 };
 
 template <bool BF16>
-__global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a) {
     __shared__ union Space {
         struct {
             Listed list[kList];
@@ -811,7 +822,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
     if (q.greedy) {
         // The first segment that begins with the row's first key.
         uint64_t at = ~0ull;
-        for (int i = tid; i < logits.segments; i += kThreads)
+        for (int i = tid; i < logits.segments; i += kPickThreads)
             if (sp.firsts[i] == ends.x) at = min(at, (uint64_t)i);
         at = least_of(at, s.digits.wave_sums);
         if (tid >= 64) return;
@@ -835,20 +846,18 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
         return;
     }
     const int n = (int)listed;
-    uint64_t sum = 0, mine = 0;
-    uint32_t count = 0;
-    if (tid < n) {
-        const uint64_t place = sp.list[tid];
-        sum = sp.below[tid], count = sp.ahead[tid];
+    for (int t = tid; t < n; t += kPickThreads) {
+        const uint64_t place = sp.list[t];
         const float x = place_value(place);
-        mine = (uint64_t)bins.of(x) << 52 | place;
-        s.p.list[tid] = Listed{mine, weight_of(x, bins.top, q.per, powers)};
+        s.p.list[t] = Listed{(uint64_t)bins.of(x) << 52 | place, weight_of(x, bins.top, q.per, powers)};
     }
     __syncthreads();
     // The listed token's cumulative weight and number: its bin's tokens up to it
     // are those at most its place in the bin below it.
-    if (tid < n) {
-        const uint64_t reach = mine & ((uint64_t(1) << 52) - 1);
+    for (int t = tid; t < n; t += kPickThreads) {
+        uint64_t sum = sp.below[t];
+        uint32_t count = sp.ahead[t];
+        const uint64_t mine = s.p.list[t].place, reach = mine & ((uint64_t(1) << 52) - 1);
 #pragma unroll 8
         for (int i = 0; i < n; ++i) {
             const Listed other = s.p.list[i];
@@ -856,7 +865,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
             sum += in ? other.weight : 0;
             count += in;
         }
-        s.p.sums[tid] = sum, s.p.counts[tid] = count;
+        s.p.sums[t] = sum, s.p.counts[t] = count;
     }
     __syncthreads();
     // The rest by one wavefront, without barriers.
@@ -910,7 +919,7 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
     sample_first_kernel<BF16><<<blocks, kThreads, 0, st>>>(a);
     sample_bins_kernel<BF16><<<blocks, kThreads, 0, st>>>(a);
     sample_list_kernel<BF16><<<blocks, kThreads, 0, st>>>(a);
-    sample_pick_kernel<BF16><<<(uint32_t)a.rows, kThreads, 0, st>>>(a);
+    sample_pick_kernel<BF16><<<(uint32_t)a.rows, kPickThreads, 0, st>>>(a);
     return hipGetLastError();
 }
 
