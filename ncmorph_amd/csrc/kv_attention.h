@@ -258,6 +258,35 @@ __device__ __forceinline__ uint32_t seen_tokens(const AttnArgs& a, const Need& d
     return see;
 }
 
+// Adds what of a token's V is not finite to the outputs of the lane's pairs that
+// see it.
+template <int HD, int CODES, int R, bool PREFIX>
+__device__ __forceinline__ void add_odd(const AttnArgs& a, int h, int token, int page,
+                                        const bool (&sees)[R], State<HD, R, PREFIX>& st, int g) {
+    typedef Tile<HD, CODES> T;
+    const int64_t row = ((int64_t)h << a.cache.page_log2) +
+                        (token & ((1 << a.cache.page_log2) - 1));
+    const char* p = a.cache.v + ((int64_t)page * a.cache.v_stride + row * HD) * T::ES;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const typename T::vec v = *(const typename T::vec*)(p + (4 * g + x) * (HD / 16) * T::ES);
+#pragma unroll
+        for (int u = 0; u < T::VW; ++u) {
+            const uint32_t odd = v[u] & not_finite<CODES>(v[u]);
+#pragma unroll
+            for (int k = 0; k < 4 / T::ES; ++k) {
+                // Where it is not finite, the value; else 0.
+                const uint32_t bits = odd >> (8 * T::ES * k);
+                const float add = T::ES == 2 ? __uint_as_float(bits << 16)
+                                             : (bits & 0x7Fu) ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+                for (int rr = 0; rr < R; ++rr)
+                    st.o[rr][4 / T::ES * u + k][x] += sees[rr] ? add : 0.0f;
+            }
+        }
+    }
+}
+
 // V where some tokens are not there, or hold a value that is not finite: 0
 // times either must stay 0 for a pair that does not see them. Tokens that are
 // not there become zero, whatever their places hold. Infinities and NaN become
@@ -287,31 +316,11 @@ __device__ __forceinline__ void clean_values(const AttnArgs& a, int h, int key, 
         const int i = 4 * (at / 16) + at % 4, tg = (at % 16) / 4;
         const uint64_t in_lanes = __ballot(g == tg && ((bad >> i) & 1u));
         if (!in_lanes) continue;
-        const int64_t page = at < 16 ? page0 : page1;
-        const int64_t row = ((int64_t)h << a.cache.page_log2) +
-                            ((key + at) & ((1 << a.cache.page_log2) - 1));
-        const char* p = a.cache.v + (page * a.cache.v_stride + row * HD) * T::ES;
+        const int page = at < 16 ? page0 : page1;
         bool sees[R];
 #pragma unroll
         for (int rr = 0; rr < R; ++rr) sees[rr] = (__shfl((int)see[rr], 16 * tg + c) >> i) & 1;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const typename T::vec v = *(const typename T::vec*)(p + (4 * g + x) * (HD / 16) * T::ES);
-#pragma unroll
-            for (int u = 0; u < T::VW; ++u) {
-                const uint32_t odd = v[u] & not_finite<CODES>(v[u]);
-#pragma unroll
-                for (int k = 0; k < 4 / T::ES; ++k) {
-                    // Where it is not finite, the value; else 0.
-                    const uint32_t bits = odd >> (8 * T::ES * k);
-                    const float add = T::ES == 2 ? __uint_as_float(bits << 16)
-                                                 : (bits & 0x7Fu) ? __builtin_nanf("") : 0.0f;
-#pragma unroll
-                    for (int rr = 0; rr < R; ++rr)
-                        st.o[rr][4 / T::ES * u + k][x] += sees[rr] ? add : 0.0f;
-                }
-            }
-        }
+        add_odd<HD, CODES, R>(a, h, key + at, page, sees, st, g);
     }
 }
 
@@ -439,13 +448,44 @@ __device__ __forceinline__ void add_tokens(const AttnArgs& a, const Need& d, int
 }
 
 
+// The tokens that a row of a group's requests sees of their prefix: those above
+// near and below limit.
+__device__ __forceinline__ void pair_sees(const AttnArgs& a, const Need& d, int row, int& near,
+                                          int& limit) {
+    // The request of the row: as many as end at or before it.
+    int lo = 0, hi = a.batch.requests - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.batch.offsets[mid + 1] > d.q.o0 + row) hi = mid;
+        else lo = mid + 1;
+    }
+    const int before = max(a.batch.starts[lo], 0);
+    limit = min(d.end, before);
+    near = d.floor - 1;
+    if (a.window > 0) {
+        int64_t pos = (int64_t)before + max(d.q.o0 + row - a.batch.offsets[lo], 0);
+        if (a.positions) pos = max(a.positions[d.q.o0 + row], before);
+        near = max(near, (int)min(max(pos - a.window, (int64_t)-1), kMaxTokens));
+    }
+}
+
+// Whether every row of requests r0 .. r1 - 1 sees every token of the group's
+// prefix, by each wavefront: what saves it the search for its rows' requests.
+__device__ __forceinline__ bool all_see(const AttnArgs& a, const Need& d, int r0, int r1) {
+    if (a.window > 0) return false;
+    int least = 0x7FFFFFFF;
+    for (int r = r0 + (int)(threadIdx.x & 63); r < r1; r += 64) least = min(least, a.batch.starts[r]);
+    return __all(least >= d.end);
+}
+
 // Tiles [first, first + count) of a unit, by the whole workgroup: into `out`
 // where part < 0, else as a part, from its row `part` on. r: the table's row.
 // PREFIX: the rows are those of several requests, and each sees the tokens below
-// d.end that lie before its own request's rows.
+// d.end that lie before its own request's rows; r1: the request behind them.
 template <int HD, int CODES, int R, bool PREFIX>
 __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r, int h, int block,
-                                         int first, int count, int64_t part, Lds<HD, R>& lds) {
+                                         int first, int count, int64_t part, Lds<HD, R>& lds,
+                                         int r1 = 0) {
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int pairs = d.q.n * a.group - block * 16 * R;  // of the unit, in all
@@ -453,6 +493,7 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
     State<HD, R, PREFIX> st;
     int far = d.floor - 1;  // the largest `near`
     int whole = d.before;   // tokens below it are seen by all, the window aside
+    const bool plain = PREFIX && all_see(a, d, r, r1);
     // A negative scale turns the queries' signs, so that the maximum of the
     // products is that of the scores.
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
@@ -477,23 +518,14 @@ __device__ __forceinline__ void run_unit(const AttnArgs& a, const Need& d, int r
         st.l[rr] = 0.0f;
         st.row[rr] = row;
         st.near[rr] = d.floor - 1;
-        int before = d.q.before, index = row;
         if constexpr (PREFIX) {
-            // The request of the row: as many as end at or before it.
-            int lo = 0, hi = a.batch.requests - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (a.batch.offsets[mid + 1] > d.q.o0 + row) hi = mid;
-                else lo = mid + 1;
-            }
-            before = max(a.batch.starts[lo], 0);
-            index = max(d.q.o0 + row - a.batch.offsets[lo], 0);
-            st.limit[rr] = min(d.end, before);
+            if (plain) st.limit[rr] = d.end;
+            else pair_sees(a, d, row, st.near[rr], st.limit[rr]);
+            far = max(far, st.near[rr]);
             whole = min(whole, st.limit[rr]);
-        }
-        if (a.window > 0) {
-            int64_t pos = (int64_t)before + index;
-            if (a.positions) pos = max(a.positions[d.q.o0 + row], before);
+        } else if (a.window > 0) {
+            int64_t pos = (int64_t)d.q.before + row;
+            if (a.positions) pos = max(a.positions[d.q.o0 + row], d.q.before);
             st.near[rr] = max(st.near[rr], (int)min(max(pos - a.window, (int64_t)-1), kMaxTokens));
             far = max(far, st.near[rr]);
         }

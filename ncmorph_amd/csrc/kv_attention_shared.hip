@@ -12,6 +12,11 @@
 // behind them, of tiles of 128 tokens; all tiles in a row are cut into equal
 // runs, one per workgroup. Every unit that is not whole in one run, and every
 // unit of rows that have a prefix, goes to the workspace in parts.
+//
+// Groups of many pairs are bound by products and softmax instead of the prefix's
+// bytes, and have a kernel of their own (kv_attention_prefix_kernel): wavefronts
+// of 32 pairs each, which share tiles of K and V as bf16 in LDS. It does the tiles
+// that every row of the group sees whole, the units above the prefix's rest.
 #include "kv_attention.h"
 
 namespace ncm {
@@ -23,10 +28,18 @@ struct SharedArgs {
     const int32_t* shared;  // [n_groups]
     int n_groups;
     int prefix_units, own_units;  // there is room for
-    int* counts;                  // units there are: the groups', the requests'
+    // Groups of many pairs: {first request, tokens, first row, rows} of what their
+    // own kernel does (NULL: it does not run), its units, their pairs and parts.
+    int4* plans;
+    int wide_units, wide_pairs;
+    int* wide_base;
+    int4* wide_joins;
+    int64_t wide_cut, whole_wide;
+    int* counts;                  // units there are: the groups', the requests', the wide ones
     int* unit_base;               // of a group
     int4* joins;                  // {first workgroup, parts, segment, unit of the segment}
     int64_t whole_prefix, whole_own;  // rows of the parts of units in one run
+    int64_t prefix_cut;               // rows of the parts of groups' units in several
 };
 
 // Group g's requests [r0, r1) and the tokens that they share; none where there
@@ -54,12 +67,6 @@ __device__ __forceinline__ int group_with(const SharedArgs& s, int r) {
     return lo < s.n_groups && s.groups[lo] <= r ? lo : -1;
 }
 
-// Tokens of request r that it reads through its group.
-__device__ __forceinline__ int prefix_of(const SharedArgs& s, int r, int before) {
-    const int g = group_with(s, r);
-    return g < 0 ? 0 : min(group_of(s, g).tokens, before);
-}
-
 template <int RP>
 __device__ __forceinline__ Need group_need(const SharedArgs& s, int g) {
     const Group q = group_of(s, g);
@@ -67,8 +74,9 @@ __device__ __forceinline__ Need group_need(const SharedArgs& s, int g) {
     Need d;
     d.q.o0 = d.q.n = 0;
     d.q.before = d.end = d.before = q.tokens;
-    d.base = d.floor = d.tile0 = 0;
-    if (q.tokens > 0) {
+    d.base = d.floor = s.plans ? s.plans[g].y : 0;
+    d.tile0 = 0;
+    if (q.tokens > d.base) {
         d.q.o0 = min(max(a.batch.offsets[q.r0], 0), a.batch.rows);
         d.q.n = max(min(a.batch.offsets[q.r1], a.batch.rows) - d.q.o0, 0);
         if (a.window > 0) {
@@ -77,7 +85,7 @@ __device__ __forceinline__ Need group_need(const SharedArgs& s, int g) {
             d.tile0 = (int)(max((int64_t)least - a.window + 1, (int64_t)0) / kTile);
         }
     }
-    d.tiles = max((d.end + kTile - 1) / kTile - d.tile0, 1);
+    d.tiles = max((d.end - d.base + kTile - 1) / kTile - d.tile0, 1);
     d.blocks = (int)(((int64_t)d.q.n * a.group + 16 * RP - 1) / (16 * RP));
     return d;
 }
@@ -90,7 +98,8 @@ __device__ __forceinline__ Need own_need(const SharedArgs& s, int r) {
     d.q = request_of(a.batch, r);
     d.end = (int)min((int64_t)d.q.before + d.q.n, cap);
     d.before = (int)min((int64_t)d.q.before, cap);
-    d.floor = prefix_of(s, r, d.before);
+    const int g = group_with(s, r);
+    d.floor = g < 0 ? 0 : min(group_of(s, g).tokens, d.before);
     const int64_t low = a.window > 0 ? max((int64_t)d.q.before - a.window + 1, (int64_t)0) : 0;
     d.base = (int)max((int64_t)d.floor, min(low, cap)) & ~15;
     d.tile0 = 0;
@@ -197,11 +206,450 @@ __global__ __launch_bounds__(256, 2) void kv_attention_shared_kernel(SharedArgs 
         if (!room) {
             // Offsets that give rows to several requests: no record, no result.
         } else if (is_group) {
-            run_unit<HD, CODES, RP, true>(a, d, group_of(s, seg).r0, h, block, first, count, part, lds);
+            const Group of = group_of(s, seg);
+            run_unit<HD, CODES, RP, true>(a, d, of.r0, h, block, first, count, part, lds, of.r1);
         } else {
             run_unit<HD, CODES, RO, false>(a, d, seg - s.n_groups, h, block, first, count, part,
                                            reinterpret_cast<Lds<HD, RO>&>(lds));
         }
+        at += count;
+    }
+}
+
+// ------------------------------------------------------- groups of many pairs
+
+constexpr int kWideTile = 64;   // tokens of a tile
+constexpr int kWidePairs = 48;  // of a group, from which on it has the kernel
+
+// A tile of K and V as bf16, rows of HD values; 16-byte chunk c of row r of K is
+// at chunk c ^ (r % 16) (HD 64: c ^ (r / 2 % 8)), so that the sixteen rows of an
+// operand's reads fall into different banks.
+template <int HD>
+struct WideTile {
+    u32x4_t k[kWideTile][HD / 8];
+    u32x4_t v[kWideTile][HD / 8];
+    float ks[kWideTile], vs[kWideTile];
+    static __device__ __forceinline__ int place(int row, int chunk) {
+        return HD == 128 ? chunk ^ (row & 15) : chunk ^ ((row >> 1) & 7);
+    }
+};
+template <int HD>
+struct WideLds {
+    WideTile<HD> tile[2];
+    uint64_t gone[4];        // of four tiles in turn: tokens that are not there
+    float m[4][2][64], l[4][2][64];
+};
+
+// What a thread brings of a tile: eight threads a token, codes of 16 bytes.
+template <int HD, int CODES>
+struct WideLoad {
+    static constexpr int ES = CODES == NCM_KV_BF16 ? 2 : 1, N = HD * ES / 128;  // of 16 bytes
+    static constexpr bool HALF = HD * ES < 128;  // 64 codes: every second thread
+    u32x4_t k[N ? N : 1], v[N ? N : 1];
+    float ks, vs;
+    bool ok;
+
+    __device__ __forceinline__ void load(const KvView& cache, int h, int token, int page) {
+        const int lane = threadIdx.x & 7;
+        ok = page >= 0;
+        const int64_t at = ((int64_t)h << cache.page_log2) + (token & ((1 << cache.page_log2) - 1));
+        const int64_t p = max(page, 0);
+        if (!HALF || lane < 4) {
+#pragma unroll
+            for (int i = 0; i < (N ? N : 1); ++i) {
+                k[i] = *(const u32x4_t*)(cache.k + (p * cache.k_stride + at * HD) * ES + 16 * (lane + 8 * i));
+                v[i] = *(const u32x4_t*)(cache.v + (p * cache.v_stride + at * HD) * ES + 16 * (lane + 8 * i));
+            }
+        }
+        if constexpr (CODES != NCM_KV_BF16)
+            if (lane == 0) ks = cache.ks[p * cache.ks_stride + at], vs = cache.vs[p * cache.vs_stride + at];
+    }
+
+    // Into the tile, zeros for a token that is not there.
+    __device__ __forceinline__ void store(WideTile<HD>& tile, uint64_t* gone) {
+        const int row = threadIdx.x >> 3, lane = threadIdx.x & 7;
+        const u32x4_t zero = {0, 0, 0, 0};
+        if (!HALF || lane < 4) {
+#pragma unroll
+            for (int i = 0; i < (N ? N : 1); ++i) {
+                const u32x4_t x = ok ? k[i] : zero, y = ok ? v[i] : zero;
+                if constexpr (CODES == NCM_KV_BF16) {
+                    const int chunk = lane + 8 * i;
+                    tile.k[row][WideTile<HD>::place(row, chunk)] = x;
+                    tile.v[row][chunk] = y;
+                } else {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        u32x4_t a, b;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            uint32_t lo, hi;
+                            widen4<CODES>(x[2 * half + j], lo, hi);
+                            a[2 * j] = lo, a[2 * j + 1] = hi;
+                            widen4<CODES>(y[2 * half + j], lo, hi);
+                            b[2 * j] = lo, b[2 * j + 1] = hi;
+                        }
+                        const int chunk = 2 * (lane + 8 * i) + half;
+                        tile.k[row][WideTile<HD>::place(row, chunk)] = a;
+                        tile.v[row][chunk] = b;
+                    }
+                }
+            }
+        }
+        if (lane == 0) {
+            if constexpr (CODES != NCM_KV_BF16) tile.ks[row] = ok ? ks : 0.0f, tile.vs[row] = ok ? vs : 0.0f;
+            if (!ok) atomicOr((unsigned long long*)gone, 1ull << row);
+        }
+    }
+};
+
+// Adds 32 tokens of a tile, from row `base` on, to a wavefront's 32 pairs, which
+// all see them; gone: those that are not there. The arithmetic is add_tokens'.
+template <int HD, int CODES>
+__device__ __forceinline__ void add_wide(State<HD, 2, false>& st,
+                                         const bf16x8_t (&q)[2][HD / 32], const WideTile<HD>& tile,
+                                         int base, uint32_t gone,
+                                         float to_log2, float lag) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    float s[2][8];
+    {
+        f32x4_t sc[2][2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int row = base + 16 * half + c;
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) sc[rr][half] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < HD / 32; ++k) {
+                const bf16x8_t op = __builtin_bit_cast(bf16x8_t, tile.k[row][WideTile<HD>::place(row, 4 * k + g)]);
+#pragma unroll
+                for (int rr = 0; rr < 2; ++rr)
+                    sc[rr][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(op, q[rr][k], sc[rr][half], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            f32x4_t ks = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (CODES != NCM_KV_BF16) ks = *(const f32x4_t*)&tile.ks[base + 16 * half + 4 * g];
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[rr][4 * half + i] = sc[rr][half][i];
+                    if constexpr (CODES != NCM_KV_BF16) s[rr][4 * half + i] *= ks[i] * to_log2;
+                }
+        }
+    }
+    if (gone)
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                s[rr][i] = (gone >> (16 * (i / 4) + 4 * g + i % 4)) & 1u ? -INFINITY : s[rr][i];
+    f32x4_t vs[2] = {{1.0f, 1.0f, 1.0f, 1.0f}, {1.0f, 1.0f, 1.0f, 1.0f}};
+    if constexpr (CODES != NCM_KV_BF16)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) vs[half] = *(const f32x4_t*)&tile.vs[base + 16 * half + 4 * g];
+    bf16x8_t p[2], rest[2];
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+        float top = s[rr][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[rr][i]);
+        top = max_over_groups(top);
+        if (__any(top > st.m[rr] + (CODES == NCM_KV_BF16 ? lag : 8.0f))) {
+            top = fmaxf(top, st.m[rr]);
+            const float d = st.m[rr] - top;
+            const float f = __builtin_amdgcn_exp2f(CODES == NCM_KV_BF16 ? d * to_log2 : d);
+            st.m[rr] = top;
+            st.l[rr] *= f;
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) st.o[rr][n] *= f;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float d = s[rr][i] - st.m[rr];
+            s[rr][i] = __builtin_amdgcn_exp2f(CODES == NCM_KV_BF16 ? d * to_log2 : d);
+            sum += s[rr][i];
+            if constexpr (CODES != NCM_KV_BF16) s[rr][i] = s[rr][i] * vs[i / 4][i % 4];
+        }
+        st.l[rr] += sum;
+        u32x4_t hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = __float_as_uint(s[rr][2 * i]), y = __float_as_uint(s[rr][2 * i + 1]);
+            hi[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+            lo[i] = bf16x2_rne(fmaf(s[rr][2 * i], 1.00000095367431640625f,
+                                    -__uint_as_float(x & 0xFFFF0000u)),
+                               fmaf(s[rr][2 * i + 1], 1.00000095367431640625f,
+                                    -__uint_as_float(y & 0xFFFF0000u)));
+        }
+        p[rr] = __builtin_bit_cast(bf16x8_t, hi);
+        rest[rr] = __builtin_bit_cast(bf16x8_t, lo);
+    }
+    // Not read ahead of the softmax: there are no registers for them beside its own.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    typedef uint32_t vec __attribute__((ext_vector_type(HD / 32)));
+    vec raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        raw[i] = ((const vec*)tile.v[base + 16 * (i / 4) + 4 * g + i % 4])[c];
+#pragma unroll
+    for (int f = 0; f < HD / 64; ++f) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            u32x4_t w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = __builtin_amdgcn_perm(raw[2 * j + 1][2 * f + n / 2], raw[2 * j][2 * f + n / 2],
+                                             n % 2 ? 0x07060302u : 0x05040100u);
+            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, w);
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr)
+                st.o[rr][4 * f + n] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rr], st.o[rr][4 * f + n], 0, 0, 0);
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr)
+                st.o[rr][4 * f + n] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest[rr], st.o[rr][4 * f + n], 0, 0, 0);
+        }
+    }
+}
+
+// What the kernel does of a group.
+struct Wide {
+    int r0, o0, rows, tiles, blocks;
+};
+__device__ __forceinline__ Wide wide_of(const SharedArgs& s, int g) {
+    const int4 p = s.plans[g];
+    return {p.x, p.z, p.w, max(p.y / kWideTile, 1),
+            (int)(((int64_t)p.w * s.a.group + s.wide_pairs - 1) / s.wide_pairs)};
+}
+
+// Tiles [first, first + count) of a group's unit, into the part that begins at row
+// `part`: NP wavefronts of 32 pairs each, and 8 / NP of such sets, which take
+// halves of the tiles and every other tile.
+template <int HD, int CODES, int NP>
+__device__ __forceinline__ void run_wide(const SharedArgs& s, const Wide& d, int h, int block,
+                                         int first, int count, int64_t part, WideLds<HD>& lds) {
+    constexpr int NS = 8 / NP, NR = NS < 2 ? 1 : 2;  // wavefronts of a tile's rounds
+    const AttnArgs& a = s.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int c = lane & 15, g = lane >> 4, np = wave % NP, ns = wave / NP;
+    const int pairs = d.rows * a.group - block * 32 * NP;
+    const int key0 = first * kWideTile, mine = key0 + (tid >> 3);
+    auto page = [&](int t) {  // of the thread's token of tile t
+        return t < count ? page_of(a.batch, a.cache, d.r0, mine + t * kWideTile) : -1;
+    };
+    WideLoad<HD, CODES> next;
+    const int page0 = page(0);
+    int page2 = page(1);
+    if (tid < 4) lds.gone[tid] = 0;
+    State<HD, 2, false> st;
+    bf16x8_t q[2][HD / 32];
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+    const float to_log2 = a.scale == 0.0f ? 1.4e-45f : fabsf(a.scale) * 1.4426950408889634f;
+    const float lag = fminf(8.0f / to_log2, 1e30f);
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+        const int pair = block * 32 * NP + min(32 * np + 16 * rr + c, pairs - 1);
+        const int row = pair / a.group, head = h * a.group + pair - row * a.group;
+        const uint16_t* from = a.q + (d.o0 + row) * a.q_stride + (int64_t)head * HD + 8 * g;
+#pragma unroll
+        for (int k = 0; k < HD / 32; ++k)
+            q[rr][k] = __builtin_bit_cast(bf16x8_t, *(const u32x4_t*)(from + 32 * k) ^ sign);
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) st.o[rr][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        st.m[rr] = kNoMax;
+        st.l[rr] = 0.0f;
+    }
+    next.load(a.cache, h, mine, page0);
+    __syncthreads();
+    next.store(lds.tile[0], &lds.gone[0]);
+    if (count > 1) next.load(a.cache, h, mine + kWideTile, page2);
+    page2 = page(2);
+    lds_barrier();
+    // Tile t is in one buffer, t + 1 in registers on its way to the other, and the
+    // page of t + 2 known.
+    for (int t = 0; t < count; ++t) {
+        const WideTile<HD>& tile = lds.tile[t & 1];
+        const uint64_t gone = uniform((int64_t)lds.gone[t & 3]);
+#pragma unroll 1
+        for (int round = 0; round < kWideTile / 32 / NR; ++round) {
+            const int base = 32 * (round * NR + ns % NR);
+            if (NS <= 2 || (t & 1) == ns / 2)
+                add_wide<HD, CODES>(st, q, tile, base, (uint32_t)(gone >> base), to_log2, lag);
+        }
+        if (tid == 0) lds.gone[(t + 2) & 3] = 0;
+        if (t + 1 < count) {
+            next.store(lds.tile[(t + 1) & 1], &lds.gone[(t + 1) & 3]);
+            if (t + 2 < count) next.load(a.cache, h, mine + (t + 2) * kWideTile, page2);
+            page2 = page(t + 3);
+        }
+        lds_barrier();  // the loads stay in flight
+    }
+    // The states of one NP wavefronts' pairs into those of the first NP: by halves,
+    // through the tiles' LDS, in chunks of a row of lanes.
+    float m[2], l[2];
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+        l[rr] = sum_over_groups(st.l[rr]);
+        m[rr] = st.m[rr];
+        if (CODES == NCM_KV_BF16 && m[rr] > kNoMax) m[rr] = fmaxf(m[rr] * to_log2, kNoMax);
+    }
+    f32x4_t* mem = (f32x4_t*)lds.tile;
+    static_assert(sizeof(lds.tile) >= 4 * 2 * (HD / 16) * 64 * 16, "four states");
+#pragma unroll
+    for (int half = NS / 2; half >= 1; half /= 2) {
+        if (ns >= half && ns < 2 * half) {
+            const int at = (wave - half * NP) * 2;
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+#pragma unroll
+                for (int n = 0; n < HD / 16; ++n) mem[((at + rr) * (HD / 16) + n) * 64 + lane] = st.o[rr][n];
+                lds.m[wave - half * NP][rr][lane] = m[rr], lds.l[wave - half * NP][rr][lane] = l[rr];
+            }
+        }
+        __syncthreads();
+        if (ns < half) {
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+                const float m2 = lds.m[wave][rr][lane], l2 = lds.l[wave][rr][lane];
+                const float top = fmaxf(m[rr], m2);
+                const float f = __builtin_amdgcn_exp2f(m[rr] - top), e = __builtin_amdgcn_exp2f(m2 - top);
+                l[rr] = l[rr] * f + l2 * e;
+                m[rr] = top;
+#pragma unroll
+                for (int n = 0; n < HD / 16; ++n)
+                    st.o[rr][n] = st.o[rr][n] * f + mem[((wave * 2 + rr) * (HD / 16) + n) * 64 + lane] * e;
+            }
+        }
+        __syncthreads();
+    }
+    if (ns == 0) {
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+            const int pr = 32 * np + 16 * rr + c;
+            if (pr >= pairs) continue;
+            const int64_t at = part + pr;
+            if (g == 0) a.part_ml[at] = float2{m[rr], l[rr]};
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int n = 0; n < HD / 16; n += 4) {
+                    f32x4_t v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = st.o[rr][n + i][x];
+                    *(f32x4_t*)(a.part_o + at * HD + (HD / 16) * (4 * g + x) + n) = v;
+                }
+        }
+    }
+    __syncthreads();
+}
+
+// What the kernel below does of each group, by a wavefront: the tiles of tokens
+// that all its requests with rows have before these.
+__global__ __launch_bounds__(256) void kv_attention_plan_kernel(SharedArgs s) {
+    const int g = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (g >= s.n_groups) return;
+    const Group q = group_of(s, g);
+    const BatchView& b = s.a.batch;
+    int least = q.tokens;
+    if (q.tokens > 0)
+        for (int r = q.r0 + lane; r < q.r1; r += 64) {
+            const Request one = request_of(b, r);
+            least = min(least, one.n > 0 ? one.before : q.tokens);
+        }
+    for (int x = 32; x; x >>= 1) least = min(least, __shfl_xor(least, x));
+    if (lane == 0) {
+        int4 plan = {q.r0, least / kWideTile * kWideTile, 0, 0};
+        if (plan.y > 0) {
+            plan.z = min(max(b.offsets[q.r0], 0), b.rows);
+            plan.w = max(min(b.offsets[q.r1], b.rows) - plan.z, 0);
+        }
+        s.plans[g] = plan;
+    }
+}
+
+template <int HD, int CODES, int NP>
+__global__ __launch_bounds__(512, 2) void kv_attention_prefix_kernel(SharedArgs s) {
+    __shared__ WideLds<HD> lds;
+    __shared__ int64_t wave_tiles[8], wave_units[8], found_at, found_units;
+    __shared__ int found;
+    const AttnArgs& a = s.a;
+    const int tid = threadIdx.x, lane = tid & 63, heads = a.cache.kv_heads;
+    // Tiles and units ahead of each thread's share of the groups.
+    const int per = (s.n_groups + 511) / 512, g0 = min(tid * per, s.n_groups);
+    const int g1 = min(g0 + per, s.n_groups);
+    int64_t tiles = 0, units = 0;
+    for (int x = g0; x < g1; ++x) {
+        const Wide d = wide_of(s, x);
+        units += (int64_t)d.blocks * heads;
+        tiles += (int64_t)d.blocks * heads * d.tiles;
+    }
+    int64_t t_sum = tiles, u_sum = units;
+    for (int x = 1; x < 64; x <<= 1) {
+        const int64_t t = __shfl_up(t_sum, x), u = __shfl_up(u_sum, x);
+        if (lane >= x) t_sum += t, u_sum += u;
+    }
+    if (lane == 63) wave_tiles[tid >> 6] = t_sum, wave_units[tid >> 6] = u_sum;
+    __syncthreads();
+    int64_t all = 0, t_at = t_sum - tiles, all_units = 0, u_at = u_sum - units;
+    for (int w = 0; w < 8; ++w) {
+        if (w < (tid >> 6)) t_at += wave_tiles[w], u_at += wave_units[w];
+        all += wave_tiles[w], all_units += wave_units[w];
+    }
+    all = uniform(all);
+    const int64_t groups = min((int64_t)gridDim.x, all);
+    const int me = all >= gridDim.x ? xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
+    if (blockIdx.x == 0) {
+        if (tid == 0) s.counts[2] = (int)min(all_units, (int64_t)s.wide_units);
+        int64_t u = u_at;
+        for (int x = g0; x < g1; ++x) {
+            s.wide_base[x] = (int)min(u, (int64_t)s.wide_units);
+            u += (int64_t)wide_of(s, x).blocks * heads;
+        }
+    }
+    if (me >= groups) return;
+    int64_t at = all * me / groups;
+    const int64_t end = all * (me + 1) / groups;
+    if (at >= t_at && at < t_at + tiles) {
+        int x = g0;
+        for (; x < g1 - 1; ++x) {
+            const Wide d = wide_of(s, x);
+            const int64_t n = (int64_t)d.blocks * heads * d.tiles;
+            if (at < t_at + n) break;
+            t_at += n, u_at += (int64_t)d.blocks * heads;
+        }
+        found = x, found_at = t_at, found_units = u_at;
+    }
+    __syncthreads();
+    int seg = uniform(found);
+    int64_t start = uniform(found_at), u0 = uniform(found_units);  // of the group
+    while (at < end) {
+        const Wide d = wide_of(s, seg);
+        const int64_t n = (int64_t)d.blocks * heads * d.tiles;
+        if (at >= start + n) {
+            start += n, u0 += (int64_t)d.blocks * heads, ++seg;
+            continue;
+        }
+        const int u = (int)((at - start) / d.tiles);
+        const int first = (int)((at - start) - (int64_t)u * d.tiles);
+        const int count = (int)min((int64_t)(d.tiles - first), end - at);
+        const bool room = u0 + u < s.wide_units;
+        int64_t part = s.whole_wide + (u0 + u) * s.wide_pairs;
+        if (first > 0) part = s.wide_cut + 2 * (int64_t)me * s.wide_pairs;
+        else if (count < d.tiles) part = s.wide_cut + (2 * (int64_t)me + 1) * s.wide_pairs;
+        if (first == 0 && tid == 0 && room) {
+            // The workgroup that has the unit's last tile ends it.
+            const int64_t last = ((at + d.tiles) * groups - 1) / all;
+            s.wide_joins[u0 + u] = int4{me, (int)(last - me) + 1, seg, u};
+        }
+        const int h = u / d.blocks;
+        if (room)
+            run_wide<HD, CODES, NP>(s, d, h, u - h * d.blocks, first, count, part, lds);
         at += count;
     }
 }
@@ -220,7 +668,11 @@ __global__ __launch_bounds__(256) void kv_attention_shared_join_kernel(SharedArg
     const int pairs = min(16 * RO, d.q.n * a.group - block * 16 * RO);
     const int g = d.floor > 0 ? group_with(s, r) : 0;
     Need p = {};
-    if (d.floor > 0) p = group_need<RP>(s, g);
+    Wide w = {};
+    if (d.floor > 0) {
+        p = group_need<RP>(s, g);
+        if (s.plans) w = wide_of(s, g);
+    }
     constexpr int L = HD / 4;  // lanes of a part
     const bool few = j.y <= 16;
     const int span = few ? 64 : 256, mine = threadIdx.x % span;
@@ -242,17 +694,28 @@ __global__ __launch_bounds__(256) void kv_attention_shared_join_kernel(SharedArg
             o = o * f + v * e;
             m = top;
         };
-        auto parts = [&](int4 u, int64_t whole, int64_t at) {
-            for (int k = k0; k < u.y; k += step)
-                take((u.y == 1 ? whole : (int64_t)(k == 0 ? 2 * u.x + 1 : 2 * (u.x + k)) * 16 * RP) + at);
-        };
         if (pr < pairs) {
-            parts(j, s.whole_own + (int64_t)blockIdx.x * 16 * RO, pr);
-            if (d.floor > 0) {
+            const int64_t whole = s.whole_own + (int64_t)blockIdx.x * 16 * RO;
+            for (int k = k0; k < j.y; k += step)
+                take((j.y == 1 ? whole : (int64_t)(k == 0 ? 2 * j.x + 1 : 2 * (j.x + k)) * 16 * RP) + pr);
+            auto group_parts = [&](int64_t its, int64_t unit, int units, int unit_pairs, const int4* joins,
+                                   int64_t cut, int64_t whole) {
+                if (its < 0 || unit >= units) return;
+                const int4 u = joins[unit];
+                for (int k = k0; k < u.y; k += step) {
+                    const int64_t slot = k == 0 ? 2 * (int64_t)u.x + 1 : 2 * ((int64_t)u.x + k);
+                    take((u.y == 1 ? whole + unit * unit_pairs : cut + slot * unit_pairs) + its % unit_pairs);
+                }
+            };
+            if (p.blocks > 0) {
                 const int64_t its = (int64_t)(d.q.o0 - p.q.o0) * a.group + pair;
-                const int64_t unit = s.unit_base[g] + (int64_t)h * p.blocks + its / (16 * RP);
-                if (its >= 0 && unit < s.counts[0])
-                    parts(s.joins[unit], s.whole_prefix + unit * 16 * RP, its % (16 * RP));
+                group_parts(its, s.unit_base[g] + (int64_t)h * p.blocks + its / (16 * RP), s.counts[0],
+                            16 * RP, s.joins, 0, s.whole_prefix);
+            }
+            if (w.blocks > 0) {
+                const int64_t its = (int64_t)(d.q.o0 - w.o0) * a.group + pair;
+                group_parts(its, s.wide_base[g] + (int64_t)h * w.blocks + its / s.wide_pairs, s.counts[2],
+                            s.wide_pairs, s.wide_joins, s.wide_cut, s.whole_wide);
             }
         }
         so[threadIdx.x] = o, sm[threadIdx.x] = m, sl[threadIdx.x] = l;
@@ -279,38 +742,53 @@ __global__ __launch_bounds__(256) void kv_attention_shared_join_kernel(SharedArg
 // How a step is laid out: by its sizes alone, so that the workspace's size and
 // the launch agree.
 struct SharedLayout {
-    int rp, ro;                     // RP and RO
-    int64_t prefix_units, own_units;  // at most
-    int64_t runs;                   // workgroups
-    int64_t some;                   // requests that may have rows
-    int64_t whole_prefix, whole_own;  // rows of parts
-    size_t base, joins, ml, o, bytes;  // offsets in the workspace
+    int rp, ro;                       // RP and RO
+    int wide;                         // NP of the groups' own kernel, or 0
+    int64_t prefix_units, own_units, wide_units;  // at most
+    int64_t runs, wide_runs;          // workgroups
+    int64_t some;                     // requests that may have rows
+    int64_t whole_prefix, whole_own, wide_cut, whole_wide;  // rows of parts
+    size_t plans, base, wide_base, joins, ml, o, bytes;     // offsets in the workspace
 };
 
 SharedLayout shared_layout(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int64_t n_groups,
-                           int q_heads) {
+                           int q_heads, bool window) {
     SharedLayout s;
     const int64_t group = q_heads / c.kv_heads, pairs = b.rows * group;
     s.some = std::max<int64_t>(1, std::min(b.requests, b.rows));
     s.ro = pairs <= 16 * s.some ? 1 : 2;
-    s.rp = pairs <= 16 * std::max<int64_t>(1, std::min(n_groups, s.some)) ? 1 : 2;
+    const int64_t per_group = pairs / std::max<int64_t>(1, std::min(n_groups, s.some));
+    s.rp = std::max(s.ro, per_group <= 16 ? 1 : 2);
+    s.wide = n_groups == 0 || window || per_group < kWidePairs ? 0 : per_group <= 64 ? 2 : per_group <= 128 ? 4 : 8;
     s.own_units = (pairs / (16 * s.ro) + s.some) * c.kv_heads;
     s.prefix_units = n_groups ? (pairs / (16 * s.rp) + n_groups) * c.kv_heads : 0;
-    const int64_t tiles = std::max<int64_t>(1, (b.table_width * c.page_size + kTile - 1) / kTile);
+    s.wide_units = s.wide ? (pairs / (32 * s.wide) + n_groups) * c.kv_heads : 0;
+    const int64_t tokens = std::max<int64_t>(1, b.table_width * c.page_size);
+    const int64_t tiles = (tokens + kTile - 1) / kTile;
     s.runs = std::min<int64_t>((s.own_units + s.prefix_units) * tiles, 2 * kCus);
+    s.wide_runs = std::min<int64_t>(s.wide_units * ((tokens + kWideTile - 1) / kWideTile), kCus);
     s.whole_prefix = 2 * s.runs * 16 * s.rp;
     s.whole_own = s.whole_prefix + s.prefix_units * 16 * s.rp;
-    const size_t rows = (size_t)(s.whole_own + s.own_units * 16 * s.ro);
-    s.base = 16;
-    s.joins = s.base + ((size_t)n_groups * 4 + 15) / 16 * 16;
-    s.ml = s.joins + 16 * (size_t)(s.prefix_units + s.own_units);
-    s.o = s.ml + (rows * 8 + 15) / 16 * 16;
+    s.wide_cut = s.whole_own + s.own_units * 16 * s.ro;
+    s.whole_wide = s.wide_cut + 2 * s.wide_runs * 32 * s.wide;
+    const size_t rows = (size_t)(s.whole_wide + s.wide_units * 32 * s.wide);
+    auto up = [](size_t bytes) { return (bytes + 15) / 16 * 16; };
+    s.plans = 16;
+    s.base = s.plans + (s.wide ? 16 * (size_t)n_groups : 0);
+    s.wide_base = s.base + up(4 * (size_t)n_groups);
+    s.joins = s.wide_base + up(4 * (size_t)n_groups);
+    s.ml = s.joins + 16 * (size_t)(s.prefix_units + s.own_units + s.wide_units);
+    s.o = s.ml + up(rows * 8);
     s.bytes = s.o + rows * c.head_dim * 4;
     return s;
 }
 
 template <int HD, int CODES, int RP, int RO>
 hipError_t launch_shared(const SharedArgs& a, const SharedLayout& s, hipStream_t st) {
+    if (s.wide) kv_attention_plan_kernel<<<(uint32_t)((a.n_groups + 3) / 4), 256, 0, st>>>(a);
+    if (s.wide == 2) kv_attention_prefix_kernel<HD, CODES, 2><<<(uint32_t)s.wide_runs, 512, 0, st>>>(a);
+    if (s.wide == 4) kv_attention_prefix_kernel<HD, CODES, 4><<<(uint32_t)s.wide_runs, 512, 0, st>>>(a);
+    if (s.wide == 8) kv_attention_prefix_kernel<HD, CODES, 8><<<(uint32_t)s.wide_runs, 512, 0, st>>>(a);
     kv_attention_shared_kernel<HD, CODES, RP, RO><<<(uint32_t)s.runs, 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -339,8 +817,10 @@ int check_shared(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch, int64
         batch->rows * q_heads > 0x7FFFFFFF || n_groups < 0 || n_groups > batch->requests)
         return NCM_E_SHAPE;
     // The join's launch has a workgroup per unit.
-    const SharedLayout s = shared_layout(*cache, *batch, n_groups, q_heads);
-    if (s.own_units + s.prefix_units > kMaxBlocks) return NCM_E_SHAPE;
+    for (bool window : {false, true}) {
+        const SharedLayout s = shared_layout(*cache, *batch, n_groups, q_heads, window);
+        if (s.own_units + s.prefix_units + s.wide_units > kMaxBlocks) return NCM_E_SHAPE;
+    }
     a->q_heads = q_heads;
     a->group = q_heads / cache->kv_heads;
     return NCM_OK;
@@ -358,8 +838,9 @@ extern "C" int ncm_kv_attention_shared_workspace(const ncm_kv_cache_t* cache,
     AttnArgs a = {};
     const int rc = check_shared(cache, batch, n_groups, q_heads, &a);
     if (rc) return rc;
-    if (batch->rows > 0 && batch->requests > 0)
-        *bytes = shared_layout(*cache, *batch, n_groups, q_heads).bytes;
+    if (batch->rows > 0 && batch->requests > 0)  // with a window or without
+        *bytes = std::max(shared_layout(*cache, *batch, n_groups, q_heads, false).bytes,
+                          shared_layout(*cache, *batch, n_groups, q_heads, true).bytes);
     return NCM_OK;
 }
 
@@ -384,7 +865,7 @@ extern "C" int ncm_kv_attention_shared_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t*
     rc = check_rows(q, q_stride, width);
     if (!rc) rc = check_rows(out, out_stride, width);
     if (rc) return rc;
-    const SharedLayout l = shared_layout(*cache, *batch, n_groups, q_heads);
+    const SharedLayout l = shared_layout(*cache, *batch, n_groups, q_heads, window > 0);
     // Offsets may give every request, and groups every group, all rows: the
     // tiles must still be counted in 64 bits, times the workgroups.
     const double most = ((double)batch->rows * q_heads / 16 + cache->kv_heads) *
@@ -402,9 +883,14 @@ extern "C" int ncm_kv_attention_shared_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t*
     s.groups = groups, s.shared = shared, s.n_groups = (int)n_groups;
     s.prefix_units = (int)l.prefix_units, s.own_units = (int)l.own_units;
     s.counts = (int*)ws;
+    if (l.wide) s.plans = (int4*)(ws + l.plans);
     s.unit_base = (int*)(ws + l.base);
+    s.wide_base = (int*)(ws + l.wide_base);
     s.joins = (int4*)(ws + l.joins);
+    s.wide_joins = s.joins + l.prefix_units + l.own_units;
     s.whole_prefix = l.whole_prefix, s.whole_own = l.whole_own;
+    s.wide_cut = l.wide_cut, s.whole_wide = l.whole_wide;
+    s.wide_units = (int)l.wide_units, s.wide_pairs = 32 * l.wide;
     const DeviceScope scope(ncm_ctx_device(ctx));
     rc = step_hip(scope.error(), "kv_attention_shared device");
     if (rc) return rc;
