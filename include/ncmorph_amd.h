@@ -230,11 +230,14 @@ int ncm_int4_quantise_dev(ncm_ctx_t* ctx, const uint16_t* w, int64_t n, int64_t 
  * bias: bf16 [n] or NULL; residual: float [m, n] or NULL, which y may be for the
  * float modes; y: float [m, n] (out_mode F32, BF16_F32) or bf16 bits (BF16). m up
  * to 2^20: made for the rows of a decode step; from some hundred rows on
- * ncm_linear_bf16 of the widened weights takes less time. Uses no workspace.
- * Device pointers. */
+ * ncm_linear_bf16 of the widened weights takes less time. workspace: at least
+ * the bytes that ncm_linear_int4_workspace gives (0: NULL will do), 16-byte
+ * aligned; the call leaves nothing there that a later one needs, and no two calls
+ * that may run at once can share it. Device pointers. */
+int ncm_linear_int4_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
 int ncm_linear_int4(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride,
                     const ncm_int4_weight_t* w, const uint16_t* bias, const float* residual,
-                    void* y, int64_t m, int out_mode);
+                    void* y, int64_t m, int out_mode, void* workspace, size_t workspace_bytes);
 
 /* The q|k|v projection and the RoPE rotation of its q and k heads
  * (root.zig:497-530) in one pass, for head_dim 64: y = the bf16 output of

@@ -53,7 +53,8 @@ SIGNATURES = [
     ("ncm_int4_bytes", i32, [i64, i64, i32, i32, C.POINTER(sz), C.POINTER(sz)]),
     ("ncm_int4_pack_dev", i32, [vp, vp, vp, vp, i64, i64, i32, vp, vp]),
     ("ncm_int4_quantise_dev", i32, [vp, vp, i64, i64, i64, i32, vp, vp, vp]),
-    ("ncm_linear_int4", i32, [vp, vp, i64, vp, vp, vp, vp, i64, i32]),
+    ("ncm_linear_int4_workspace", i32, [i64, i64, i64, C.POINTER(sz)]),
+    ("ncm_linear_int4", i32, [vp, vp, i64, vp, vp, vp, vp, i64, i32, vp, sz]),
     ("ncm_linear_bf16_rope64", i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, vp]),
     ("ncm_linear_f32", i32, [vp, vp, vp, vp, i64, i64, i64]),
     ("ncm_bf16_from_f32_dev", i32, [vp, vp, vp, i64, i32]),

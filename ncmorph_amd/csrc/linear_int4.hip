@@ -32,6 +32,8 @@ struct Int4Args {
     int64_t x_stride;
     int m, n, k, blocks;  // of 128 inputs
     bool wide;            // 4 outputs of a row in one access
+    float* parts;         // [splits][m][n] where the inputs are split, else NULL
+    int splits;
 };
 
 // Scales of 16 outputs, a block of 128 inputs: [128 / GROUP][16], two bytes, or
@@ -44,14 +46,56 @@ struct Stage {
     static constexpr int G = 128 / GROUP;
     u32x4_t w[NT];
     u32x4_t x[MT][4];
-    uint32_t s[NT][G][ZEROS ? 4 : 2];
+    uint32_t s[NT];  // a dword of the tile's scales, by lane
 };
 
-template <int GROUP, bool ZEROS, int NT, int MT, int OUT>
+// Four outputs of a row, from column `col` on.
+template <int OUT>
+__device__ __forceinline__ void store_block(const Int4Args& a, f32x4_t v, int row, int64_t col) {
+    if (row >= a.m) return;
+    int64_t at = (int64_t)row * a.n + col;
+    const int left = (int)min((int64_t)4, a.n - col);
+    if (left <= 0) return;
+    if (a.wide) {
+        if (a.bias) {
+            const u32x2_t bits = *(const u32x2_t*)(a.bias + col);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] += __uint_as_float(j % 2 ? bits[j / 2] & 0xFFFF0000u : bits[j / 2] << 16);
+        }
+        if (a.residual) v += *(const f32x4_t*)(a.residual + at);
+        if constexpr (OUT == NCM_OUT_BF16) {
+            *(u32x2_t*)((uint16_t*)a.y + at) =
+                u32x2_t{bf16x2_bits_rne(v[0], v[1]), bf16x2_bits_rne(v[2], v[3])};
+        } else {
+            if constexpr (OUT == NCM_OUT_BF16_F32)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(bf16_bits_rne(v[j]) << 16);
+            *(f32x4_t*)((float*)a.y + at) = v;
+        }
+    } else {
+        for (int j = 0; j < left; ++j) {
+            float f = v[j];
+            if (a.bias) f += __uint_as_float((uint32_t)a.bias[col + j] << 16);
+            if (a.residual) f += a.residual[at + j];
+            if constexpr (OUT == NCM_OUT_BF16) ((uint16_t*)a.y)[at + j] = (uint16_t)bf16_bits_rne(f);
+            else ((float*)a.y)[at + j] =
+                OUT == NCM_OUT_F32 ? f : __uint_as_float(bf16_bits_rne(f) << 16);
+        }
+    }
+}
+
+// DEPTH: blocks of 128 inputs that a wavefront loads ahead.
+template <int GROUP, bool ZEROS, int NT, int MT, int DEPTH, int OUT>
 __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
     typedef Stage<GROUP, ZEROS, NT, MT> S;
     constexpr int G = S::G, STEPS = 4 / G;  // MFMA steps of a group
+    constexpr int SB = scale_bytes<GROUP, ZEROS>() / 4;
     __shared__ f32x4_t parts[kWaves][NT * MT][64];
+    // Each wavefront's scales on their way from one coalesced load to the lanes
+    // that need them (loaded by those lanes: 36 us in place of XX for 28672 x 4096
+    // in groups of 32 with zero points).
+    __shared__ __attribute__((aligned(16))) uint32_t scales[kWaves][NT][SB];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int64_t tile0 = (int64_t)blockIdx.x * NT;
@@ -62,12 +106,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
         for (int t = 0; t < NT; ++t) {
             const int64_t at = min(tile0 + t, (int64_t)tiles - 1) * a.blocks + b;
             s.w[t] = a.codes[at * 64 + lane];
-            const char* p = a.scales + at * scale_bytes<GROUP, ZEROS>() + g * (ZEROS ? 16 : 8);
-#pragma unroll
-            for (int i = 0; i < G; ++i)
-#pragma unroll
-                for (int j = 0; j < (ZEROS ? 4 : 2); ++j)
-                    s.s[t][i][j] = ((const uint32_t*)(p + i * (ZEROS ? 64 : 32)))[j];
+            s.s[t] = ((const uint32_t*)a.scales)[at * SB + min(lane, SB - 1)];
         }
 #pragma unroll
         for (int r = 0; r < MT; ++r) {
@@ -89,6 +128,9 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
     const u32x4_t one_bits = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
     const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, one_bits);
     auto add = [&](const S& s) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (lane < SB) scales[wave][t][lane] = s.s[t];
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             f32x4_t of_x[MT], of_q[NT][MT];
@@ -117,28 +159,37 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
                 }
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t* words = &scales[wave][t][i * (ZEROS ? 16 : 8) + g * (ZEROS ? 4 : 2)];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t word = s.s[t][i][ZEROS ? j : j / 2];
+                    const uint32_t word = words[ZEROS ? j : j / 2];
                     const float scale = __uint_as_float(!ZEROS && j % 2 == 0 ? word << 16 : word & 0xFFFF0000u);
                     const float zero = ZEROS ? __uint_as_float(word << 16) : 136.0f;
 #pragma unroll
                     for (int r = 0; r < MT; ++r)
                         sum[t][r][j] = fmaf(scale, fmaf(-zero, of_x[r][j], of_q[t][r][j]), sum[t][r][j]);
                 }
+            }
         }
+        asm volatile("" ::: "memory");  // the next block's scales stay behind these reads
     };
 
-    S now, next;
-    int b = wave;
-    if (b < a.blocks) load(now, b);
-    while (b < a.blocks) {
-        const int after = b + kWaves;
-        if (after < a.blocks) load(next, after);
-        add(now);
-        now = next;
-        b = after;
+    S now[DEPTH], next[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+        if (wave + i * kWaves < a.blocks) load(now[i], wave + i * kWaves);
+    for (int b = wave; b < a.blocks; b += DEPTH * kWaves) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+            const int after = b + (DEPTH + i) * kWaves;
+            if (after < a.blocks) load(next[i], after);
+        }
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i)
+            if (b + i * kWaves < a.blocks) add(now[i]);
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) now[i] = next[i];
     }
 
 #pragma unroll
@@ -154,40 +205,192 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = v[j] + p[j];
         }
-        const int row = m0 + 16 * (i % MT) + c;
-        const int64_t col = (tile0 + i / MT) * 16 + 4 * g;
-        if (row >= a.m) continue;
-        const int64_t at = (int64_t)row * a.n + col;
-        const int left = (int)min((int64_t)4, a.n - col);
-        if (left <= 0) continue;
-        if (a.wide) {
-            if (a.bias) {
-                const u32x2_t bits = *(const u32x2_t*)(a.bias + col);
+        store_block<OUT>(a, v, m0 + 16 * (i % MT) + c, (tile0 + i / MT) * 16 + 4 * g);
+    }
+}
+
+// More rows: the rows of x are shared by NW wavefronts of 32 outputs each, in LDS,
+// and 8 / NW sets of these take every 8 / NW-th 128 inputs. Weights go from memory
+// to registers a block ahead; scales through LDS, which gives each lane its four
+// outputs' without 64 registers for them. 16-byte chunk c of row r of x is at
+// chunk c ^ (r % 16), so that an operand's sixteen rows fall into different banks.
+template <int GROUP, bool ZEROS, int NW, int MT, int OUT>
+__global__ __launch_bounds__(512, 2) void linear_int4_rows_kernel(Int4Args a) {
+    constexpr int KW = 8 / NW, G = 128 / GROUP, STEPS = 4 / G, NT = 2, ROWS = 16 * MT;
+    constexpr int SB = scale_bytes<GROUP, ZEROS>() / 4;  // dwords of a tile's block
+    constexpr int PER = KW * ROWS * 16 / 512;            // chunks of x a thread brings
+    __shared__ u32x4_t xs[2][KW][ROWS][16];
+    __shared__ __attribute__((aligned(16))) uint32_t scales[2][8][NT * SB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4, nw = wave % NW, kw = wave / NW;
+    const int64_t tile0 = ((int64_t)blockIdx.x * NW + nw) * NT;
+    const int tiles = (a.n + 15) / 16, m0 = blockIdx.y * ROWS;
+    // The workgroup's steps of KW blocks.
+    const int all = (a.blocks + KW - 1) / KW;
+    const int step0 = (int)((int64_t)all * blockIdx.z / a.splits);
+    const int steps = (int)((int64_t)all * (blockIdx.z + 1) / a.splits) - step0;
+
+    u32x4_t w[NT], x[PER];
+    uint32_t s[(NT * SB + 63) / 64];
+    auto load_w = [&](int step) {
+        const int b = min((step0 + step) * KW + kw, a.blocks - 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    v[j] += __uint_as_float(j % 2 ? bits[j / 2] & 0xFFFF0000u : bits[j / 2] << 16);
-            }
-            if (a.residual) v += *(const f32x4_t*)(a.residual + at);
-            if constexpr (OUT == NCM_OUT_BF16) {
-                *(u32x2_t*)((uint16_t*)a.y + at) =
-                    u32x2_t{bf16x2_bits_rne(v[0], v[1]), bf16x2_bits_rne(v[2], v[3])};
-            } else {
-                if constexpr (OUT == NCM_OUT_BF16_F32)
+        for (int t = 0; t < NT; ++t) {
+            const int64_t at = min(tile0 + t, (int64_t)tiles - 1) * a.blocks + b;
+            w[t] = a.codes[at * 64 + lane];
+        }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(bf16_bits_rne(v[j]) << 16);
-                *(f32x4_t*)((float*)a.y + at) = v;
-            }
-        } else {
-            for (int j = 0; j < left; ++j) {
-                float f = v[j];
-                if (a.bias) f += __uint_as_float((uint32_t)a.bias[col + j] << 16);
-                if (a.residual) f += a.residual[at + j];
-                if constexpr (OUT == NCM_OUT_BF16) ((uint16_t*)a.y)[at + j] = (uint16_t)bf16_bits_rne(f);
-                else ((float*)a.y)[at + j] =
-                    OUT == NCM_OUT_F32 ? f : __uint_as_float(bf16_bits_rne(f) << 16);
+        for (int i = 0; i < (NT * SB + 63) / 64; ++i) {
+            const int d = min(i * 64 + lane, NT * SB - 1);
+            const int64_t at = min(tile0 + d / SB, (int64_t)tiles - 1) * a.blocks + b;
+            s[i] = ((const uint32_t*)a.scales)[at * SB + d % SB];
+        }
+    };
+    auto load_x = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int chunk = tid + 512 * i, row = chunk / 16 % ROWS, set = chunk / (16 * ROWS);
+            const int64_t k = 128 * ((int64_t)(step0 + step) * KW + set) + 8 * (chunk % 16);
+            x[i] = u32x4_t{0, 0, 0, 0};
+            if (m0 + row < a.m && k < a.k) x[i] = *(const u32x4_t*)(a.x + (m0 + row) * a.x_stride + k);
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int chunk = tid + 512 * i, row = chunk / 16 % ROWS, set = chunk / (16 * ROWS);
+            xs[buffer][set][row][(chunk ^ row) & 15] = x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < (NT * SB + 63) / 64; ++i)
+            if (i * 64 + lane < NT * SB) scales[buffer][wave][i * 64 + lane] = s[i];
+    };
+
+    f32x4_t sum[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < MT; ++r) sum[t][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const u32x4_t one_bits = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, one_bits);
+
+    load_w(0);
+    load_x(0);
+    put(0);
+    u32x4_t now[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) now[t] = w[t];
+    if (steps > 1) load_w(1), load_x(1);
+    lds_barrier();
+    for (int step = 0; step < steps; ++step) {
+        const int b = step & 1;
+        if ((step0 + step) * KW + kw < a.blocks) {
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                f32x4_t of_x[MT], of_q[NT][MT];
+#pragma unroll
+                for (int r = 0; r < MT; ++r) {
+                    of_x[r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) of_q[t][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+#pragma unroll
+                for (int e = STEPS * i; e < STEPS * (i + 1); ++e) {
+                    bf16x8_t q[NT];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        u32x4_t bits;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) bits[j] = ((now[t][e] >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+                        q[t] = __builtin_bit_cast(bf16x8_t, bits);
+                    }
+#pragma unroll
+                    for (int r = 0; r < MT; ++r) {
+                        const bf16x8_t rows =
+                            __builtin_bit_cast(bf16x8_t, xs[b][kw][16 * r + c][(4 * e + g) ^ c]);
+                        of_x[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, rows, of_x[r], 0, 0, 0);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            of_q[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q[t], rows, of_q[t][r], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const uint32_t* p = &scales[b][wave][t * SB + i * (ZEROS ? 16 : 8) + g * (ZEROS ? 4 : 2)];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t word = p[ZEROS ? j : j / 2];
+                        const float scale =
+                            __uint_as_float(!ZEROS && j % 2 == 0 ? word << 16 : word & 0xFFFF0000u);
+                        const float zero = ZEROS ? __uint_as_float(word << 16) : 136.0f;
+#pragma unroll
+                        for (int r = 0; r < MT; ++r)
+                            sum[t][r][j] = fmaf(scale, fmaf(-zero, of_x[r][j], of_q[t][r][j]), sum[t][r][j]);
+                    }
+                }
             }
         }
+        if (step + 1 < steps) {
+            put(b ^ 1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) now[t] = w[t];
+            if (step + 2 < steps) load_w(step + 2), load_x(step + 2);
+        }
+        lds_barrier();
     }
+    // The sets' sums, added in order.
+    f32x4_t* parts = (f32x4_t*)xs;
+    static_assert(sizeof(xs) >= (KW - 1) * NW * NT * MT * 1024, "the other sets' sums");
+    if (kw > 0)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < MT; ++r)
+                parts[((((kw - 1) * NW + nw) * NT + t) * MT + r) * 64 + lane] = sum[t][r];
+    __syncthreads();
+    if (kw == 0)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < MT; ++r) {
+                f32x4_t v = sum[t][r];
+#pragma unroll
+                for (int other = 0; other < KW - 1; ++other) {
+                    const f32x4_t p = parts[(((other * NW + nw) * NT + t) * MT + r) * 64 + lane];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = v[j] + p[j];
+                }
+                const int row = m0 + 16 * r + c;
+                const int64_t col = (tile0 + t) * 16 + 4 * g;
+                if (!a.parts) store_block<OUT>(a, v, row, col);
+                else if (row < a.m) {
+                    float* p = a.parts + ((int64_t)blockIdx.z * a.m + row) * a.n + col;
+                    if (a.n % 4 == 0 && col < a.n) *(f32x4_t*)p = v;
+                    else
+                        for (int j = 0; j < min((int64_t)4, a.n - col); ++j) p[j] = v[j];
+                }
+            }
+}
+
+// The splits' sums, added in order.
+template <int OUT>
+__global__ __launch_bounds__(256) void linear_int4_join_kernel(Int4Args a) {
+    const int64_t quads = (a.n + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads * a.m) return;
+    const int row = (int)(i / quads);
+    const int64_t col = (i - row * quads) * 4, at = (int64_t)row * a.n + col;
+    f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = a.parts + (int64_t)s * a.m * a.n + at;
+        if (a.n % 4 == 0) {
+            const f32x4_t x = *(const f32x4_t*)p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = v[j] + x[j];
+        } else {
+            for (int j = 0; j < min((int64_t)4, a.n - col); ++j) v[j] = v[j] + p[j];
+        }
+    }
+    store_block<OUT>(a, v, row, col);
 }
 
 // Codes, a byte each, into the products' order; outputs past n and inputs past
@@ -270,27 +473,54 @@ int check_int4(int64_t n, int64_t k, int group) {
     return (n + 15) / 16 * ((k + 127) / 128) > kMaxBlocks ? NCM_E_SHAPE : NCM_OK;
 }
 
-template <int GROUP, bool ZEROS, int NT, int MT>
-void launch_out(const Int4Args& a, int out, dim3 grid, hipStream_t st) {
-    if (out == NCM_OUT_F32) linear_int4_kernel<GROUP, ZEROS, NT, MT, NCM_OUT_F32><<<grid, 64 * kWaves, 0, st>>>(a);
-    else if (out == NCM_OUT_BF16) linear_int4_kernel<GROUP, ZEROS, NT, MT, NCM_OUT_BF16><<<grid, 64 * kWaves, 0, st>>>(a);
-    else linear_int4_kernel<GROUP, ZEROS, NT, MT, NCM_OUT_BF16_F32><<<grid, 64 * kWaves, 0, st>>>(a);
+template <typename F>
+void with_out(int out, F f) {
+    if (out == NCM_OUT_F32) f(std::integral_constant<int, NCM_OUT_F32>());
+    else if (out == NCM_OUT_BF16) f(std::integral_constant<int, NCM_OUT_BF16>());
+    else f(std::integral_constant<int, NCM_OUT_BF16_F32>());
+}
+
+// How a product is laid out, by its sizes.
+struct Int4Layout {
+    int rows;      // of a workgroup, 0: the kernel of few rows
+    int splits;    // of the inputs
+    size_t bytes;  // of the workspace
+};
+constexpr int kFewRows = 16;
+
+Int4Layout int4_layout(int64_t m, int64_t n, int64_t k) {
+    Int4Layout l = {0, 1, 0};
+    if (m <= kFewRows) return l;
+    l.rows = m <= 32 ? 32 : 64;
+    // Workgroups of 128 outputs. Fewer than the CUs: the inputs are split, at most
+    // to two steps of 256 each (every output tile reads all of x, so narrower
+    // tiles would only move the load to that).
+    const int64_t groups = (n + 127) / 128 * ((m + l.rows - 1) / l.rows);
+    const int64_t steps = (k + 255) / 256;
+    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(groups, 1), steps / 2, 16}));
+    if (l.splits > 1) l.bytes = (size_t)l.splits * m * n * 4;
+    return l;
 }
 
 template <int GROUP, bool ZEROS>
-void launch(const Int4Args& a, int out, hipStream_t st) {
+void launch(const Int4Args& a, const Int4Layout& l, int out, hipStream_t st) {
     const int64_t tiles = (a.n + 15) / 16;
-    auto go = [&](auto nt, auto mt) {
-        constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value;
-        launch_out<GROUP, ZEROS, NT, MT>(
-            a, out, dim3((uint32_t)((tiles + NT - 1) / NT), (uint32_t)((a.m + 16 * MT - 1) / (16 * MT))), st);
-    };
-    const std::integral_constant<int, 1> one;
-    const std::integral_constant<int, 2> two;
-    const std::integral_constant<int, 4> four;
-    if (a.m <= 16) go(one, one);
-    else if (a.m <= 32) go(two, two);
-    else go(two, four);
+    with_out(out, [&](auto mode) {
+        constexpr int OUT = decltype(mode)::value;
+        if (l.rows == 0) {
+            // Two blocks ahead where there are few wavefronts to wait on each other.
+            if (tiles < 512) linear_int4_kernel<GROUP, ZEROS, 1, 1, 2, OUT><<<(uint32_t)tiles, 64 * kWaves, 0, st>>>(a);
+            else linear_int4_kernel<GROUP, ZEROS, 1, 1, 1, OUT><<<(uint32_t)tiles, 64 * kWaves, 0, st>>>(a);
+            return;
+        }
+        const dim3 grid((uint32_t)((tiles + 7) / 8), (uint32_t)((a.m + l.rows - 1) / l.rows), (uint32_t)l.splits);
+        if (l.rows == 32) linear_int4_rows_kernel<GROUP, ZEROS, 4, 2, OUT><<<grid, 512, 0, st>>>(a);
+        else linear_int4_rows_kernel<GROUP, ZEROS, 4, 4, OUT><<<grid, 512, 0, st>>>(a);
+        if (l.splits > 1) {
+            const int64_t quads = ((int64_t)a.n + 3) / 4 * a.m;
+            linear_int4_join_kernel<OUT><<<(uint32_t)((quads + 255) / 256), 256, 0, st>>>(a);
+        }
+    });
 }
 
 }  // namespace
@@ -347,9 +577,21 @@ extern "C" int ncm_int4_pack_dev(ncm_ctx_t* ctx, const uint8_t* codes, const uin
     return step_hip(hipGetLastError(), "int4_pack launch");
 }
 
+extern "C" int ncm_linear_int4_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes) {
+    using namespace ncm;
+    if (!bytes) return NCM_E_NULL;
+    *bytes = 0;
+    const int rc = check_int4(n, k, 32);
+    if (rc) return rc;
+    if (m < 0 || m > (1 << 20)) return NCM_E_SHAPE;
+    *bytes = int4_layout(m, n, k).bytes;
+    return NCM_OK;
+}
+
 extern "C" int ncm_linear_int4(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stride,
                                const ncm_int4_weight_t* w, const uint16_t* bias,
-                               const float* residual, void* y, int64_t m, int out_mode) {
+                               const float* residual, void* y, int64_t m, int out_mode,
+                               void* workspace, size_t workspace_bytes) {
     using namespace ncm;
     if (!ctx || !w) return NCM_E_NULL;
     int rc = check_int4(w->n, w->k, w->group);
@@ -366,17 +608,22 @@ extern "C" int ncm_linear_int4(ncm_ctx_t* ctx, const uint16_t* x, int64_t x_stri
         (uintptr_t)bias % 2 || (uintptr_t)residual % 4)
         return NCM_E_ARG;
     if (residual == y && size == 2) return NCM_E_ARG;
+    const Int4Layout l = int4_layout(m, w->n, w->k);
+    if (l.bytes && !workspace) return NCM_E_NULL;
+    if (workspace_bytes < l.bytes) return NCM_E_LENGTH;
+    if (l.bytes && (uintptr_t)workspace % 16) return NCM_E_ARG;
     const bool wide = w->n % 4 == 0 && (uintptr_t)y % (4 * size) == 0 && (uintptr_t)bias % 8 == 0 &&
                       (uintptr_t)residual % 16 == 0;
     const Int4Args a = {x, (const u32x4_t*)w->codes, (const char*)w->scales, bias, residual, y,
-                        x_stride, (int)m, (int)w->n, (int)w->k, (int)((w->k + 127) / 128), wide};
+                        x_stride, (int)m, (int)w->n, (int)w->k, (int)((w->k + 127) / 128), wide,
+                        l.bytes ? (float*)workspace : nullptr, l.splits};
     const DeviceScope scope(ncm_ctx_device(ctx));
     rc = step_hip(scope.error(), "linear_int4 device");
     if (rc) return rc;
     const hipStream_t st = ncm_ctx_stream(ctx);
     auto go = [&](auto group) {
         constexpr int GROUP = decltype(group)::value;
-        w->has_zeros ? launch<GROUP, true>(a, out_mode, st) : launch<GROUP, false>(a, out_mode, st);
+        w->has_zeros ? launch<GROUP, true>(a, l, out_mode, st) : launch<GROUP, false>(a, l, out_mode, st);
     };
     if (w->group == 32) go(std::integral_constant<int, 32>());
     else if (w->group == 64) go(std::integral_constant<int, 64>());

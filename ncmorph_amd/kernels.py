@@ -369,12 +369,13 @@ def quantise_int4(w, group: int, symmetric: bool = True, ctx=None):
 
 
 def linear_int4(x, w: Int4Weight, bias=None, residual=None, out=None, out_mode: str = "f32",
-                ctx=None):
+                workspace=None, ctx=None):
     """y = x @ weight.T (+ bias) (+ residual) with 4-bit weights: x
     torch.bfloat16 [m, >= k] with contiguous rows, bias bf16 [n], residual
     float32 [m, n], sums in fp32 and one rounding; out [m, n] float32 ("f32",
     "bf16_f32") or torch.bfloat16 ("bf16"), for the float modes residual itself
-    if wanted. For the rows of a decode step; it uses no workspace."""
+    if wanted. For the rows of a decode step. workspace: uint8 scratch, taken from
+    torch's allocator where not given and needed."""
     import torch
 
     W = "linear_int4"
@@ -392,10 +393,21 @@ def linear_int4(x, w: Int4Weight, bias=None, residual=None, out=None, out_mode: 
     else:
         po = a.dev(out, "out", _out_dtypes(mode), (m, n))
     a.seen += w.named
+    size = 0
+    pw = None
+    if workspace is not None:
+        pw, size = a.dev(workspace, "workspace", ("uint8",)), workspace.numel()
     a.done()
+    if workspace is None and m > 16:  # fewer rows need none
+        need = C.c_size_t()
+        check(lib().ncm_linear_int4_workspace(m, n, w.k, C.byref(need)), W)
+        size = need.value
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+            pw = workspace.data_ptr()
     ctx = stream_context(x.device, ctx)
     check(lib().ncm_linear_int4(ctx.handle, px, stride if m > 1 else (w.k + 7) // 8 * 8,
-                                C.byref(w.struct), pb, pr, po, m, mode), W)
+                                C.byref(w.struct), pb, pr, po, m, mode, pw, size), W)
     return out
 
 

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from ncmorph_amd import kernels
-from ncmorph_amd._lib import NCM_E_ARG, NCM_E_NULL, NCM_E_SHAPE, NcmError, lib
+from ncmorph_amd._lib import NCM_E_ARG, NCM_E_LENGTH, NCM_E_NULL, NCM_E_SHAPE, NcmError, lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 bf, u8 = torch.bfloat16, torch.uint8
@@ -61,6 +61,7 @@ def test_wrappers(ncm):
     _raises(NCM_E_ARG, K, x, w, out_mode="fp8")
     _raises(NCM_E_ARG, K, x, w, out=z(3, 20))
     _raises(NCM_E_SHAPE, K, x, w, out=z(2, 20), out_mode="bf16")
+    _raises(NCM_E_ARG, K, x, w, workspace=z(64))
 
 
 def test_library(ncm):
@@ -72,7 +73,8 @@ def test_library(ncm):
                                                  has_zeros=0), **k)))
 
     def Y(**k):
-        d = dict(ctx=ctx, x=p, stride=136, w=weight(), bias=no, residual=no, y=p, m=3, mode=0)
+        d = dict(ctx=ctx, x=p, stride=136, w=weight(), bias=no, residual=no, y=p, m=3, mode=0,
+                 ws=no, size=0)
         return L.ncm_linear_int4(*dict(d, **k).values())
 
     for bad in (dict(ctx=no), dict(w=no), dict(x=no), dict(y=no), dict(w=weight(codes=no)),
@@ -86,6 +88,15 @@ def test_library(ncm):
                 dict(residual=p + 2), dict(w=weight(codes=p + 8)), dict(w=weight(scales=p + 8)),
                 dict(residual=p, y=p, mode=2)):
         assert Y(**bad) == NCM_E_ARG, bad
+    big = weight(n=256, k=4096)
+    assert Y(w=big, stride=4096, m=64) == NCM_E_NULL
+    assert Y(w=big, stride=4096, m=64, ws=p) == NCM_E_LENGTH
+    assert Y(w=big, stride=4096, m=64, ws=p + 4, size=1 << 30) == NCM_E_ARG
+    need = C.c_size_t()
+    ws = L.ncm_linear_int4_workspace
+    assert ws(64, 256, 4096, C.byref(need)) == 0 and need.value % (64 * 256 * 4) == 0 < need.value
+    assert ws(16, 256, 4096, C.byref(need)) == 0 and need.value == 0
+    assert ws(16, 256, 4096, None) == NCM_E_NULL and ws(-1, 256, 4096, C.byref(need)) == NCM_E_SHAPE
     assert Y(m=0) == 0 and Y(w=weight(n=0)) == 0
     a, b = C.c_size_t(), C.c_size_t()
     assert L.ncm_int4_bytes(20, 136, 64, 0, C.byref(a), C.byref(b)) == 0
