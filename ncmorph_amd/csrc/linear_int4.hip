@@ -41,11 +41,11 @@ struct Int4Args {
 template <int GROUP, bool ZEROS>
 constexpr int scale_bytes() { return 128 / GROUP * 16 * (ZEROS ? 4 : 2); }
 
-template <int GROUP, bool ZEROS, int NT, int MT>
+template <int GROUP, bool ZEROS, int NT, int MT, bool HELD>
 struct Stage {
     static constexpr int G = 128 / GROUP;
     u32x4_t w[NT];
-    u32x4_t x[MT][4];
+    u32x4_t x[HELD ? 1 : MT][4];
     uint32_t s[NT];  // a dword of the tile's scales, by lane
 };
 
@@ -85,17 +85,19 @@ __device__ __forceinline__ void store_block(const Int4Args& a, f32x4_t v, int ro
     }
 }
 
-// DEPTH: blocks of 128 inputs that a wavefront loads ahead.
-template <int GROUP, bool ZEROS, int NT, int MT, int DEPTH, int OUT>
+// DEPTH: blocks of 128 inputs that a wavefront loads ahead. HELD: all of x is in
+// LDS, [m][blocks][16] chunks, which leaves registers for more wavefronts.
+template <int GROUP, bool ZEROS, int NT, int MT, int DEPTH, bool HELD, int OUT>
 __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
-    typedef Stage<GROUP, ZEROS, NT, MT> S;
+    typedef Stage<GROUP, ZEROS, NT, MT, HELD> S;
     constexpr int G = S::G, STEPS = 4 / G;  // MFMA steps of a group
     constexpr int SB = scale_bytes<GROUP, ZEROS>() / 4;
     __shared__ f32x4_t parts[kWaves][NT * MT][64];
     // Each wavefront's scales on their way from one coalesced load to the lanes
-    // that need them (loaded by those lanes: 36 us in place of XX for 28672 x 4096
+    // that need them (loaded by those lanes: 36 us in place of 25 for 28672 x 4096
     // in groups of 32 with zero points).
     __shared__ __attribute__((aligned(16))) uint32_t scales[kWaves][NT][SB];
+    extern __shared__ u32x4_t held[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int64_t tile0 = (int64_t)blockIdx.x * NT;
@@ -108,16 +110,17 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
             s.w[t] = a.codes[at * 64 + lane];
             s.s[t] = ((const uint32_t*)a.scales)[at * SB + min(lane, SB - 1)];
         }
+        if constexpr (!HELD)
 #pragma unroll
-        for (int r = 0; r < MT; ++r) {
-            const int row = m0 + 16 * r + c;
+            for (int r = 0; r < MT; ++r) {
+                const int row = m0 + 16 * r + c;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = 128 * b + 32 * i + 8 * g;
-                s.x[r][i] = u32x4_t{0, 0, 0, 0};
-                if (row < a.m && k < a.k) s.x[r][i] = *(const u32x4_t*)(a.x + row * a.x_stride + k);
+                for (int i = 0; i < 4; ++i) {
+                    const int k = 128 * b + 32 * i + 8 * g;
+                    s.x[r][i] = u32x4_t{0, 0, 0, 0};
+                    if (row < a.m && k < a.k) s.x[r][i] = *(const u32x4_t*)(a.x + row * a.x_stride + k);
+                }
             }
-        }
     };
 
     f32x4_t sum[NT][MT];
@@ -127,7 +130,19 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
         for (int r = 0; r < MT; ++r) sum[t][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const u32x4_t one_bits = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
     const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, one_bits);
-    auto add = [&](const S& s) {
+    auto add = [&](const S& s, int b) {
+        u32x4_t x[MT][4];
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (HELD) {
+                    x[r][i] = u32x4_t{0, 0, 0, 0};
+                    if (c < a.m) x[r][i] = held[(c * a.blocks + b) * 16 + 4 * i + g];
+                } else {
+                    x[r][i] = s.x[r][i];
+                }
+            }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
             if (lane < SB) scales[wave][t][lane] = s.s[t];
@@ -145,7 +160,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
 #pragma unroll
                 for (int r = 0; r < MT; ++r)
                     of_x[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        ones, __builtin_bit_cast(bf16x8_t, s.x[r][e]), of_x[r], 0, 0, 0);
+                        ones, __builtin_bit_cast(bf16x8_t, x[r][e]), of_x[r], 0, 0, 0);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     u32x4_t q;
@@ -154,7 +169,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
 #pragma unroll
                     for (int r = 0; r < MT; ++r)
                         of_q[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(bf16x8_t, q), __builtin_bit_cast(bf16x8_t, s.x[r][e]),
+                            __builtin_bit_cast(bf16x8_t, q), __builtin_bit_cast(bf16x8_t, x[r][e]),
                             of_q[t][r], 0, 0, 0);
                 }
             }
@@ -179,6 +194,13 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i)
         if (wave + i * kWaves < a.blocks) load(now[i], wave + i * kWaves);
+    if constexpr (HELD) {
+        for (int i = threadIdx.x; i < a.m * a.blocks * 16; i += 64 * kWaves) {
+            const int row = i / (a.blocks * 16), k = 8 * (i - row * a.blocks * 16);
+            held[i] = k < a.k ? *(const u32x4_t*)(a.x + row * a.x_stride + k) : u32x4_t{0, 0, 0, 0};
+        }
+        lds_barrier();
+    }
     for (int b = wave; b < a.blocks; b += DEPTH * kWaves) {
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i) {
@@ -187,7 +209,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
         }
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i)
-            if (b + i * kWaves < a.blocks) add(now[i]);
+            if (b + i * kWaves < a.blocks) add(now[i], b + i * kWaves);
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i) now[i] = next[i];
     }
@@ -508,9 +530,15 @@ void launch(const Int4Args& a, const Int4Layout& l, int out, hipStream_t st) {
     with_out(out, [&](auto mode) {
         constexpr int OUT = decltype(mode)::value;
         if (l.rows == 0) {
-            // Two blocks ahead where there are few wavefronts to wait on each other.
-            if (tiles < 512) linear_int4_kernel<GROUP, ZEROS, 1, 1, 2, OUT><<<(uint32_t)tiles, 64 * kWaves, 0, st>>>(a);
-            else linear_int4_kernel<GROUP, ZEROS, 1, 1, 1, OUT><<<(uint32_t)tiles, 64 * kWaves, 0, st>>>(a);
+            const uint32_t blocks = (uint32_t)tiles;
+            const size_t held = (size_t)a.m * a.blocks * 256;
+            // Two blocks ahead where there are few wavefronts to wait on each other
+            // (4096 x 14336: 13.4 us, 15.5 one ahead; 28672 x 4096: 24, 22), else x in
+            // LDS where that is little (28672 x 4096, one row: 16.8 us, 22.4 without;
+            // four: 21.2, 25; six, 48 KB of x: 26.4, 25.5).
+            if (tiles < 512) linear_int4_kernel<GROUP, ZEROS, 1, 1, 2, false, OUT><<<blocks, 64 * kWaves, 0, st>>>(a);
+            else if (held <= 32 * 1024) linear_int4_kernel<GROUP, ZEROS, 1, 1, 1, true, OUT><<<blocks, 64 * kWaves, held, st>>>(a);
+            else linear_int4_kernel<GROUP, ZEROS, 1, 1, 1, false, OUT><<<blocks, 64 * kWaves, 0, st>>>(a);
             return;
         }
         const dim3 grid((uint32_t)((tiles + 7) / 8), (uint32_t)((a.m + l.rows - 1) / l.rows), (uint32_t)l.splits);
