@@ -22,15 +22,24 @@
 namespace ncm {
 namespace {
 
+// What is known of a group before its units are cut: its first request and its
+// rows (none where there is no prefix), the prefix's tokens, those of them that
+// the kernel for many pairs does, and the tile that the narrow units begin with.
+struct GroupPlan {
+    int r0, r1, o0, n;
+    int tokens, done, tile0, pad;
+};
+
 struct SharedArgs {
     AttnArgs a;
     const int32_t* groups;  // [n_groups + 1]
     const int32_t* shared;  // [n_groups]
     int n_groups;
     int prefix_units, own_units;  // there is room for
-    // Groups of many pairs: {first request, tokens, first row, rows} of what their
-    // own kernel does (NULL: it does not run), its units, their pairs and parts.
-    int4* plans;
+    GroupPlan* plans;
+    int* floors;         // of each request: tokens that it reads through its group
+    // The kernel for groups of many pairs, its units, their pairs (0: it does not
+    // run) and parts.
     int wide_units, wide_pairs;
     int* wide_base;
     int4* wide_joins;
@@ -42,20 +51,6 @@ struct SharedArgs {
     int64_t prefix_cut;               // rows of the parts of groups' units in several
 };
 
-// Group g's requests [r0, r1) and the tokens that they share; none where there
-// is nothing to share them with.
-struct Group {
-    int r0, r1, tokens;
-};
-__device__ __forceinline__ Group group_of(const SharedArgs& s, int g) {
-    Group q;
-    q.r0 = min(max(s.groups[g], 0), s.a.batch.requests);
-    q.r1 = min(max(s.groups[g + 1], q.r0), s.a.batch.requests);
-    q.tokens = q.r1 - q.r0 < 2
-                   ? 0
-                   : (int)min((int64_t)max(s.shared[g], 0), s.a.batch.capacity);
-    return q;
-}
 // The group of request r, or -1.
 __device__ __forceinline__ int group_with(const SharedArgs& s, int r) {
     int lo = 0, hi = s.n_groups;  // the first group that ends behind r
@@ -67,26 +62,62 @@ __device__ __forceinline__ int group_with(const SharedArgs& s, int r) {
     return lo < s.n_groups && s.groups[lo] <= r ? lo : -1;
 }
 
-template <int RP>
-__device__ __forceinline__ Need group_need(const SharedArgs& s, int g) {
-    const Group q = group_of(s, g);
-    const AttnArgs& a = s.a;
-    Need d;
-    d.q.o0 = d.q.n = 0;
-    d.q.before = d.end = d.before = q.tokens;
-    d.base = d.floor = s.plans ? s.plans[g].y : 0;
-    d.tile0 = 0;
-    if (q.tokens > d.base) {
-        d.q.o0 = min(max(a.batch.offsets[q.r0], 0), a.batch.rows);
-        d.q.n = max(min(a.batch.offsets[q.r1], a.batch.rows) - d.q.o0, 0);
-        if (a.window > 0) {
-            int least = q.tokens;
-            for (int r = q.r0; r < q.r1; ++r) least = min(least, max(a.batch.starts[r], 0));
-            d.tile0 = (int)(max((int64_t)least - a.window + 1, (int64_t)0) / kTile);
+constexpr int kWideTile = 64;   // tokens of a tile of the kernel for many pairs
+constexpr int kWidePairs = 48;  // of a group, from which on it has that kernel
+
+// The plans, a wavefront per group, and behind them the floors, a thread per
+// request: once, instead of by every workgroup of the kernels that cut the units.
+__global__ __launch_bounds__(256) void kv_attention_plan_kernel(SharedArgs s, int group_blocks) {
+    const BatchView& b = s.a.batch;
+    auto tokens_of = [&](int g, int r0, int r1) {
+        return r1 - r0 < 2 ? 0 : (int)min((int64_t)max(s.shared[g], 0), b.capacity);
+    };
+    auto first_of = [&](int g) { return min(max(s.groups[g], 0), b.requests); };
+    if ((int)blockIdx.x >= group_blocks) {
+        const int r = ((int)blockIdx.x - group_blocks) * 256 + (int)threadIdx.x;
+        if (r >= b.requests) return;
+        const int before = (int)min((int64_t)max(b.starts[r], 0), b.capacity);
+        const int g = group_with(s, r);
+        int floor = 0;
+        if (g >= 0) {
+            const int r0 = first_of(g);
+            floor = min(tokens_of(g, r0, min(max(s.groups[g + 1], r0), b.requests)), before);
         }
+        s.floors[r] = floor;
+        return;
     }
+    const int g = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (g >= s.n_groups) return;
+    GroupPlan p = {};
+    p.r0 = first_of(g);
+    p.r1 = min(max(s.groups[g + 1], p.r0), b.requests);
+    p.tokens = tokens_of(g, p.r0, p.r1);
+    if (p.tokens > 0) {
+        p.o0 = min(max(b.offsets[p.r0], 0), b.rows);
+        p.n = max(min(b.offsets[p.r1], b.rows) - p.o0, 0);
+        int least = p.tokens;  // before its requests with rows
+        for (int r = p.r0 + lane; r < p.r1; r += 64) {
+            const Request one = request_of(b, r);
+            least = min(least, one.n > 0 ? one.before : p.tokens);
+        }
+        for (int x = 32; x; x >>= 1) least = min(least, __shfl_xor(least, x));
+        if (s.wide_pairs) p.done = least / kWideTile * kWideTile;
+        if (s.a.window > 0)
+            p.tile0 = (int)(max((int64_t)least - s.a.window + 1, (int64_t)0) / kTile);
+    }
+    if (lane == 0) s.plans[g] = p;
+}
+
+template <int RP>
+__device__ __forceinline__ Need group_need(const SharedArgs& s, const GroupPlan& p) {
+    Need d;
+    d.q.o0 = p.o0;
+    d.q.n = p.tokens > p.done ? p.n : 0;
+    d.q.before = d.end = d.before = p.tokens;
+    d.base = d.floor = p.done;
+    d.tile0 = p.tile0;
     d.tiles = max((d.end - d.base + kTile - 1) / kTile - d.tile0, 1);
-    d.blocks = (int)(((int64_t)d.q.n * a.group + 16 * RP - 1) / (16 * RP));
+    d.blocks = (int)(((int64_t)d.q.n * s.a.group + 16 * RP - 1) / (16 * RP));
     return d;
 }
 
@@ -95,11 +126,10 @@ __device__ __forceinline__ Need own_need(const SharedArgs& s, int r) {
     const AttnArgs& a = s.a;
     const int64_t cap = a.batch.capacity;
     Need d;
+    d.floor = s.floors[r];
     d.q = request_of(a.batch, r);
     d.end = (int)min((int64_t)d.q.before + d.q.n, cap);
     d.before = (int)min((int64_t)d.q.before, cap);
-    const int g = group_with(s, r);
-    d.floor = g < 0 ? 0 : min(group_of(s, g).tokens, d.before);
     const int64_t low = a.window > 0 ? max((int64_t)d.q.before - a.window + 1, (int64_t)0) : 0;
     d.base = (int)max((int64_t)d.floor, min(low, cap)) & ~15;
     d.tile0 = 0;
@@ -110,7 +140,7 @@ __device__ __forceinline__ Need own_need(const SharedArgs& s, int r) {
 
 template <int RP, int RO>
 __device__ __forceinline__ Need segment_need(const SharedArgs& s, int seg) {
-    return seg < s.n_groups ? group_need<RP>(s, seg) : own_need<RO>(s, seg - s.n_groups);
+    return seg < s.n_groups ? group_need<RP>(s, s.plans[seg]) : own_need<RO>(s, seg - s.n_groups);
 }
 
 // RP and RO: 16 pairs of a group's and of a request's unit.
@@ -159,7 +189,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_shared_kernel(SharedArgs 
         int64_t u = u_at;
         for (int x = s0; x < min(s1, s.n_groups); ++x) {
             s.unit_base[x] = (int)min(u, (int64_t)s.prefix_units);
-            u += (int64_t)group_need<RP>(s, x).blocks * heads;
+            u += (int64_t)group_need<RP>(s, s.plans[x]).blocks * heads;
         }
     }
     if (me >= groups) return;
@@ -178,11 +208,12 @@ __global__ __launch_bounds__(256, 2) void kv_attention_shared_kernel(SharedArgs 
     __syncthreads();
     int seg = uniform(found);
     int64_t start = uniform(found_at), u0 = uniform(found_units);  // of the segment
+    Need d = segment_need<RP, RO>(s, seg);
     while (at < end) {
-        const Need d = segment_need<RP, RO>(s, seg);
         const int64_t n = (int64_t)d.blocks * heads * d.tiles;
         if (at >= start + n) {
             start += n, u0 += (int64_t)d.blocks * heads, ++seg;
+            d = segment_need<RP, RO>(s, seg);
             continue;
         }
         const bool is_group = seg < s.n_groups;
@@ -206,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_shared_kernel(SharedArgs 
         if (!room) {
             // Offsets that give rows to several requests: no record, no result.
         } else if (is_group) {
-            const Group of = group_of(s, seg);
+            const GroupPlan& of = s.plans[seg];
             run_unit<HD, CODES, RP, true>(a, d, of.r0, h, block, first, count, part, lds, of.r1);
         } else {
             run_unit<HD, CODES, RO, false>(a, d, seg - s.n_groups, h, block, first, count, part,
@@ -217,9 +248,6 @@ __global__ __launch_bounds__(256, 2) void kv_attention_shared_kernel(SharedArgs 
 }
 
 // ------------------------------------------------------- groups of many pairs
-
-constexpr int kWideTile = 64;   // tokens of a tile
-constexpr int kWidePairs = 48;  // of a group, from which on it has the kernel
 
 // A tile of K and V as bf16, rows of HD values; 16-byte chunk c of row r of K is
 // at chunk c ^ (r % 16) (HD 64: c ^ (r / 2 % 8)), so that the sixteen rows of an
@@ -423,9 +451,10 @@ struct Wide {
     int r0, o0, rows, tiles, blocks;
 };
 __device__ __forceinline__ Wide wide_of(const SharedArgs& s, int g) {
-    const int4 p = s.plans[g];
-    return {p.x, p.z, p.w, max(p.y / kWideTile, 1),
-            (int)(((int64_t)p.w * s.a.group + s.wide_pairs - 1) / s.wide_pairs)};
+    const GroupPlan& p = s.plans[g];
+    const int rows = p.done > 0 ? p.n : 0;
+    return {p.r0, p.o0, rows, max(p.done / kWideTile, 1),
+            (int)(((int64_t)rows * s.a.group + s.wide_pairs - 1) / s.wide_pairs)};
 }
 
 // Tiles [first, first + count) of a group's unit, into the part that begins at row
@@ -549,30 +578,6 @@ __device__ __forceinline__ void run_wide(const SharedArgs& s, const Wide& d, int
     __syncthreads();
 }
 
-// What the kernel below does of each group, by a wavefront: the tiles of tokens
-// that all its requests with rows have before these.
-__global__ __launch_bounds__(256) void kv_attention_plan_kernel(SharedArgs s) {
-    const int g = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
-    if (g >= s.n_groups) return;
-    const Group q = group_of(s, g);
-    const BatchView& b = s.a.batch;
-    int least = q.tokens;
-    if (q.tokens > 0)
-        for (int r = q.r0 + lane; r < q.r1; r += 64) {
-            const Request one = request_of(b, r);
-            least = min(least, one.n > 0 ? one.before : q.tokens);
-        }
-    for (int x = 32; x; x >>= 1) least = min(least, __shfl_xor(least, x));
-    if (lane == 0) {
-        int4 plan = {q.r0, least / kWideTile * kWideTile, 0, 0};
-        if (plan.y > 0) {
-            plan.z = min(max(b.offsets[q.r0], 0), b.rows);
-            plan.w = max(min(b.offsets[q.r1], b.rows) - plan.z, 0);
-        }
-        s.plans[g] = plan;
-    }
-}
-
 template <int HD, int CODES, int NP>
 __global__ __launch_bounds__(512, 2) void kv_attention_prefix_kernel(SharedArgs s) {
     __shared__ WideLds<HD> lds;
@@ -628,11 +633,12 @@ __global__ __launch_bounds__(512, 2) void kv_attention_prefix_kernel(SharedArgs 
     __syncthreads();
     int seg = uniform(found);
     int64_t start = uniform(found_at), u0 = uniform(found_units);  // of the group
+    Wide d = wide_of(s, seg);
     while (at < end) {
-        const Wide d = wide_of(s, seg);
         const int64_t n = (int64_t)d.blocks * heads * d.tiles;
         if (at >= start + n) {
             start += n, u0 += (int64_t)d.blocks * heads, ++seg;
+            d = wide_of(s, seg);
             continue;
         }
         const int u = (int)((at - start) / d.tiles);
@@ -670,8 +676,8 @@ __global__ __launch_bounds__(256) void kv_attention_shared_join_kernel(SharedArg
     Need p = {};
     Wide w = {};
     if (d.floor > 0) {
-        p = group_need<RP>(s, g);
-        if (s.plans) w = wide_of(s, g);
+        p = group_need<RP>(s, s.plans[g]);
+        if (s.wide_pairs) w = wide_of(s, g);
     }
     constexpr int L = HD / 4;  // lanes of a part
     const bool few = j.y <= 16;
@@ -748,7 +754,7 @@ struct SharedLayout {
     int64_t runs, wide_runs;          // workgroups
     int64_t some;                     // requests that may have rows
     int64_t whole_prefix, whole_own, wide_cut, whole_wide;  // rows of parts
-    size_t plans, base, wide_base, joins, ml, o, bytes;     // offsets in the workspace
+    size_t plans, floors, base, wide_base, joins, ml, o, bytes;     // offsets in the workspace
 };
 
 SharedLayout shared_layout(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int64_t n_groups,
@@ -774,7 +780,8 @@ SharedLayout shared_layout(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int
     const size_t rows = (size_t)(s.whole_wide + s.wide_units * 32 * s.wide);
     auto up = [](size_t bytes) { return (bytes + 15) / 16 * 16; };
     s.plans = 16;
-    s.base = s.plans + (s.wide ? 16 * (size_t)n_groups : 0);
+    s.floors = s.plans + sizeof(GroupPlan) * (size_t)n_groups;
+    s.base = s.floors + up(4 * (size_t)b.requests);
     s.wide_base = s.base + up(4 * (size_t)n_groups);
     s.joins = s.wide_base + up(4 * (size_t)n_groups);
     s.ml = s.joins + 16 * (size_t)(s.prefix_units + s.own_units + s.wide_units);
@@ -785,7 +792,9 @@ SharedLayout shared_layout(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int
 
 template <int HD, int CODES, int RP, int RO>
 hipError_t launch_shared(const SharedArgs& a, const SharedLayout& s, hipStream_t st) {
-    if (s.wide) kv_attention_plan_kernel<<<(uint32_t)((a.n_groups + 3) / 4), 256, 0, st>>>(a);
+    const int group_blocks = (a.n_groups + 3) / 4;
+    kv_attention_plan_kernel<<<(uint32_t)(group_blocks + (a.a.batch.requests + 255) / 256), 256, 0, st>>>(
+        a, group_blocks);
     if (s.wide == 2) kv_attention_prefix_kernel<HD, CODES, 2><<<(uint32_t)s.wide_runs, 512, 0, st>>>(a);
     if (s.wide == 4) kv_attention_prefix_kernel<HD, CODES, 4><<<(uint32_t)s.wide_runs, 512, 0, st>>>(a);
     if (s.wide == 8) kv_attention_prefix_kernel<HD, CODES, 8><<<(uint32_t)s.wide_runs, 512, 0, st>>>(a);
@@ -883,7 +892,8 @@ extern "C" int ncm_kv_attention_shared_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t*
     s.groups = groups, s.shared = shared, s.n_groups = (int)n_groups;
     s.prefix_units = (int)l.prefix_units, s.own_units = (int)l.own_units;
     s.counts = (int*)ws;
-    if (l.wide) s.plans = (int4*)(ws + l.plans);
+    s.plans = (GroupPlan*)(ws + l.plans);
+    s.floors = (int*)(ws + l.floors);
     s.unit_base = (int*)(ws + l.base);
     s.wide_base = (int*)(ws + l.wide_base);
     s.joins = (int4*)(ws + l.joins);
