@@ -765,11 +765,18 @@ SharedLayout shared_layout(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int
     s.ro = pairs <= 16 * s.some ? 1 : 2;
     const int64_t per_group = pairs / std::max<int64_t>(1, std::min(n_groups, s.some));
     s.rp = std::max(s.ro, per_group <= 16 ? 1 : 2);
-    s.wide = n_groups == 0 || window || per_group < kWidePairs ? 0 : per_group <= 64 ? 2 : per_group <= 128 ? 4 : 8;
+    s.wide = n_groups == 0 || window || per_group < kWidePairs ? 0 : per_group <= 64 ? 2 : 4;
+    const int64_t tokens = std::max<int64_t>(1, b.table_width * c.page_size);
+    // Eight wavefronts of pairs, each tile of the prefix brought once for 256, where
+    // that leaves a workgroup tiles enough to be worth the state that it writes and
+    // the join reads (1024 pairs behind 16000 tokens, 31 tiles each: 136 us, 158
+    // with four; 256 behind 8192, 4 tiles each: 35 and a join of 11.8 us, 36 and 8.6).
+    if (s.wide == 4 && per_group > 128 &&
+        (pairs / 256 + n_groups) * c.kv_heads * (tokens / kWideTile) >= 12 * kCus)
+        s.wide = 8;
     s.own_units = (pairs / (16 * s.ro) + s.some) * c.kv_heads;
     s.prefix_units = n_groups ? (pairs / (16 * s.rp) + n_groups) * c.kv_heads : 0;
     s.wide_units = s.wide ? (pairs / (32 * s.wide) + n_groups) * c.kv_heads : 0;
-    const int64_t tokens = std::max<int64_t>(1, b.table_width * c.page_size);
     const int64_t tiles = (tokens + kTile - 1) / kTile;
     s.runs = std::min<int64_t>((s.own_units + s.prefix_units) * tiles, 2 * kCus);
     s.wide_runs = std::min<int64_t>(s.wide_units * ((tokens + kWideTile - 1) / kWideTile), kCus);
