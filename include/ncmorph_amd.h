@@ -192,7 +192,7 @@ int ncm_linear_bf16_swiglu(ncm_ctx_t* ctx, const uint16_t* x, const uint16_t* w,
 /* A weight matrix [n, k] in 4-bit codes, in the order in which ncm_linear_int4
  * reads it (ncm_int4_pack_dev): weight = (code - zero) * scale, codes and zeros 0
  * .. 15, one bf16 scale (and one zero, or 8 for all) per output and group of 32,
- * 64 or 128 inputs. n up to 2^28, k a multiple of 8 up to 2^24 (the last group
+ * 64 or 128 inputs. n up to 2^26, k a multiple of 8 up to 2^24 (the last group
  * may be short), and ceil(n / 16) * ceil(k / 128) below 2^24. */
 typedef struct ncm_int4_weight {
     const void* codes;   /* ncm_int4_bytes' bytes, 16-byte aligned */

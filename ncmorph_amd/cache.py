@@ -337,6 +337,8 @@ def extend(pool, page_table, new, starts, rows: int, page_size: int, tree_mask=N
     if tree_mask is not None:
         _, words = _ck.dims(tree_mask, "tree_mask", W, 2)
     pm = a.dev(tree_mask, "tree_mask", _ck.U64, (rows, words), optional=True)
+    if rows < 0:
+        raise NcmError(NCM_E_SHAPE, W, "rows must not be negative")
     a.done()
     dev = page_table.device
     # One allocation for what is int32, slots apart.

@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256) void int4_quantise_kernel(const uint16_t* w, i
 }
 
 int check_int4(int64_t n, int64_t k, int group) {
-    if (n < 0 || n > (1 << 28) || k < 8 || k > (1 << 24) || k % 8 ||
+    if (n < 0 || n > (1 << 26) || k < 8 || k > (1 << 24) || k % 8 ||
         (group != 32 && group != 64 && group != 128))
         return NCM_E_SHAPE;
     // A workgroup per 16 outputs and 128 inputs packs them.

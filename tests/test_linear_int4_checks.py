@@ -82,7 +82,8 @@ def test_library(ncm):
         assert Y(**bad) == NCM_E_NULL, bad
     for bad in (dict(m=-1), dict(m=(1 << 20) + 1), dict(stride=128), dict(w=weight(k=132)),
                 dict(w=weight(k=0)), dict(w=weight(n=-1)), dict(w=weight(group=48)),
-                dict(w=weight(n=1 << 28, k=1 << 10))):
+                dict(w=weight(n=1 << 28, k=1 << 10)), dict(w=weight(n=(1 << 26) + 1, k=8),
+                                                           stride=8)):
         assert Y(**bad) == NCM_E_SHAPE, bad
     for bad in (dict(mode=3), dict(x=p + 8), dict(stride=140), dict(y=p + 2), dict(bias=p + 1),
                 dict(residual=p + 2), dict(w=weight(codes=p + 8)), dict(w=weight(scales=p + 8)),

@@ -44,6 +44,7 @@ def test_wrappers():
     _raises(NCM_E_ARG, E, pool, z(5, 3).t(), l, l, 4, 16)
     _raises(NCM_E_SHAPE, E, pool, t, l, l, 4, 16, tree_mask=z(3, 1, dtype=torch.int64))
     _raises(NCM_E_ARG, E, pool, t, l, l, 4, 16, tree_mask=z(4, 1))
+    _raises(NCM_E_SHAPE, E, pool, t, l, l, -1, 16)
     for fn in (cache.share, cache.release):
         assert "GPU" in _raises(NCM_E_ARG, fn, pool, t, l, l, 16)
         _raises(NCM_E_ARG, fn, None, t, l, l, 16)
