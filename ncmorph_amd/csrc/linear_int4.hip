@@ -13,8 +13,12 @@
 //
 // Bound by the weights' bytes for few rows. They are packed once in the order
 // of the lanes: 16 outputs and 128 inputs are 1 KB, a wavefront's 16-byte load.
-// A workgroup makes 16 NT outputs of 16 MT rows, its eight wavefronts taking
-// every eighth 128 inputs; their sums are added in order through LDS.
+// A workgroup makes 16 outputs of up to 16 rows, its eight wavefronts taking
+// every eighth 128 inputs; their sums are added in order through LDS. 28672 x 4096
+// in groups of 128, weights from HBM: one row 16.8 us (3.6 TB/s), 8 rows 28, 16 33;
+// in groups of 32 with zeros, a scale and two fp32 operations an output, row and
+// group: 20 and 35. More rows (linear_int4_rows_kernel) are bound by the unpacking
+// and the group sums, repeated for every 32 rows: 256 rows 125 us (480 TFLOP/s).
 #include "step.h"
 
 namespace ncm {
@@ -41,12 +45,12 @@ struct Int4Args {
 template <int GROUP, bool ZEROS>
 constexpr int scale_bytes() { return 128 / GROUP * 16 * (ZEROS ? 4 : 2); }
 
-template <int GROUP, bool ZEROS, int NT, int MT, bool HELD>
+// What a wavefront loads of 128 inputs.
+template <bool HELD>
 struct Stage {
-    static constexpr int G = 128 / GROUP;
-    u32x4_t w[NT];
-    u32x4_t x[HELD ? 1 : MT][4];
-    uint32_t s[NT];  // a dword of the tile's scales, by lane
+    u32x4_t w;
+    u32x4_t x[HELD ? 1 : 4];
+    uint32_t s;  // a dword of the tile's scales, by lane
 };
 
 // Four outputs of a row, from column `col` on.
@@ -87,104 +91,69 @@ __device__ __forceinline__ void store_block(const Int4Args& a, f32x4_t v, int ro
 
 // DEPTH: blocks of 128 inputs that a wavefront loads ahead. HELD: all of x is in
 // LDS, [m][blocks][16] chunks, which leaves registers for more wavefronts.
-template <int GROUP, bool ZEROS, int NT, int MT, int DEPTH, bool HELD, int OUT>
+template <int GROUP, bool ZEROS, int DEPTH, bool HELD, int OUT>
 __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
-    typedef Stage<GROUP, ZEROS, NT, MT, HELD> S;
-    constexpr int G = S::G, STEPS = 4 / G;  // MFMA steps of a group
+    typedef Stage<HELD> S;
+    constexpr int G = 128 / GROUP, STEPS = 4 / G;  // MFMA steps of a group
     constexpr int SB = scale_bytes<GROUP, ZEROS>() / 4;
-    __shared__ f32x4_t parts[kWaves][NT * MT][64];
+    __shared__ f32x4_t parts[kWaves][64];
     // Each wavefront's scales on their way from one coalesced load to the lanes
     // that need them (loaded by those lanes: 36 us in place of 25 for 28672 x 4096
     // in groups of 32 with zero points).
-    __shared__ __attribute__((aligned(16))) uint32_t scales[kWaves][NT][SB];
+    __shared__ __attribute__((aligned(16))) uint32_t scales[kWaves][SB];
     extern __shared__ u32x4_t held[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int64_t tile0 = (int64_t)blockIdx.x * NT;
-    const int tiles = (a.n + 15) / 16, m0 = blockIdx.y * 16 * MT;
+    const int64_t tile = blockIdx.x;
 
     auto load = [&](S& s, int b) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int64_t at = min(tile0 + t, (int64_t)tiles - 1) * a.blocks + b;
-            s.w[t] = a.codes[at * 64 + lane];
-            s.s[t] = ((const uint32_t*)a.scales)[at * SB + min(lane, SB - 1)];
-        }
+        const int64_t at = tile * a.blocks + b;
+        s.w = a.codes[at * 64 + lane];
+        s.s = ((const uint32_t*)a.scales)[at * SB + min(lane, SB - 1)];
         if constexpr (!HELD)
 #pragma unroll
-            for (int r = 0; r < MT; ++r) {
-                const int row = m0 + 16 * r + c;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = 128 * b + 32 * i + 8 * g;
-                    s.x[r][i] = u32x4_t{0, 0, 0, 0};
-                    if (row < a.m && k < a.k) s.x[r][i] = *(const u32x4_t*)(a.x + row * a.x_stride + k);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int k = 128 * b + 32 * i + 8 * g;
+                s.x[i] = u32x4_t{0, 0, 0, 0};
+                if (c < a.m && k < a.k) s.x[i] = *(const u32x4_t*)(a.x + c * a.x_stride + k);
             }
     };
 
-    f32x4_t sum[NT][MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < MT; ++r) sum[t][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
     const u32x4_t one_bits = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
     const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, one_bits);
     auto add = [&](const S& s, int b) {
-        u32x4_t x[MT][4];
+        bf16x8_t x[4];
 #pragma unroll
-        for (int r = 0; r < MT; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (HELD) {
-                    x[r][i] = u32x4_t{0, 0, 0, 0};
-                    if (c < a.m) x[r][i] = held[(c * a.blocks + b) * 16 + 4 * i + g];
-                } else {
-                    x[r][i] = s.x[r][i];
-                }
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (HELD) {
+                u32x4_t bits = {0, 0, 0, 0};
+                if (c < a.m) bits = held[(c * a.blocks + b) * 16 + 4 * i + g];
+                x[i] = __builtin_bit_cast(bf16x8_t, bits);
+            } else {
+                x[i] = __builtin_bit_cast(bf16x8_t, s.x[i]);
             }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-            if (lane < SB) scales[wave][t][lane] = s.s[t];
+        }
+        if (lane < SB) scales[wave][lane] = s.s;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            f32x4_t of_x[MT], of_q[NT][MT];
-#pragma unroll
-            for (int r = 0; r < MT; ++r) {
-                of_x[r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) of_q[t][r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+            f32x4_t of_x = {0.0f, 0.0f, 0.0f, 0.0f}, of_q = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int e = STEPS * i; e < STEPS * (i + 1); ++e) {
+                of_x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, x[e], of_x, 0, 0, 0);
+                u32x4_t q;
 #pragma unroll
-                for (int r = 0; r < MT; ++r)
-                    of_x[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        ones, __builtin_bit_cast(bf16x8_t, x[r][e]), of_x[r], 0, 0, 0);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    u32x4_t q;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) q[j] = ((s.w[t][e] >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
-#pragma unroll
-                    for (int r = 0; r < MT; ++r)
-                        of_q[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(bf16x8_t, q), __builtin_bit_cast(bf16x8_t, x[r][e]),
-                            of_q[t][r], 0, 0, 0);
-                }
+                for (int j = 0; j < 4; ++j) q[j] = ((s.w[e] >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+                of_q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, q), x[e], of_q,
+                                                               0, 0, 0);
             }
+            const uint32_t* words = &scales[wave][i * (ZEROS ? 16 : 8) + g * (ZEROS ? 4 : 2)];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint32_t* words = &scales[wave][t][i * (ZEROS ? 16 : 8) + g * (ZEROS ? 4 : 2)];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t word = words[ZEROS ? j : j / 2];
-                    const float scale = __uint_as_float(!ZEROS && j % 2 == 0 ? word << 16 : word & 0xFFFF0000u);
-                    const float zero = ZEROS ? __uint_as_float(word << 16) : 136.0f;
-#pragma unroll
-                    for (int r = 0; r < MT; ++r)
-                        sum[t][r][j] = fmaf(scale, fmaf(-zero, of_x[r][j], of_q[t][r][j]), sum[t][r][j]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t word = words[ZEROS ? j : j / 2];
+                const float scale = __uint_as_float(!ZEROS && j % 2 == 0 ? word << 16 : word & 0xFFFF0000u);
+                const float zero = ZEROS ? __uint_as_float(word << 16) : 136.0f;
+                sum[j] = fmaf(scale, fmaf(-zero, of_x[j], of_q[j]), sum[j]);
             }
         }
         asm volatile("" ::: "memory");  // the next block's scales stay behind these reads
@@ -214,31 +183,33 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
         for (int i = 0; i < DEPTH; ++i) now[i] = next[i];
     }
 
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < MT; ++r) parts[wave][t * MT + r][lane] = sum[t][r];
+    parts[wave][lane] = sum;
     __syncthreads();
-    for (int i = wave; i < NT * MT; i += kWaves) {
-        f32x4_t v = parts[0][i][lane];
+    if (wave > 0) return;
+    f32x4_t v = parts[0][lane];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) {
-            const f32x4_t p = parts[w][i][lane];
+    for (int w = 1; w < kWaves; ++w) {
+        const f32x4_t p = parts[w][lane];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = v[j] + p[j];
-        }
-        store_block<OUT>(a, v, m0 + 16 * (i % MT) + c, (tile0 + i / MT) * 16 + 4 * g);
+        for (int j = 0; j < 4; ++j) v[j] = v[j] + p[j];
     }
+    store_block<OUT>(a, v, c, tile * 16 + 4 * g);
 }
 
-// More rows: the rows of x are shared by NW wavefronts of 32 outputs each, in LDS,
-// and 8 / NW sets of these take every 8 / NW-th 128 inputs. Weights go from memory
-// to registers a block ahead; scales through LDS, which gives each lane its four
-// outputs' without 64 registers for them. 16-byte chunk c of row r of x is at
+// More rows, 32 a workgroup: they are shared by NW wavefronts of 32 outputs each,
+// in LDS, and 8 / NW sets of these take every 8 / NW-th 128 inputs. Weights go from
+// memory to registers a block ahead; scales through LDS, which gives each lane its
+// four outputs' without 64 registers for them. 16-byte chunk c of row r of x is at
 // chunk c ^ (r % 16), so that an operand's sixteen rows fall into different banks.
-template <int GROUP, bool ZEROS, int NW, int MT, int OUT>
+// 32 rows leave room for two workgroups a CU, of which one computes while the other
+// waits: 28672 x 4096 in groups of 128, 256 rows 125 us, 136 with 64 rows a
+// workgroup and half the reads of the weights; 96 rows 57, 68; 4096 x 14336,
+// 128 rows 38, 38.5.
+constexpr int kRowsOf = 32;
+template <int GROUP, bool ZEROS, int OUT>
 __global__ __launch_bounds__(512, 2) void linear_int4_rows_kernel(Int4Args a) {
-    constexpr int KW = 8 / NW, G = 128 / GROUP, STEPS = 4 / G, NT = 2, ROWS = 16 * MT;
+    constexpr int NW = 4, KW = 8 / NW, G = 128 / GROUP, STEPS = 4 / G, NT = 2;
+    constexpr int ROWS = kRowsOf, MT = ROWS / 16;
     constexpr int SB = scale_bytes<GROUP, ZEROS>() / 4;  // dwords of a tile's block
     constexpr int PER = KW * ROWS * 16 / 512;            // chunks of x a thread brings
     __shared__ u32x4_t xs[2][KW][ROWS][16];
@@ -504,22 +475,28 @@ void with_out(int out, F f) {
 
 // How a product is laid out, by its sizes.
 struct Int4Layout {
-    int rows;      // of a workgroup, 0: the kernel of few rows
+    bool few;      // rows: the kernel without shared ones
     int splits;    // of the inputs
     size_t bytes;  // of the workspace
 };
+// 4096 x 4096, 16 rows: 7.4 us, 11.9 in the kernel of more rows; 4096 x 14336: 18.8,
+// 19.4; 28672 x 4096: 33, 28 (8 rows 28, 28).
 constexpr int kFewRows = 16;
 
 Int4Layout int4_layout(int64_t m, int64_t n, int64_t k) {
-    Int4Layout l = {0, 1, 0};
-    if (m <= kFewRows) return l;
-    l.rows = m <= 32 ? 32 : 64;
-    // Workgroups of 128 outputs. Fewer than the CUs: the inputs are split, at most
-    // to two steps of 256 each (every output tile reads all of x, so narrower
-    // tiles would only move the load to that).
-    const int64_t groups = (n + 127) / 128 * ((m + l.rows - 1) / l.rows);
+    Int4Layout l = {m <= kFewRows, 1, 0};
+    if (l.few) return l;
+    // Workgroups of 128 outputs. Where they leave a CU without two, the inputs are
+    // split, with at least four steps of 256 each; where they leave one without any,
+    // with at least two (every output tile reads all of x, so narrower tiles would
+    // only move the load to that). 28672 x 4096, 32 rows: 28 us, 30 without a split;
+    // 4096 x 14336, 64: 25 in 8, 29 in 4 parts, unsplit 71; 4096 x 4096, 64: 13.8 in
+    // 4, 15.6 in 8 parts of two steps, but 32 rows 12.6 in 8 of two, 12.8 in 4.
+    // More than 8 parts lose: 4096 x 14336, 17 rows in 16 20.7 us, in 8 19.6.
+    const int64_t groups = std::max<int64_t>(1, (n + 127) / 128 * ((m + kRowsOf - 1) / kRowsOf));
     const int64_t steps = (k + 255) / 256;
-    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(groups, 1), steps / 2, 16}));
+    const int64_t parts = std::max(std::min(512 / groups, steps / 4), std::min(256 / groups, steps / 2));
+    l.splits = (int)std::clamp<int64_t>(parts, 1, 8);
     if (l.splits > 1) l.bytes = (size_t)l.splits * m * n * 4;
     return l;
 }
@@ -529,21 +506,20 @@ void launch(const Int4Args& a, const Int4Layout& l, int out, hipStream_t st) {
     const int64_t tiles = (a.n + 15) / 16;
     with_out(out, [&](auto mode) {
         constexpr int OUT = decltype(mode)::value;
-        if (l.rows == 0) {
+        if (l.few) {
             const uint32_t blocks = (uint32_t)tiles;
             const size_t held = (size_t)a.m * a.blocks * 256;
             // Two blocks ahead where there are few wavefronts to wait on each other
             // (4096 x 14336: 13.4 us, 15.5 one ahead; 28672 x 4096: 24, 22), else x in
             // LDS where that is little (28672 x 4096, one row: 16.8 us, 22.4 without;
             // four: 21.2, 25; six, 48 KB of x: 26.4, 25.5).
-            if (tiles < 512) linear_int4_kernel<GROUP, ZEROS, 1, 1, 2, false, OUT><<<blocks, 64 * kWaves, 0, st>>>(a);
-            else if (held <= 32 * 1024) linear_int4_kernel<GROUP, ZEROS, 1, 1, 1, true, OUT><<<blocks, 64 * kWaves, held, st>>>(a);
-            else linear_int4_kernel<GROUP, ZEROS, 1, 1, 1, false, OUT><<<blocks, 64 * kWaves, 0, st>>>(a);
+            if (tiles < 512) linear_int4_kernel<GROUP, ZEROS, 2, false, OUT><<<blocks, 64 * kWaves, 0, st>>>(a);
+            else if (held <= 32 * 1024) linear_int4_kernel<GROUP, ZEROS, 1, true, OUT><<<blocks, 64 * kWaves, held, st>>>(a);
+            else linear_int4_kernel<GROUP, ZEROS, 1, false, OUT><<<blocks, 64 * kWaves, 0, st>>>(a);
             return;
         }
-        const dim3 grid((uint32_t)((tiles + 7) / 8), (uint32_t)((a.m + l.rows - 1) / l.rows), (uint32_t)l.splits);
-        if (l.rows == 32) linear_int4_rows_kernel<GROUP, ZEROS, 4, 2, OUT><<<grid, 512, 0, st>>>(a);
-        else linear_int4_rows_kernel<GROUP, ZEROS, 4, 4, OUT><<<grid, 512, 0, st>>>(a);
+        const dim3 grid((uint32_t)((tiles + 7) / 8), (uint32_t)((a.m + kRowsOf - 1) / kRowsOf), (uint32_t)l.splits);
+        linear_int4_rows_kernel<GROUP, ZEROS, OUT><<<grid, 512, 0, st>>>(a);
         if (l.splits > 1) {
             const int64_t quads = ((int64_t)a.n + 3) / 4 * a.m;
             linear_int4_join_kernel<OUT><<<(uint32_t)((quads + 255) / 256), 256, 0, st>>>(a);

@@ -16,7 +16,7 @@
 namespace ncm {
 namespace {
 
-constexpr int kOneRequests = 1024, kOneRows = 4096;
+constexpr int kOneRequests = 1024, kOneRows = 2048;
 
 struct PoolView {
     int32_t* free;

@@ -903,11 +903,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
 }
 
 // How many slices a row is cut into: 512 workgroups in all where that leaves a
-// slice 16384 logits.
+// slice 8192 logits, at most one per lane of ends_of.
+constexpr int64_t kMaxSlices = 64;
 int64_t slices_of(int64_t rows, int64_t vocab) {
-    return std::max<int64_t>(1, std::min<int64_t>((vocab + 16383) / 16384, 512 / std::max<int64_t>(rows, 1)));
+    return std::max<int64_t>(1, std::min<int64_t>({(vocab + 8191) / 8192, 512 / std::max<int64_t>(rows, 1), kMaxSlices}));
 }
-static_assert(kMaxVocab / 16384 <= 64, "ends_of has a lane per slice");
 int64_t row_bytes_of(int64_t slices, int64_t vocab) {
     const int64_t segments = vocab / 256 + 2;
     return (sizeof(RowRule) + sizeof(Ranges) + kBins * 12 + kList * 20 + slices * 8 + (segments + 1) * 4 + 15) / 16 * 16;
