@@ -479,12 +479,15 @@ struct Int4Layout {
     int splits;    // of the inputs
     size_t bytes;  // of the workspace
 };
-// 4096 x 4096, 16 rows: 7.4 us, 11.9 in the kernel of more rows; 4096 x 14336: 18.8,
-// 19.4; 28672 x 4096: 33, 28 (8 rows 28, 28).
-constexpr int kFewRows = 16;
+// A workgroup of the kernel of few rows reads all of x for 16 outputs, one of the
+// other for 128, which counts where there are many of both. us in the one and the
+// other, groups of 128: 4096 x 4096, 16 rows 7.3, 11.9; 16384 x 4096, 16 19.0, 16.8;
+// 28672 x 4096, 8 25.5, 22.7 (groups of 32: 27.7, 29.9), 12 29.8, 23.2 (31.6, 30.2);
+// 65536 x 4096, 2 31, 35, 5 43, 35 (52, 49); 128256 x 2048, 4 37, 37, 8 49, 37.
+bool few_rows(int64_t m, int64_t n) { return m <= 4 || (m <= 16 && m * n <= (1 << 18)); }
 
 Int4Layout int4_layout(int64_t m, int64_t n, int64_t k) {
-    Int4Layout l = {m <= kFewRows, 1, 0};
+    Int4Layout l = {few_rows(m, n), 1, 0};
     if (l.few) return l;
     // Workgroups of 128 outputs. Where they leave a CU without two, the inputs are
     // split, with at least four steps of 256 each; where they leave one without any,

@@ -398,7 +398,7 @@ def linear_int4(x, w: Int4Weight, bias=None, residual=None, out=None, out_mode: 
     if workspace is not None:
         pw, size = a.dev(workspace, "workspace", ("uint8",)), workspace.numel()
     a.done()
-    if workspace is None and m > 16:  # fewer rows need none
+    if workspace is None and m > 4:  # fewer rows need none
         need = C.c_size_t()
         check(lib().ncm_linear_int4_workspace(m, n, w.k, C.byref(need)), W)
         size = need.value
