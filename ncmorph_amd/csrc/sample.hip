@@ -902,11 +902,18 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     }
 }
 
-// How many slices a row is cut into: 512 workgroups in all where that leaves a
-// slice 8192 logits, at most one per lane of ends_of.
+// How many slices a row is cut into: up to 256 workgroups in all as long as a
+// slice has 8192 logits, up to 512 as long as it has 16384; at most one per lane
+// of ends_of. 128256 logits, top-k and top-p: one row 20.0 us, 21.2 in slices of
+// 16384; 24 rows 29.4 in slices of 8192 up to 512 workgroups, 25.5 in those of
+// 16384; without rules one row 19, 23. 150 rows of 151936: 48 us, 55 with up to 256
+// workgroups, 61 with up to 1024.
 constexpr int64_t kMaxSlices = 64;
 int64_t slices_of(int64_t rows, int64_t vocab) {
-    return std::max<int64_t>(1, std::min<int64_t>({(vocab + 8191) / 8192, 512 / std::max<int64_t>(rows, 1), kMaxSlices}));
+    rows = std::max<int64_t>(rows, 1);
+    const int64_t fine = std::min((vocab + 8191) / 8192, 256 / rows);
+    const int64_t coarse = std::min((vocab + 16383) / 16384, 512 / rows);
+    return std::clamp<int64_t>(std::max(fine, coarse), 1, kMaxSlices);
 }
 int64_t row_bytes_of(int64_t slices, int64_t vocab) {
     const int64_t segments = vocab / 256 + 2;
