@@ -752,7 +752,7 @@ typedef struct ncm_page_pool {
     int32_t* free;    /* [pages] */
     int32_t* count;   /* [1] pages on the stack */
     int32_t* refs;    /* [pages] table entries that hold a page */
-    int64_t* marks;   /* [pages] of a release's own use between calls INT64_MAX */
+    int64_t* marks;   /* [pages] a release's scratch, INT64_MAX before and after it */
     int64_t pages;    /* at most 2^30 */
 } ncm_page_pool_t;
 

@@ -17,6 +17,12 @@
 // bytes, and have a kernel of their own (kv_attention_prefix_kernel): wavefronts
 // of 32 pairs each, which share tiles of K and V as bf16 in LDS. It does the tiles
 // that every row of the group sees whole, the units above the prefix's rest.
+//
+// Measured, 32 heads over 8 of 128, 64 requests behind 8192 tokens, e4m3: 4.7 + 34.4
+// + 24 + 8.4 us for plan, prefix, own tokens and join; 256 requests behind 16000,
+// bf16: 4.6 + 135 (500 TFLOP/s) + 63 + 13. The prefix kernel spends
+// 4 us a tile of 64 tokens and 256 pairs, a third of it in the matrix cores: products
+// and softmax of one wavefront hardly overlap those of the other on its SIMD.
 #include "kv_attention.h"
 
 namespace ncm {
@@ -63,7 +69,14 @@ __device__ __forceinline__ int group_with(const SharedArgs& s, int r) {
 }
 
 constexpr int kWideTile = 64;   // tokens of a tile of the kernel for many pairs
-constexpr int kWidePairs = 48;  // of a group, from which on it has that kernel
+// Groups have that kernel from so many pairs each and (row, head) pairs x tokens x
+// head_dim in all on, the tokens those that the table has room for: it is a launch
+// more, whose workgroups start for 6 us. With it and without, head_dim 128, 8 K/V
+// heads, us: one group behind 8192 tokens and 64 own ones each, 64 pairs 43.6, 42.7,
+// 128 49, 56, 256 58, 87; with 512 own ones, 128 60, 50, 256 73, 69; behind 1024, 256
+// 43, 30. Eight groups behind 4096, 32 pairs 68, 59, 48 81, 94, 128 144, 175.
+constexpr int kWidePairs = 48;
+constexpr int64_t kWideWork = int64_t(5) << 28;
 
 // The plans, a wavefront per group, and behind them the floors, a thread per
 // request: once, instead of by every workgroup of the kernels that cut the units.
@@ -765,8 +778,11 @@ SharedLayout shared_layout(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int
     s.ro = pairs <= 16 * s.some ? 1 : 2;
     const int64_t per_group = pairs / std::max<int64_t>(1, std::min(n_groups, s.some));
     s.rp = std::max(s.ro, per_group <= 16 ? 1 : 2);
-    s.wide = n_groups == 0 || window || per_group < kWidePairs ? 0 : per_group <= 64 ? 2 : 4;
     const int64_t tokens = std::max<int64_t>(1, b.table_width * c.page_size);
+    const bool many = pairs * c.kv_heads * tokens * c.head_dim >= kWideWork && per_group >= kWidePairs;
+    // Two wavefronts of pairs where a group fills no more (eight groups of 48 pairs
+    // behind 4096 tokens: 81 us, 88 with four; of 128: 159, 144).
+    s.wide = n_groups == 0 || window || !many ? 0 : per_group <= 64 ? 2 : 4;
     // Eight wavefronts of pairs, each tile of the prefix brought once for 256, where
     // that leaves a workgroup tiles enough to be worth the state that it writes and
     // the join reads (1024 pairs behind 16000 tokens, 31 tiles each: 136 us, 158

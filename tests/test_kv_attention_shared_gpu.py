@@ -116,6 +116,71 @@ def test_windows(cuda, window, given):
     close(got, ref, mag)
 
 
+class Roomy(Shared):
+    """A table with room for so many tokens that groups of many pairs take the
+    kernel that is theirs, 2^31 (row, head) pairs x tokens x head_dim."""
+
+    def to(self, cuda):
+        kv, table, offsets, starts = super().to(cuda)
+        page = kv.k.shape[2]
+        width = 2 ** 31 // (self.rows * self.q_heads * kv.k.shape[3] * page) + 1
+        more = torch.full((table.shape[0], max(width, table.shape[1])), -1, dtype=I32, device=cuda)
+        more[:, :table.shape[1]] = table
+        return kv, more, offsets, starts
+
+    def run(self, cuda, q, q_heads, **kw):
+        self.q_heads = q_heads
+        return super().run(cuda, q, q_heads, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8, I8])
+@pytest.mark.parametrize("share", [16, 40])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_groups_of_many_pairs(cuda, case, share, dtype):
+    """Sixteen or forty heads a K/V head: 16 to 1040 pairs a group."""
+    new, before, groups, shared = CASES[case]
+    hd, page, heads = (64, 128)[case % 2], (16, 32, 64)[case % 3], 1 + case % 2
+    s = Roomy(60 + case, new, before, heads, hd, page, dtype, groups, shared, extra_rows=2)
+    q = queries(case, s.rows, heads * share * hd)
+    ref, mag = f64.attention(s, q, heads * share, f64.chain(new), chained=True)
+    close(s.run(cuda, q.to(cuda), heads * share), ref, mag)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_trees_of_many_pairs(cuda, hd, dtype):
+    new, before = [13, 7, 1, 30, 70], [200, 190, 300, 180, 181]
+    s = Roomy(71, new, before, 2, hd, 16, dtype, [0, 3, 5], [185, 170])
+    seen = f64.tree(72, new)
+    mask = f64.bits(seen, s.rows, 2)
+    q = queries(73, s.rows, 16 * hd)
+    ref, mag = f64.attention(s, q, 16, seen)
+    close(s.run(cuda, q.to(cuda), 16, tree_mask=mask.to(cuda)), ref, mag)
+
+
+def test_missing_pages_and_infinities_of_many_pairs(cuda):
+    """A page that is not there, and an infinity among the values, in a prefix
+    that the kernel for many pairs reads."""
+    new, before = [1] * 6, [200, 180, 190, 200, 185, 199]
+    s = Roomy(74, new, before, 1, 64, 16, BF16, [0, 6], [176])
+    s.table[0, 3] = -1                                    # tokens 48 .. 63
+    s.tokens[1][0][100, 0, 5] = math.inf
+    p = int(s.table[0, 100 // 16])
+    s.pages[1][p, 0, 100 % 16, 5] = math.inf
+    q = queries(75, s.rows, 24 * 64)
+    got = s.run(cuda, q.to(cuda), 24).float().cpu().view(6, 24, 64)
+    assert bool((got[..., 5] == math.inf).all())
+    for r, c in enumerate(before):
+        at = [i for i in range(c + 1) if not 48 <= i < 64]
+        there = lambda x: torch.cat([x[0][:176], x[r][176:]])[at][:, 0].double()  # noqa: E731
+        k, v = there(s.tokens[0]), there(s.tokens[1])
+        v[:, 5] = 0
+        w = torch.softmax(q[r].view(24, 64).double() @ k.t() / 8, 1)
+        rest = got[r].double().clone()
+        rest[:, 5] = 0
+        assert bool(((rest - w @ v).abs() <= f64.attention_bound(w @ v, w @ v.abs())).all())
+
+
 def test_missing_pages(cuda):
     """A page that the first request's row lacks is not there for the group; one
     that its own row lacks is not for a request."""
