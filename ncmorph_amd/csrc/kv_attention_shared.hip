@@ -76,7 +76,7 @@ constexpr int kWideTile = 64;   // tokens of a tile of the kernel for many pairs
 // 128 49, 56, 256 58, 87; with 512 own ones, 128 60, 50, 256 73, 69; behind 1024, 256
 // 43, 30. Eight groups behind 4096, 32 pairs 68, 59, 48 81, 94, 128 144, 175.
 constexpr int kWidePairs = 48;
-constexpr int64_t kWideWork = int64_t(5) << 28;
+constexpr double kWideWork = 5 * 0x1p28;
 
 // The plans, a wavefront per group, and behind them the floors, a thread per
 // request: once, instead of by every workgroup of the kernels that cut the units.
@@ -779,7 +779,7 @@ SharedLayout shared_layout(const ncm_kv_cache_t& c, const ncm_kv_batch_t& b, int
     const int64_t per_group = pairs / std::max<int64_t>(1, std::min(n_groups, s.some));
     s.rp = std::max(s.ro, per_group <= 16 ? 1 : 2);
     const int64_t tokens = std::max<int64_t>(1, b.table_width * c.page_size);
-    const bool many = pairs * c.kv_heads * tokens * c.head_dim >= kWideWork && per_group >= kWidePairs;
+    const bool many = (double)pairs * c.kv_heads * tokens * c.head_dim >= kWideWork && per_group >= kWidePairs;
     // Two wavefronts of pairs where a group fills no more (eight groups of 48 pairs
     // behind 4096 tokens: 81 us, 88 with four; of 128: 159, 144).
     s.wide = n_groups == 0 || window || !many ? 0 : per_group <= 64 ? 2 : 4;

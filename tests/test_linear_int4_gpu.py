@@ -105,6 +105,25 @@ def test_rounded(cuda, out_mode, m, n, k, group, zeros):
         check(into, y, e, k, group, out_mode)
 
 
+@pytest.mark.parametrize("m,n,k,group,zeros", [
+    (4, 52437, 136, 32, True), (5, 52437, 136, 64, False), (9, 29131, 264, 128, True),
+    (16, 16384, 520, 32, True), (16, 16385, 520, 32, True), (16, 16401, 2056, 128, False)])
+def test_few_rows_of_many_outputs(cuda, m, n, k, group, zeros):
+    """Either side of 2^18 outputs in all, where rows begin to be shared."""
+    codes, scales, z = weights(n + k, n, k, group, zeros)
+    g = torch.Generator().manual_seed(m)
+    x, bias = torch.randn(m, k, generator=g).to(BF16), torch.randn(n, generator=g).to(BF16)
+    residual = torch.randn(m, n, generator=g)
+    w = kernels.pack_int4(codes.to(cuda), scales.to(cuda), group,
+                          zeros=None if z is None else z.to(cuda))
+    y, e = exact(x, codes, scales, z, group, bias, residual)
+    out = residual.to(cuda)
+    got = kernels.linear_int4(x.to(cuda), w, bias=bias.to(cuda), residual=out, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    # Bias and residual round at the size of the terms, not of the sum.
+    check(got, y, e + 0.5 * (bias.abs() + residual.abs()).double(), k, group, "f32")
+
+
 @pytest.mark.parametrize("n", [31, 32])
 @pytest.mark.parametrize("out_mode", ["f32", "bf16"])
 def test_strides_and_alignment(cuda, n, out_mode):
