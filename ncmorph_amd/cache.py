@@ -200,7 +200,9 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
     groups (int32 [n + 1], ascending) and shared (int32 [n]): requests groups[g]
     .. groups[g + 1] - 1 hold the same first shared[g] tokens; of the tokens
     before a request's rows those are read through the page table's row of its
-    group's first request, once for the whole group."""
+    group's first request, once for the whole group. That takes three or four
+    launches where a call without groups takes two: it pays from about eight
+    requests behind 2000 common tokens on, or five behind 8000."""
     import torch
 
     W = "cache.attention"
