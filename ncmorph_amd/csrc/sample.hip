@@ -62,7 +62,7 @@ struct RowRule {
     double top_p;    // 1: off
     double min_p;    // 0: off
     double uniform;
-    float bins;      // bins a unit of logit, at least
+    float bins;      // bins a unit of half a logit, at least; above 0
     int top_k;       // 0: off
     int greedy;
     int request;     // -1: none
@@ -143,7 +143,7 @@ __device__ __forceinline__ RowRule rule_of(const SampleArgs& a, int row) {
     const float t = u.temperature ? u.temperature[r] : 1.0f;
     q.greedy = !(t > 0.0f);
     q.per = 32.0 * 1.44269504088896340736 / (double)fmaxf(t, 0x1p-96f);
-    q.bins = 64.0f / fmaxf(t, 0x1p-96f);
+    q.bins = 128.0f / fminf(fmaxf(t, 0x1p-96f), 3.40282347e38f);
     q.top_k = u.top_k ? max(u.top_k[r], 0) : 0;
     q.top_p = u.top_p ? (double)u.top_p[r] : 1.0;
     if (!(q.top_p < 1.0)) q.top_p = 1.0;
@@ -441,11 +441,16 @@ __device__ void pick_by_digits(const SampleArgs& a, int row, const RowRule& q, f
 }
 
 // The row's bins: at least 64 a unit of (max - x) / T, or 2047 over all its
-// values where these lie closer.
+// values where these lie closer. By halves, whose differences fp32 holds for any
+// two values; `per` is above 0, so that only what is no token gives a NaN.
 struct Bins {
+    float half;  // of the largest value
     float top, per;
+    // Bins from the largest value to x: negative for +infinity, which counts as
+    // the largest finite value.
+    __device__ __forceinline__ float distance(float x) const { return fmaf(x, -0.5f, half) * per; }
     __device__ __forceinline__ int of(float x) const {
-        return (int)fminf((top - x) * per, (float)(kBins - 1));
+        return (int)fminf(distance(x), (float)(kBins - 1));
     }
 };
 
@@ -456,14 +461,15 @@ __device__ __forceinline__ uint2 ends_of(const RowSpace& sp, int slices) {
     return make_uint2(wave_min_xor(e.x), ~wave_min_xor(~e.y));
 }
 __device__ __forceinline__ Bins bins_of(uint2 ends, const RowRule& q) {
-    const float top = key_value(ends.x), range = top - key_value(ends.y);
-    return {top, range > 0.0f ? fmaxf(q.bins, fminf(2047.0f / range, 0x1p100f)) : q.bins};
+    const float top = key_value(ends.x), half = 0.5f * top;
+    const float range = half - 0.5f * key_value(ends.y);
+    return {half, top, range > 0.0f ? fmaxf(q.bins, fminf(2047.0f / range, 0x1p101f)) : q.bins};
 }
 
 // The bin where weights fall below min_p.
 __device__ __forceinline__ int weak_bin(const Bins& bins, const RowRule& q) {
     // log(min_p) T of the logits' distance from the largest, in bins.
-    const double d = -log(q.min_p) * (32.0 * 1.44269504088896340736) / q.per * (double)bins.per;
+    const double d = -log(q.min_p) * (16.0 * 1.44269504088896340736) / q.per * (double)bins.per;
     return (int)fmin(d, (double)kBins);
 }
 
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_list_kernel(SampleArgs a) 
     // largest, is -infinity here.
     const float near = g.first() > 0 ? (float)g.first() : -INFINITY, far = (float)(g.last() + 1);
     auto ok = [&](float x) {
-        const float d = (bins.top - x) * bins.per;
+        const float d = bins.distance(x);
         return d >= near && (d < far || far == (float)kBins);
     };
     wanted.template each<BF16 ? 2 : 4>(logits, ok, [&](const auto& x, int first) {
