@@ -466,10 +466,12 @@ __device__ __forceinline__ Bins bins_of(uint2 ends, const RowRule& q) {
     return {half, top, range > 0.0f ? fmaxf(q.bins, fminf(2047.0f / range, 0x1p101f)) : q.bins};
 }
 
-// The bin where weights fall below min_p.
+// The bin where weights fall below the least that min_p keeps: as they are
+// rounded, those from half a unit below it on reach it.
 __device__ __forceinline__ int weak_bin(const Bins& bins, const RowRule& q) {
-    // log(min_p) T of the logits' distance from the largest, in bins.
-    const double d = -log(q.min_p) * (16.0 * 1.44269504088896340736) / q.per * (double)bins.per;
+    // The logarithm times T: the logits' distance from the largest, in bins.
+    const double border = ((double)least_weight(q) - 0.5) / kOne;
+    const double d = -log(border) * (16.0 * 1.44269504088896340736) / q.per * (double)bins.per;
     return (int)fmin(d, (double)kBins);
 }
 
@@ -737,7 +739,7 @@ __device__ __forceinline__ Ranges ranges_of(const Cumulative& c, const Bins& bin
     }
     g.strong = kBins, g.sure = 0, g.pad = 0;
     if (q.min_p > 0.0) {
-        // A bin to either side for the rounding of logarithm and bins.
+        // A bin to either side for the rounding of weights, logarithm and bins.
         const int b = weak_bin(bins, q);
         const int low = max(b - 1, 0), high = min(b + 1, kBins - 1);
         if (c.sums[low] < most) {

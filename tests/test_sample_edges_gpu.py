@@ -54,3 +54,16 @@ def test_largest_temperatures(cuda, least):
         compare(cuda, x, u, t=t)
         compare(cuda, x, u, t=t, m=np.full(4, least))
         compare(cuda, x, u, t=t, p=np.full(4, 0.8), m=np.full(4, least))
+
+
+def test_cuts_among_the_least_weights(cuda):
+    """min_p next to 2^-43, the unit of the weights: the tokens whose rounded
+    weights reach it, 900 to a row, drawn from the row's very end."""
+    g = np.random.default_rng(1)
+    x = -np.concatenate([np.full((3, 900), 30.2), g.uniform(27, 30.4, (45, 900))]).astype(np.float32)
+    x[:, 450] = 0
+    m = np.concatenate([[1e-13, 1.1368e-13, 1.14e-13], 10 ** g.uniform(-14, -11.5, 45)])
+    for back in (0, 40, 400):
+        u = np.full(48, 1 - (1 + back) * 2.0 ** -44)
+        compare(cuda, torch.from_numpy(x), u, m=m, wide=True)
+        compare(cuda, torch.from_numpy(x), u, m=m, k=np.full(48, 901), wide=True)
