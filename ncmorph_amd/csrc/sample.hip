@@ -210,12 +210,20 @@ __device__ __forceinline__ uint64_t weight_of(float x, float top, double per, co
     return (uint64_t)__double_as_longlong(fma(p, scale, 0x1p52)) & ((uint64_t(1) << 52) - 1);
 }
 
-// floor(f * total) and whether it is more than that; f in [0, 1].
+// floor(f * total) and whether it is more than that, exactly: the product of f's 53
+// bits, f = m 2^-s, and the total's 64. f in [0, 1].
 __device__ __forceinline__ uint64_t share_of(double f, uint64_t total, bool& more) {
-    const uint64_t m = (uint64_t)(f * 0x1p53);  // f < 1 has no bit behind but below 2^-53
+    const uint64_t bits = (uint64_t)__double_as_longlong(f), e = (bits >> 52) & 0x7FF;
+    const uint64_t m = (bits & ((uint64_t(1) << 52) - 1)) | (e ? uint64_t(1) << 52 : 0);
+    const int s = 1075 - max((int)e, 1);  // 52 at least
     const uint64_t lo = m * total, hi = __umul64hi(m, total);
-    more = (lo & ((uint64_t(1) << 53) - 1)) != 0 || (double)m != f * 0x1p53;
-    return (hi << 11) | (lo >> 53);
+    if (s < 64) {
+        more = (lo & ((uint64_t(1) << s) - 1)) != 0;
+        return (hi << (64 - s)) | (lo >> s);
+    }
+    const int t = min(s - 64, 63);  // hi is below 2^53
+    more = lo != 0 || (hi & ((uint64_t(1) << t) - 1)) != 0;
+    return hi >> t;
 }
 
 // The cumulative weight at which a part p of `total` is reached, and a draw's.

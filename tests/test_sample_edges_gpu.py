@@ -67,3 +67,13 @@ def test_cuts_among_the_least_weights(cuda):
         u = np.full(48, 1 - (1 + back) * 2.0 ** -44)
         compare(cuda, torch.from_numpy(x), u, m=m, wide=True)
         compare(cuda, torch.from_numpy(x), u, m=m, k=np.full(48, 901), wide=True)
+
+
+@pytest.mark.parametrize("n", [3, 7, 11, 100, 999, 40000])
+def test_draws_a_step_from_a_border(cuda, n):
+    """n equal tokens and 64-bit numbers next to k / n, whose last bits are below
+    2^-53 where k / n is small."""
+    edge = np.unique(np.arange(n) * 64 // max(n, 64) / n) if n > 200 else np.arange(n) / n
+    u = np.concatenate([edge, np.nextafter(edge, 1), np.maximum(np.nextafter(edge, 0), 0),
+                        edge[1:] * (1 + 2.0 ** -50), edge[1:] * 2.0 ** -20])
+    compare(cuda, torch.zeros(1, n).repeat(len(u), 1), u, wide=True)
