@@ -767,6 +767,7 @@ typedef struct ncm_page_pool {
 /* Request r holds, besides sources[r], the pages that the first tokens[r] tokens
  * of that request's sequence fill (tokens[r] / page_size, rounded down: the
  * next page of either is its own, and what the source has there is not copied).
+ * Neither goes on from inside a page that both hold (ncm_pages_extend_dev).
  * A source that is r or no request leaves r as it was; what row r's first
  * entries held before is not released. A row must not be a source and get pages
  * in one call. */
@@ -783,8 +784,14 @@ int ncm_pages_share_dev(ncm_ctx_t* ctx, const ncm_page_pool_t* pool, int32_t* pa
  * or -1 where that token is not there. Rows of no request get position 0 and
  * slot -1. The pages that the tokens begin are taken from the pool in the order
  * of requests and tokens; missing[0] is how many the pool did not have (their
- * entries become -1: those tokens are not there). pool NULL: no page is taken,
- * the table has them already. workspace: int32 [requests + 2]. */
+ * entries become -1: those tokens are not there). A request that begins inside a
+ * page with more than one holder (one cut back into what it shares) would write
+ * over what the others read: its tokens of that page have slot -1 and the page
+ * counts as missing. The entry stays, and ncm_kv_write_dev goes by the table: a
+ * step is written where missing[0] is 0, otherwise the request is cut to whole
+ * pages first, and the tokens behind these are added again. pool NULL: no page is
+ * taken, the table has them already, and holders are not looked at. workspace:
+ * int32 [requests + 2]. */
 int ncm_pages_extend_dev(ncm_ctx_t* ctx, const ncm_page_pool_t* pool, const int32_t* added,
                          const int32_t* starts, int32_t* page_table, int64_t requests,
                          int64_t table_width, int64_t table_stride, int page_size, int64_t rows,
@@ -795,8 +802,9 @@ int ncm_pages_extend_dev(ncm_ctx_t* ctx, const ncm_page_pool_t* pool, const int3
  * less): the pages behind are released, their entries become -1. Pages without
  * a holder go back to the stack in the order of requests and tokens, the first
  * on top: a release of what an extension took leaves the pool as it was.
- * Entries of a page beyond its holders release nothing. workspace: int32
- * [requests + 2]. */
+ * Entries of a page beyond its holders release nothing. A sequence cut inside a
+ * page that others hold too keeps the page, but cannot go on there: the next
+ * ncm_pages_extend_dev says so. workspace: int32 [requests + 2]. */
 int ncm_pages_release_dev(ncm_ctx_t* ctx, const ncm_page_pool_t* pool, int32_t* page_table,
                           const int32_t* lens, const int32_t* keep, int64_t requests,
                           int64_t table_width, int64_t table_stride, int page_size,

@@ -308,8 +308,9 @@ def share(pool: PagePool, page_table, sources, tokens, page_size: int, ctx=None)
     """Lets request r hold the whole pages of the first tokens[r] tokens of
     request sources[r] (int32 [requests]; its own number or -1: nothing) besides
     that one, in the first entries of its row of page_table, which must hold no
-    pages. tokens[r] // page_size pages; r's sequence goes on behind them. A row
-    cannot be a source and get pages in one call."""
+    pages. tokens[r] // page_size pages; r's sequence goes on behind them, and so
+    does the source's (`extend`). A row cannot be a source and get pages in one
+    call."""
     a = _ck.Args("cache.share")
     got, pt, n, width, stride = _tables(a, pool, page_table, (sources, tokens),
                                         ("sources", "tokens"))
@@ -329,7 +330,12 @@ def extend(pool, page_table, new, starts, rows: int, page_size: int, tree_mask=N
     index), slots (int64 [rows]: page * page_size + token % page_size; -1 where
     the token is not there) and missing (int32 [1]: pages that the pool did not
     have; their tokens are not there). Rows of no request get position 0 and
-    slot -1. pool None: page_table has every page already."""
+    slot -1. A request that begins inside a page with more than one holder (cut
+    back into what it shares) would write over what the others read: its tokens
+    of that page have slot -1, and the page counts in missing. `write` goes by
+    the table, so write where missing is 0; otherwise `release` the request to
+    whole pages and add the tokens behind these again. pool None: page_table has
+    every page already, and holders are not looked at."""
     import torch
 
     W = "cache.extend"
@@ -364,7 +370,8 @@ def release(pool: PagePool, page_table, lens, keep, page_size: int, ctx=None):
     where that is not less): page_table's entries behind become -1, and pages
     that no table holds any more go back to the pool. Drafted tokens that were
     rejected: keep the accepted; finished requests: keep 0. What an `extend` took
-    leaves the pool, released, as it was before."""
+    leaves the pool, released, as it was before. A page cut in part stays with
+    the request, which goes on in it only where nobody else holds it (`extend`)."""
     import torch
 
     a = _ck.Args("cache.release")

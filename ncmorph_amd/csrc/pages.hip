@@ -96,10 +96,13 @@ __device__ __forceinline__ int find(const int32_t* at, int requests, int x) {
     return lo;
 }
 
-__device__ __forceinline__ void fill_row(const ExtendArgs& a, const int32_t* offsets,
+// Whether the row is a request's first and begins inside a page with more than one
+// holder: what it would write there others read.
+__device__ __forceinline__ bool fill_row(const ExtendArgs& a, const int32_t* offsets,
                                          const int32_t* ahead, int base, int row) {
     int position = 0;
     int64_t slot = -1;
+    bool refused = false;
     if (row < offsets[a.p.requests]) {
         const int r = find(offsets, a.p.requests, row), i = row - offsets[r];
         const int n = offsets[r + 1] - offsets[r], start = tokens_of(a.starts[r]);
@@ -120,12 +123,15 @@ __device__ __forceinline__ void fill_row(const ExtendArgs& a, const int32_t* off
             const bool fresh = a.p.pool.free && page >= first;
             const int id = fresh ? taken(a.p.pool, base, ahead[r] + (int)page - first)
                                  : a.p.table[r * a.p.stride + page];
-            if (id >= 0 && (!a.p.pool.free || id < a.p.pool.pages))
-                slot = ((int64_t)id << a.p.log2) + (t & ((1 << a.p.log2) - 1));
+            const bool there = id >= 0 && (!a.p.pool.free || id < a.p.pool.pages);
+            const bool others = there && a.p.pool.free && !fresh && a.p.pool.refs[id] > 1;
+            if (there && !others) slot = ((int64_t)id << a.p.log2) + (t & ((1 << a.p.log2) - 1));
+            refused = others && i == 0;
         }
     }
     a.positions[row] = position;
     a.slots[row] = slot;
+    return refused;
 }
 
 __device__ __forceinline__ void fill_page(const ExtendArgs& a, const int32_t* ahead, int base,
@@ -142,6 +148,7 @@ template <bool ONE>
 __global__ __launch_bounds__(1024) void extend_scan_kernel(ExtendArgs a) {
     __shared__ int64_t waves[16];
     __shared__ int32_t near_offsets[ONE ? kOneRequests + 1 : 1], near_ahead[ONE ? kOneRequests + 1 : 1];
+    __shared__ int refused;
     const int requests = a.p.requests, per = (requests + 1023) / 1024;
     const int r0 = min((int)threadIdx.x * per, requests), r1 = min(r0 + per, requests);
     int32_t* ahead = ONE ? near_ahead : a.space;
@@ -177,6 +184,7 @@ __global__ __launch_bounds__(1024) void extend_scan_kernel(ExtendArgs a) {
         if (ONE) near_offsets[requests] = clipped(all);
         ahead[requests] = (int)taken_in_all;
         if (!ONE) a.space[requests + 1] = base;
+        if (ONE) refused = 0;
         *a.missing = (int)max(taken_in_all - base, (int64_t)0);
     }
     __syncthreads();
@@ -184,8 +192,11 @@ __global__ __launch_bounds__(1024) void extend_scan_kernel(ExtendArgs a) {
     if (threadIdx.x == 0 && a.p.pool.free) *a.p.pool.count = (int)max(base - taken_in_all, (int64_t)0);
     if constexpr (ONE) {
         for (int row = threadIdx.x; row < a.rows; row += 1024)
-            fill_row(a, near_offsets, near_ahead, base, row);
+            if (fill_row(a, near_offsets, near_ahead, base, row)) atomicAdd(&refused, 1);
         for (int e = threadIdx.x; e < (int)taken_in_all; e += 1024) fill_page(a, near_ahead, base, e);
+        __syncthreads();
+        if (threadIdx.x == 0 && refused)
+            *a.missing = (int)max(taken_in_all - base, (int64_t)0) + refused;
     }
 }
 
@@ -193,7 +204,7 @@ __global__ __launch_bounds__(256) void extend_fill_kernel(ExtendArgs a, int row_
     const int base = a.space[a.p.requests + 1];
     const int i = (int)(blockIdx.x * 256 + threadIdx.x);
     if ((int)blockIdx.x < row_blocks) {
-        if (i < a.rows) fill_row(a, a.offsets, a.space, base, i);
+        if (i < a.rows && fill_row(a, a.offsets, a.space, base, i)) atomicAdd(a.missing, 1);
     } else if (i - row_blocks * 256 < a.space[a.p.requests]) {
         fill_page(a, a.space, base, i - row_blocks * 256);
     }
