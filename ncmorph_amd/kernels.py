@@ -307,7 +307,7 @@ class Int4Weight:
     """A weight matrix [n, k] in 4-bit codes, packed for linear_int4 (pack_int4
     makes it). It keeps the addresses of its two buffers."""
 
-    __slots__ = ("codes", "scales", "n", "k", "group", "struct", "named")
+    __slots__ = ("codes", "scales", "n", "k", "group", "struct", "named", "plain_rows")
 
     def __init__(self, codes, scales, n: int, k: int, group: int, has_zeros: bool):
         a = _ck.Args("Int4Weight")
@@ -318,6 +318,15 @@ class Int4Weight:
         self.codes, self.scales, self.n, self.k, self.group = codes, scales, n, k, group
         self.struct = _Int4(pc, ps, n, k, group, int(has_zeros))
         self.named = tuple(a.seen)
+        # So many rows need no workspace, as the library says (64 at most are
+        # asked for): the shortest calls need not ask again.
+        self.plain_rows = 0
+        need = C.c_size_t()
+        while self.plain_rows < 64:
+            check(lib().ncm_linear_int4_workspace(self.plain_rows + 1, n, k, C.byref(need)), a.where)
+            if need.value:
+                break
+            self.plain_rows += 1
 
 
 def pack_int4(codes, scales, group: int, zeros=None, ctx=None) -> Int4Weight:
@@ -398,7 +407,7 @@ def linear_int4(x, w: Int4Weight, bias=None, residual=None, out=None, out_mode: 
     if workspace is not None:
         pw, size = a.dev(workspace, "workspace", ("uint8",)), workspace.numel()
     a.done()
-    if workspace is None and m > 4:  # fewer rows need none
+    if workspace is None and m > w.plain_rows:
         need = C.c_size_t()
         check(lib().ncm_linear_int4_workspace(m, n, w.k, C.byref(need)), W)
         size = need.value
