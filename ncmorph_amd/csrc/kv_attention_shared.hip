@@ -53,8 +53,9 @@ struct SharedArgs {
     int* counts;                  // units there are: the groups', the requests', the wide ones
     int* unit_base;               // of a group
     int4* joins;                  // {first workgroup, parts, segment, unit of the segment}
-    int64_t whole_prefix, whole_own;  // rows of the parts of units in one run
-    int64_t prefix_cut;               // rows of the parts of groups' units in several
+    // Rows of the parts of units in one run. Those of the others begin at row 0: two
+    // of 16 RP rows a workgroup, of groups' units and requests' alike.
+    int64_t whole_prefix, whole_own;
 };
 
 // The group of request r, or -1.
