@@ -733,7 +733,8 @@ int ncm_kv_attention_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,
  * (before its rows, that is) is read through the page table's row of the group's
  * first request, once for all of them. A request of no group, of a group of one
  * or with shared[g] <= 0 reads its own row alone. All else is as there; the sums
- * are made in another order. */
+ * are made in another order. The host's sizes, batch's table_width among them,
+ * decide which kernels run: one no wider than the longest sequence is best. */
 int ncm_kv_attention_shared_workspace(const ncm_kv_cache_t* cache, const ncm_kv_batch_t* batch,
                                       int64_t n_groups, int q_heads, size_t* bytes);
 int ncm_kv_attention_shared_dev(ncm_ctx_t* ctx, const ncm_kv_cache_t* cache,

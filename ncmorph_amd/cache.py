@@ -201,8 +201,12 @@ def attention(q, kv: KvCache, q_heads: int, page_table, offsets, starts, tree_ma
     .. groups[g + 1] - 1 hold the same first shared[g] tokens; of the tokens
     before a request's rows those are read through the page table's row of its
     group's first request, once for the whole group. That takes three or four
-    launches where a call without groups takes two: it pays from about eight
-    requests behind 2000 common tokens on, or five behind 8000."""
+    launches where a call without groups takes two: with few tokens of their own
+    it pays from about twelve requests behind 1000 common tokens on, five behind
+    2000 to 8000, four behind 16000; with 500 of their own from sixteen behind
+    2000, six behind 8000. The sizes that the host knows, page_table's width
+    among them, choose the kernels: columns of a wide table, no more than the
+    longest request has, take less time than all of it."""
     import torch
 
     W = "cache.attention"

@@ -18,9 +18,9 @@
 // of 32 pairs each, which share tiles of K and V as bf16 in LDS. It does the tiles
 // that every row of the group sees whole, the units above the prefix's rest.
 //
-// Measured, 32 heads over 8 of 128, 64 requests behind 8192 tokens, e4m3: 4.7 + 34.4
-// + 24 + 8.4 us for plan, prefix, own tokens and join; 256 requests behind 16000,
-// bf16: 4.6 + 135 (500 TFLOP/s) + 63 + 13. The prefix kernel spends
+// Measured, 32 heads over 8 of 128, 64 requests behind 8192 tokens, e4m3: 4.8 + 34.6
+// + 24 + 8.5 us for plan, prefix, own tokens and join; 256 requests behind 16000,
+// bf16: 4.7 + 131 (510 TFLOP/s) + 62 + 13. The prefix kernel spends
 // 4 us a tile of 64 tokens and 256 pairs, a third of it in the matrix cores: products
 // and softmax of one wavefront hardly overlap those of the other on its SIMD.
 #include "kv_attention.h"
@@ -75,7 +75,10 @@ constexpr int kWideTile = 64;   // tokens of a tile of the kernel for many pairs
 // more, whose workgroups start for 6 us. With it and without, head_dim 128, 8 K/V
 // heads, us: one group behind 8192 tokens and 64 own ones each, 64 pairs 43.6, 42.7,
 // 128 49, 56, 256 58, 87; with 512 own ones, 128 60, 50, 256 73, 69; behind 1024, 256
-// 43, 30. Eight groups behind 4096, 32 pairs 68, 59, 48 81, 94, 128 144, 175.
+// 43, 30. Eight groups behind 4096, 32 pairs 68, 59, 48 81, 94, 128 144, 175. The
+// prefixes' lengths are on the device, the table's width stands for them: in a table
+// much wider than the step a short prefix takes this kernel too (one group behind
+// 1024, 64 requests, 256 pairs: 29 us in a table of 1100 tokens, 49 in one of 32768).
 constexpr int kWidePairs = 48;
 constexpr double kWideWork = 5 * 0x1p28;
 

@@ -15,10 +15,11 @@
 // of the lanes: 16 outputs and 128 inputs are 1 KB, a wavefront's 16-byte load.
 // A workgroup makes 16 outputs of up to 16 rows, its eight wavefronts taking
 // every eighth 128 inputs; their sums are added in order through LDS. 28672 x 4096
-// in groups of 128, weights from HBM: one row 16.8 us (3.6 TB/s), 8 rows 28, 16 33;
-// in groups of 32 with zeros, a scale and two fp32 operations an output, row and
-// group: 20 and 35. More rows (linear_int4_rows_kernel) are bound by the unpacking
-// and the group sums, repeated for every 32 rows: 256 rows 125 us (480 TFLOP/s).
+// in groups of 128, weights from HBM: one row 17 us (3.6 TB/s), 4 rows 21, 8 26; in
+// groups of 32 with zeros, a scale and two fp32 operations an output, row and group:
+// 19, 24 and 27. More rows (linear_int4_rows_kernel; here from 10 on) are bound by the
+// unpacking and the group sums, repeated for every 32 rows: 16 rows 24 and 30 us, 256
+// rows 112 (540 TFLOP/s) and 149.
 #include "step.h"
 
 namespace ncm {
@@ -202,9 +203,9 @@ __global__ __launch_bounds__(64 * kWaves) void linear_int4_kernel(Int4Args a) {
 // four outputs' without 64 registers for them. 16-byte chunk c of row r of x is at
 // chunk c ^ (r % 16), so that an operand's sixteen rows fall into different banks.
 // 32 rows leave room for two workgroups a CU, of which one computes while the other
-// waits: 28672 x 4096 in groups of 128, 256 rows 125 us, 136 with 64 rows a
-// workgroup and half the reads of the weights; 96 rows 57, 68; 4096 x 14336,
-// 128 rows 38, 38.5.
+// waits: 28672 x 4096 in groups of 128, 256 rows 112 us, 136 with 64 rows a
+// workgroup and half the reads of the weights; 96 rows 55, 67; 4096 x 14336,
+// 128 rows 36.5, 43.
 constexpr int kRowsOf = 32;
 template <int GROUP, bool ZEROS, int OUT>
 __global__ __launch_bounds__(512, 2) void linear_int4_rows_kernel(Int4Args a) {

@@ -9,9 +9,9 @@
 // follows, down to the stack's order.
 //
 // A few bytes a row and a page: bound by the launches and the chain of loads in
-// each. 48 requests: extend 6.3 us, release 2.8 + 3.0 + 3.2; 200 prompts of about
-// 500 tokens behind 2000 shared ones: share 7.0, extend 4.9 + 4.7, release 9.4 +
-// 3.8 + 4.6.
+// each. 48 requests: extend 6.6 us, release 2.8 + 3.0 + 3.2; 200 prompts of about
+// 500 tokens behind 2000 shared ones: share 7.1, extend 5.0 + 4.8, release 9.1 +
+// 3.3 + 4.9.
 //
 // Up to 1024 requests and 2048 rows are extended by one workgroup in one launch
 // (1024 requests of one row: 6.6 us, 8.8 in two; 16 of 128: 5.9, 6.9), more by one

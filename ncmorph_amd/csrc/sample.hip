@@ -19,15 +19,23 @@
 //      their tokens into a list, from the segments that can have some;
 //   4. each listed token's cumulative weight, exactly, from its bin's and the
 //      listed tokens of its bin; cuts and draw are minima over these.
-// Bound by the four launches' chains of loads for few rows: 4.6 + 6.6 + 8.1 + 6.0 us
-// for 4 rows of 128256 with all rules. For many by the operations of step 2 (an exp in
-// 64 bits and two LDS atomics a token) and the two later reads, which L2 serves in
-// part: 150 rows of 151936, 19 (4.9 TB/s) + 31 + 21 + 7.
+// Bound by the four launches' chains of loads for few rows: 4.6 + 6.5 + 8.4 + 6.0 us
+// for 4 rows of 128256 with all rules in use. For many by the operations of step 2 (an
+// exp in 64 bits and two LDS atomics a token) and the two later reads, which L2 serves
+// in part: 151 rows of 151936, half of the logits masked, all rules in use by some rows,
+// 19 (4.9 TB/s) + 32 + 22 + 7. Step 4 compares every pair of listed tokens: the same
+// rows where one lists 515 take 127 us in place of 78.
 //
-// A row that lists more than 1024 (many equal logits) is done digit by digit
-// of the token's 52-bit place in the order (32 bits of the logit, 20 of the id):
-// sums of the tokens by their next digit, then the digit where the target is
-// passed.
+// A row that lists more than 1024 is done digit by digit of the token's 52-bit place
+// in the order (32 bits of the logit, 20 of the id): sums of the tokens by their next
+// digit, then the digit where the target is passed. One workgroup reads the row once
+// and five times a cut and the draw for that. It happens where the tokens of a bin are
+// many: bf16 logits away from zero (about 20 they are 1/8 apart), equal logits, and a
+// flat row whose range a finite mask stretches, so that its bins are 1/64 T wide. One
+// row of 128256, us, without rules and with top_p 0.95: bf16 about 20 with a standard
+// deviation of 2, 484 and 892 (64 rows 517 and 935), about 0 with top_p 46; fp32 with a
+// deviation of 1 and some logits at -1e9, with top_p 705, without those 51; all equal
+// 1010 and 1925. top_k keeps the lists short (50 and the mask: 21).
 #include "step.h"
 
 namespace ncm {
@@ -925,10 +933,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
 
 // How many slices a row is cut into: up to 256 workgroups in all as long as a
 // slice has 8192 logits, up to 512 as long as it has 16384; at most one per lane
-// of ends_of. 128256 logits, top-k and top-p: one row 20.0 us, 21.2 in slices of
-// 16384; 24 rows 29.4 in slices of 8192 up to 512 workgroups, 25.5 in those of
-// 16384; without rules one row 19, 23. 150 rows of 151936: 48 us, 55 with up to 256
-// workgroups, 61 with up to 1024.
+// of ends_of. In a graph, top-k 64 and top-p 0.95: one row of 128256 20.6 us, 22.1 in
+// slices of 16384; 24 rows 25.7, 29.4 in slices of 8192 up to 512 workgroups; 150 rows
+// of 151936 48.9, 54.9 with up to 256 workgroups, 61.5 with up to 1024. Without rules
+// one row 19.4, 23.0; 150 rows 83, 124 and 85.
 constexpr int64_t kMaxSlices = 64;
 int64_t slices_of(int64_t rows, int64_t vocab) {
     rows = std::max<int64_t>(rows, 1);
